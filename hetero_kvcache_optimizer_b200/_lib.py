@@ -27,7 +27,7 @@ DT_F16, DT_BF16, DT_F32 = 0, 1, 2
 FMT_REF, FMT_FP16MIN = 0, 1
 ROLE_K, ROLE_V = 0, 1
 
-DEVERR_TIMEOUT, DEVERR_BAD_PAGE, DEVERR_CAPACITY = 1, 2, 4
+DEVERR_TIMEOUT, DEVERR_BAD_PAGE, DEVERR_CAPACITY, DEVERR_BAD_POSITION = 1, 2, 4, 8
 APPEND_EARLY = 1  # HKV_APPEND_EARLY
 
 c_i32, c_i64, c_u32, c_f32, c_vp, c_sz = (ctypes.c_int32, ctypes.c_int64, ctypes.c_uint32,
@@ -47,6 +47,12 @@ class HkvDenseKV(ctypes.Structure):
                 ("lengths", c_vp), ("len", c_i32), ("reserved", c_i32)]
 
 
+class HkvRows(ctypes.Structure):
+    _fields_ = [("data", c_vp), ("stride_b", c_i64), ("stride_h", c_i64), ("stride_t", c_i64),
+                ("heads", c_i32), ("reserved", c_i32)]
+
+
+P_rows = ctypes.POINTER(HkvRows)
 P_store = ctypes.POINTER(HkvInt4Store)
 P_dense = ctypes.POINTER(HkvDenseKV)
 
@@ -99,6 +105,12 @@ SIGNATURES = {
     "hkv_event_wait": (c_i32, [c_vp, c_i64]),
     "hkv_qk_scores_flat": (c_i32, [c_vp, c_i32, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32, c_vp, c_vp]),
     "hkv_selftest_bounded_wait": (c_i32, [c_i64, c_i32, c_vp]),
+    "hkv_norm_rope": (c_i32, [P_rows, P_rows, P_rows, P_rows, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, c_i32, c_f32,
+                              c_vp, c_i32, c_i64, c_i64, c_vp, c_i64, c_i32, c_i32, c_i32, c_vp]),
+    "hkv_pages_workspace_bytes": (c_sz, [P_store, c_i32, c_i32]),
+    "hkv_pages_fork": (c_i32, [P_store, c_i32, c_i32, c_vp, c_vp, c_vp, c_sz, c_vp]),
+    "hkv_pages_reserve": (c_i32, [P_store, c_i32, c_i32, c_vp, c_i32, c_vp, c_vp, c_sz, c_vp]),
+    "hkv_pages_compact": (c_i32, [P_store, c_i32, c_i32, P_store, c_vp, c_vp, c_sz, c_vp]),
 }
 
 _lib = None

@@ -13,6 +13,8 @@
 #include "hkv_quant.cuh"   // before the decode kernel: its fused append quantises with it
 #include "hkv_decode.cuh"
 #include "hkv_prefill.cuh"
+#include "hkv_norm_rope.cuh"
+#include "hkv_pages.cuh"
 
 #define HKV_VERSION 100
 
@@ -48,11 +50,12 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // drain: 4.82 -> 4.68 ms for config 2's 896 chunk launches); the append kernel,
 // whose blocks would wait resident beside the decode kernel's, measured slower
 // with it (2.608 ms) and launches normally. HKV_PDL (bit mask: 1 decode,
-// 2 append, 4 quantise-pack; default 5) overrides this for experiments.
+// 2 append, 4 quantise-pack, 8 norm + rotation and page operations; default 13)
+// overrides this for experiments.
 bool pdl_enabled(int which) {
   static const int mask = [] {
     const char* e = std::getenv("HKV_PDL");
-    return e ? std::atoi(e) : 5;
+    return e ? std::atoi(e) : 13;
   }();
   return (mask & which) != 0;
 }
@@ -553,6 +556,23 @@ hkv_status launch_prefill_f(const hkv::PrefillParams& p, int group, cudaStream_t
   return HKV_ERR_UNSUPPORTED;
 }
 
+// --------------------------------------------------------------------------- norm + rotation
+template <typename T, int MODE, int kHeads>
+cudaError_t launch_norm_rope(hkv::NormRopeParams& p, cudaStream_t st) {
+  for (int i = 0; i < 2; ++i) p.chunks[i] = cdiv(p.H[i], kHeads);
+  const int64_t items = (int64_t)p.B * p.T * (p.chunks[0] + p.chunks[1]);
+  const int64_t grid = (items + hkv::kNrThreads / 32 - 1) / (hkv::kNrThreads / 32);
+  return launch_pdl(8, hkv::norm_rope_kernel<T, MODE, kHeads>, dim3((unsigned)grid), dim3(hkv::kNrThreads), 0, st, p);
+}
+
+template <typename T>
+cudaError_t launch_norm_rope_t(hkv::NormRopeParams& p, int mode, cudaStream_t st) {
+  // Two heads a warp while that leaves warps to spare (a decode step), else eight.
+  const bool few = (int64_t)p.B * p.T * (p.H[0] + p.H[1]) <= (int64_t)device_sms() * 64;
+#define HKV_NR(MODE) (few ? launch_norm_rope<T, MODE, 2>(p, st) : launch_norm_rope<T, MODE, 8>(p, st))
+  return mode == hkv::kNrLane ? HKV_NR(hkv::kNrLane) : mode == hkv::kNrAdjacent ? HKV_NR(hkv::kNrAdjacent) : HKV_NR(hkv::kNrAny);
+#undef HKV_NR
+}
 }  // namespace
 
 // =========================================================================== C ABI
@@ -1226,6 +1246,201 @@ hkv_status hkv_event_wait(hkv_event_t ev, int64_t timeout_us) {
     if (el.count() >= timeout_us) return HKV_ERR_TIMEOUT;
     std::this_thread::sleep_for(std::chrono::microseconds(20));
   }
+}
+
+// --------------------------------------------------------------------------- norm + rotation
+hkv_status hkv_norm_rope(const hkv_rows* q, const hkv_rows* k, const hkv_rows* q_out, const hkv_rows* k_out,
+                         int32_t dtype, int32_t B, int32_t T, int32_t D, const void* q_weight,
+                         const void* k_weight, int32_t weight_dtype, float eps, const void* positions,
+                         int32_t position_bits, int64_t pos_stride_b, int64_t pos_stride_t, const float* table,
+                         int64_t table_stride, int32_t max_pos, int32_t rot, int32_t adjacent,
+                         hkv_stream_t stream) {
+  if (B <= 0 || T < 0 || (!q && !k) || !q != !q_out || !k != !k_out) return HKV_ERR_ARG;
+  if (D != HKV_D) return HKV_ERR_UNSUPPORTED;
+  if (dtype != HKV_DT_F16 && dtype != HKV_DT_BF16) return HKV_ERR_ARG;
+  if ((q_weight || k_weight) && (weight_dtype < HKV_DT_F16 || weight_dtype > HKV_DT_F32)) return HKV_ERR_ARG;
+  if (!(eps >= 0.f) || !std::isfinite(eps)) return HKV_ERR_ARG;
+  if (table) {
+    if (!positions || (position_bits != 32 && position_bits != 64)) return HKV_ERR_ARG;
+    if (rot < 2 || rot > HKV_D || rot % 2 || max_pos <= 0 || table_stride < rot) return HKV_ERR_ARG;
+  } else if (rot != 0) {
+    return HKV_ERR_ARG;
+  }
+  hkv::NormRopeParams p;
+  std::memset(&p, 0, sizeof(p));
+  const hkv_rows* in[2] = {q, k};
+  const hkv_rows* out[2] = {q_out, k_out};
+  const void* w[2] = {q_weight, k_weight};
+  for (int i = 0; i < 2; ++i) {
+    if (!in[i]) continue;
+    const hkv_rows &x = *in[i], &y = *out[i];
+    if (!x.data || !y.data || x.heads <= 0 || x.heads != y.heads) return HKV_ERR_ARG;
+    if ((reinterpret_cast<uintptr_t>(x.data) | reinterpret_cast<uintptr_t>(y.data)) & 1u) return HKV_ERR_ARG;
+    if ((B > 1 && !y.stride_b) || (y.heads > 1 && !y.stride_h) || (T > 1 && !y.stride_t)) return HKV_ERR_ARG;
+    p.x[i] = x.data;
+    p.y[i] = y.data;
+    p.w[i] = w[i];
+    p.w_dtype[i] = weight_dtype;
+    p.H[i] = x.heads;
+    const int64_t xs[3] = {x.stride_b, x.stride_h, x.stride_t}, ys[3] = {y.stride_b, y.stride_h, y.stride_t};
+    p.vec[i] = aligned16(x.data) && aligned16(y.data);
+    for (int j = 0; j < 3; ++j) {
+      p.xs[i][j] = xs[j];
+      p.ys[i][j] = ys[j];
+      p.vec[i] = p.vec[i] && xs[j] % 8 == 0 && ys[j] % 8 == 0;
+    }
+  }
+  if ((int64_t)B * T * (p.H[0] + p.H[1]) >= (int64_t(1) << 33)) return HKV_ERR_UNSUPPORTED;
+  if (T == 0) return HKV_OK;
+  p.pos = table ? positions : nullptr;
+  p.pos64 = position_bits == 64;
+  p.ps_b = pos_stride_b;
+  p.ps_t = pos_stride_t;
+  p.table = table;
+  p.table_stride = table_stride;
+  p.max_pos = table ? max_pos : 1;
+  p.rot = rot;
+  p.eps = eps;
+  p.B = B;
+  p.T = T;
+  const int mode = adjacent ? hkv::kNrAdjacent : rot % 16 == 0 ? hkv::kNrLane : hkv::kNrAny;
+  const cudaError_t e = dtype == HKV_DT_F16 ? launch_norm_rope_t<__half>(p, mode, S(stream))
+                                            : launch_norm_rope_t<__nv_bfloat16>(p, mode, S(stream));
+  if (e != cudaSuccess) return cuda_fail(e);
+  return launch_status();
+}
+
+// --------------------------------------------------------------------------- pages
+namespace {
+hkv_status check_paged(const hkv_int4_store* s, int B, int H) {
+  const hkv_status rc = check_store(s);
+  if (rc != HKV_OK) return rc;
+  if (!s->page_table || !s->lengths || s->num_pages <= 0 || B <= 0 || H <= 0) return HKV_ERR_ARG;
+  if ((int64_t)B * H * s->max_pages >= (int64_t(1) << 30)) return HKV_ERR_UNSUPPORTED;
+  return HKV_OK;
+}
+
+// Workspace: new table | new lengths | want | from | vecs | list (3 per want) |
+// count | first (one per page), int32 each. At most one want per entry.
+size_t pages_words(const hkv_int4_store* s, int B, int H) {
+  const size_t e = (size_t)B * H * s->max_pages;
+  return 7 * e + B + 4 + s->num_pages;
+}
+
+void pages_params(hkv::PagesParams& p, const hkv_int4_store* s, int B, int H, int32_t* refs, void* ws) {
+  std::memset(&p, 0, sizeof(p));
+  const size_t e = (size_t)B * H * s->max_pages;
+  p.pool = static_cast<uint8_t*>(s->pages);
+  p.src_pool = p.pool;
+  p.stride = p.src_stride = s->page_stride;
+  p.table = const_cast<int32_t*>(s->page_table);
+  p.lengths = const_cast<int32_t*>(s->lengths);
+  p.refs = refs;
+  p.B = B;
+  p.H = H;
+  p.max_pages = s->max_pages;
+  p.num_pages = s->num_pages;
+  p.page_tokens = s->page_tokens;
+  p.block_bytes = block_bytes(s->format, s->group);
+  int32_t* w = static_cast<int32_t*>(ws);
+  p.new_table = w;
+  p.want = w + e;
+  p.from = w + 2 * e;
+  p.vecs = w + 3 * e;
+  p.list = w + 4 * e;
+  p.new_lengths = w + 7 * e;
+  p.count = p.new_lengths + B;
+  p.first = p.count + 4;
+}
+
+// CTAs of an apply launch: enough to fill the GPU, no more than there is to do.
+int pages_grid(int64_t entries, int64_t copies, int64_t page_bytes) {
+  const int64_t work = std::max((entries + 4 * hkv::kPgThreads - 1) / (4 * hkv::kPgThreads),
+                                copies * ((page_bytes + hkv::kPgChunk - 1) / hkv::kPgChunk));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(work, (int64_t)device_sms() * 6));
+}
+}  // namespace
+
+size_t hkv_pages_workspace_bytes(const hkv_int4_store* store, int32_t B, int32_t H) {
+  return check_paged(store, B, H) == HKV_OK ? 4 * pages_words(store, B, H) : 0;
+}
+
+hkv_status hkv_pages_fork(const hkv_int4_store* store, int32_t B, int32_t H, int32_t* refs, const int32_t* parents,
+                          void* workspace, size_t workspace_bytes, hkv_stream_t stream) {
+  hkv_status rc = check_paged(store, B, H);
+  if (rc != HKV_OK) return rc;
+  if (!refs || !parents) return HKV_ERR_ARG;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < 4 * pages_words(store, B, H)) return HKV_ERR_CAPACITY;
+  hkv::PagesParams p;
+  pages_params(p, store, B, H, refs, workspace);
+  p.parents = parents;
+  p.wants = B * H;
+  const int per = H * store->max_pages;
+  cudaError_t e = launch_pdl(8, hkv::pages_fork_map_kernel, dim3(B, std::min(16, cdiv(per, 2 * hkv::kPgThreads))),
+                             dim3(hkv::kPgThreads), 0, S(stream), p);
+  if (e == cudaSuccess) e = launch_pdl(8, hkv::pages_give_kernel, dim3(1), dim3(hkv::kPgGive), 0, S(stream), p, p.new_table);
+  if (e == cudaSuccess)
+    e = launch_pdl(8, hkv::pages_fork_apply_kernel, dim3(pages_grid((int64_t)B * per, (int64_t)B * H, store->page_stride)),
+                   dim3(hkv::kPgThreads), 0, S(stream), p);
+  return e == cudaSuccess ? launch_status() : cuda_fail(e);
+}
+
+hkv_status hkv_pages_reserve(const hkv_int4_store* store, int32_t B, int32_t H, int32_t* refs, int32_t tokens,
+                             const int32_t* tokens_of, void* workspace, size_t workspace_bytes, hkv_stream_t stream) {
+  hkv_status rc = check_paged(store, B, H);
+  if (rc != HKV_OK) return rc;
+  if (!refs || tokens < 0) return HKV_ERR_ARG;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < 4 * pages_words(store, B, H)) return HKV_ERR_CAPACITY;
+  if (tokens == 0) return HKV_OK;
+  // more than a row holds is wanted: the entries behind the row's end are flagged
+  const int64_t per = std::min<int64_t>(cdiv(tokens, store->page_tokens) + 1, store->max_pages);
+  if ((int64_t)tokens > (int64_t)store->max_pages * store->page_tokens) return HKV_ERR_CAPACITY;
+  hkv::PagesParams p;
+  pages_params(p, store, B, H, refs, workspace);
+  p.extra = tokens;
+  p.extra_of = tokens_of;
+  p.wants = (int)(per * B * H);
+  cudaError_t e = launch_pdl(8, hkv::pages_reserve_map_kernel, dim3(std::min(device_sms(), cdiv(p.wants, hkv::kPgThreads))),
+                             dim3(hkv::kPgThreads), 0, S(stream), p);
+  if (e == cudaSuccess) e = launch_pdl(8, hkv::pages_give_kernel, dim3(1), dim3(hkv::kPgGive), 0, S(stream), p, p.table);
+  return e == cudaSuccess ? launch_status() : cuda_fail(e);
+}
+
+hkv_status hkv_pages_compact(const hkv_int4_store* src, int32_t B, int32_t H, const hkv_int4_store* into,
+                             int32_t* into_refs, void* workspace, size_t workspace_bytes, hkv_stream_t stream) {
+  hkv_status rc = check_paged(src, B, H);
+  if (rc != HKV_OK) return rc;
+  if ((rc = check_paged(into, B, H)) != HKV_OK) return rc;
+  if (!into_refs || src->format != into->format || src->group != into->group || src->page_tokens != into->page_tokens ||
+      into->max_pages < src->max_pages)
+    return HKV_ERR_ARG;
+  const uint8_t *a = static_cast<const uint8_t*>(src->pages), *b = static_cast<const uint8_t*>(into->pages);
+  if (a < b + (int64_t)into->num_pages * into->page_stride && b < a + (int64_t)src->num_pages * src->page_stride) return HKV_ERR_ARG;
+  if (src->page_table == into->page_table || src->lengths == into->lengths) return HKV_ERR_ARG;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < 4 * pages_words(src, B, H)) return HKV_ERR_CAPACITY;
+  hkv::PagesParams p;
+  pages_params(p, src, B, H, into_refs, workspace);
+  p.src_table = src->page_table;
+  p.src_lengths = src->lengths;
+  p.src_max_pages = src->max_pages;
+  p.src_num_pages = src->num_pages;
+  p.pool = static_cast<uint8_t*>(into->pages);
+  p.stride = into->page_stride;
+  p.table = const_cast<int32_t*>(into->page_table);
+  p.lengths = const_cast<int32_t*>(into->lengths);
+  p.max_pages = into->max_pages;
+  p.num_pages = into->num_pages;
+  const int64_t entries = (int64_t)B * H * src->max_pages;
+  cudaError_t e = cudaMemsetAsync(p.first, 0x7f, (size_t)src->num_pages * 4, S(stream));
+  if (e == cudaSuccess) e = cudaMemsetAsync(into_refs, 0, (size_t)into->num_pages * 4, S(stream));
+  if (e == cudaSuccess)
+    e = launch_pdl(8, hkv::pages_compact_map_kernel, dim3(pages_grid(entries, 0, 1)), dim3(hkv::kPgThreads), 0, S(stream), p);
+  if (e == cudaSuccess) e = launch_pdl(8, hkv::pages_compact_give_kernel, dim3(1), dim3(hkv::kPgGive), 0, S(stream), p);
+  if (e == cudaSuccess)
+    e = launch_pdl(8, hkv::pages_compact_apply_kernel,
+                   dim3(pages_grid((int64_t)B * H * into->max_pages, std::min<int64_t>(entries, into->num_pages), src->page_stride)),
+                   dim3(hkv::kPgThreads), 0, S(stream), p);
+  return e == cudaSuccess ? launch_status() : cuda_fail(e);
 }
 
 }  // extern "C"

@@ -7,6 +7,7 @@ passed as raw pointers plus sizes.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from typing import Optional, Tuple, Union
@@ -38,6 +39,18 @@ def _require_cuda(*ts: torch.Tensor) -> None:
             raise RuntimeError(
                 "hetero_kv kernels need CUDA tensors (HKV_ERR_UNSUPPORTED for CPU tensors: "
                 "there is no CPU fallback)")
+
+
+def launch_on(device: torch.device, stream: Optional[torch.cuda.Stream] = None):
+    """Context in which ``device`` is the current device and ``stream`` (None:
+    its current stream) the current stream, for the launches and for what they
+    allocate: memory taken on one stream and first written on another could
+    still be in use by the first."""
+    if stream is not None:
+        if stream.device != device:
+            raise ValueError(f"stream of {stream.device} for tensors on {device}")
+        return torch.cuda.stream(stream)
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def page_bytes(fmt: str, group: int, page_tokens: int) -> int:
@@ -82,6 +95,41 @@ class Int4KVStore:
                            if self.paged else None)
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=self.device)
         self.len_hint = 0  # host-side upper bound of lengths (sizes the split-KV grid)
+
+    @classmethod
+    def wrap(cls, pool: torch.Tensor, page_table: Optional[torch.Tensor], lengths: torch.Tensor, kv_heads: int, *,
+             fmt: str = "ref", group: int = 32, page_tokens: int = 256, len_hint: int = 0) -> "Int4KVStore":
+        """A store over memory that the caller owns, nothing copied: ``pool``
+        uint8 [num_pages, page_bytes], ``page_table`` int32 [B * kv_heads,
+        max_pages] (None: the dense mode, max_pages consecutive pages per unit)
+        and ``lengths`` int32 [B], contiguous and on one device. Several stores
+        may share a pool (e.g. a prompt's pages and its samples' own)."""
+        if fmt not in FORMATS:
+            raise ValueError(f"fmt must be one of {list(FORMATS)}")
+        nbytes = page_bytes(fmt, group, page_tokens)
+        units = lengths.numel() * kv_heads
+        if pool.dtype != torch.uint8 or pool.dim() != 2 or pool.shape[1] != nbytes or not pool.is_contiguous():
+            raise ValueError(f"pool must be a contiguous uint8 [num_pages, {nbytes}] tensor")
+        if lengths.dtype != torch.int32 or lengths.dim() != 1 or not lengths.is_contiguous() or units == 0:
+            raise ValueError("lengths must be a contiguous int32 [B] tensor")
+        if page_table is None:
+            if pool.shape[0] == 0 or pool.shape[0] % units:
+                raise ValueError(f"without a page table the pool holds whole rows of pages for {units} units")
+        elif (page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != units
+              or page_table.shape[1] == 0 or not page_table.is_contiguous()):
+            raise ValueError(f"page_table must be a contiguous int32 [{units}, max_pages] tensor")
+        if any(t.device != pool.device for t in (lengths, page_table) if t is not None):
+            raise ValueError("pool, page_table and lengths must be on one device")
+        s = cls.__new__(cls)
+        s.batch, s.kv_heads, s.fmt, s.group, s.page_tokens = lengths.numel(), kv_heads, fmt, group, page_tokens
+        s.paged = page_table is not None
+        s.num_pages = pool.shape[0]
+        s.max_pages = page_table.shape[1] if s.paged else s.num_pages // units
+        s.capacity = s.max_pages * page_tokens
+        s.page_bytes = nbytes
+        s.device, s.pool, s.page_table, s.lengths = pool.device, pool, page_table, lengths
+        s.len_hint = int(len_hint)
+        return s
 
     def struct(self, len_hint: Optional[int] = None, b0: int = 0) -> L.HkvInt4Store:
         """The C view of this store; ``b0`` > 0 views sequences [b0, batch)
@@ -596,3 +644,106 @@ def repack_ref(codes: torch.Tensor, scales: torch.Tensor, zps: torch.Tensor, gro
     st = store.struct()
     L.check(L.load().hkv_repack_ref(c.data_ptr(), s.data_ptr(), z.data_ptr(), B, H, S_, group, role,
                                     ctypes.byref(st), _stream(stream)), "hkv_repack_ref")
+
+
+def rope_table(max_pos: int, rot_dim: int = HEAD_DIM, base: float = 10000.0, scale: float = 1.0,
+               device: Union[str, torch.device] = "cuda") -> torch.Tensor:
+    """Rotation table f32 [max_pos, rot_dim] for ``norm_rope``: cos, then sin, of
+    position * scale * base ** (-2 i / rot_dim). The angles are taken in 64 bits:
+    in 32 a position of 131,071 would be off by up to 0.004 radian."""
+    if max_pos <= 0 or rot_dim < 2 or rot_dim > HEAD_DIM or rot_dim % 2:
+        raise ValueError(f"bad rotation table: max_pos={max_pos}, rot_dim={rot_dim}")
+    i = torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device)
+    ang = torch.outer(torch.arange(max_pos, dtype=torch.float64, device=device) * scale, base ** (-i / rot_dim))
+    return torch.cat((ang.cos(), ang.sin()), dim=1).to(torch.float32)
+
+
+def _rows(x: torch.Tensor) -> L.HkvRows:
+    r = L.HkvRows()
+    r.data, r.heads = x.data_ptr(), x.shape[1]
+    r.stride_b, r.stride_h = x.stride(0), x.stride(1)
+    r.stride_t = x.stride(2) if x.dim() == 4 else 0
+    return r
+
+
+def norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: Optional[torch.Tensor] = None,
+              table: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,
+              k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, adjacent: bool = False,
+              q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None, stream=None):
+    """Queries [B, Hq, T, 128] and keys [B, Hkv, T, 128] (or [B, H, 128] for one
+    token each; f16 or bf16, any strides, e.g. slices of a packed projection)
+    made ready for the cache in one launch: every head's vector is divided by its
+    root mean square and multiplied by ``q_weight`` / ``k_weight`` [128] (None:
+    left as it is), then its first ``table.shape[1]`` dimensions are turned by
+    the angles of the token's position, in pairs (i, i + rot / 2), or with
+    ``adjacent`` (2 i, 2 i + 1). fp32 inside, rounded once.
+
+    ``positions``: int32 or int64 [B, T] ([T] for all sequences; [B] for one
+    token each). Rows of a negative position (padding) are not written; one
+    behind the table sets DEVERR_BAD_POSITION and is not written either.
+    ``table``: f32 [max_pos, rot] of cos | sin (``rope_table``); None: no
+    rotation. ``q_out`` / ``k_out``: where to write, e.g. q and k themselves.
+    Either of q and k may be None. Returns (q_out, k_out)."""
+    ins = [x for x in (q, k) if x is not None]
+    if not ins:
+        raise ValueError("norm_rope needs q or k")
+    _require_cuda(*(t for t in (q, k, positions, table, q_weight, k_weight, q_out, k_out) if t is not None))
+    x0 = ins[0]
+    if x0.dim() not in (3, 4) or x0.shape[-1] != HEAD_DIM:
+        raise ValueError("q and k must be [B, H, T, 128] or [B, H, 128]")
+    B, T = x0.shape[0], (x0.shape[2] if x0.dim() == 4 else 1)
+    outs = []
+    for x, o, name in ((q, q_out, "q"), (k, k_out, "k")):
+        if x is None:
+            if o is not None:
+                raise ValueError(f"{name}_out without {name}")
+            outs.append(None)
+            continue
+        if x.dim() != x0.dim() or x.shape[0] != B or x.shape[2:] != x0.shape[2:] or x.dtype != x0.dtype:
+            raise ValueError("q and k must have one batch, length, head size and dtype")
+        if o is not None and (o.shape != x.shape or o.dtype != x.dtype):
+            raise ValueError(f"{name}_out must have the shape and dtype of {name}")
+        if x.stride(-1) != 1 or (o is not None and o.stride(-1) != 1):
+            raise ValueError("the head dimension must be contiguous")
+        outs.append(o)
+    dt = dtype_code(x0.dtype)
+    if dt == L.DT_F32:
+        raise TypeError("norm_rope takes float16 or bfloat16")
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    for w in weights:
+        if w.shape != (HEAD_DIM,) or not w.is_contiguous() or w.dtype != weights[0].dtype:
+            raise ValueError("norm weights must be contiguous [128] tensors of one dtype")
+    rot = max_pos = tstride = ps_b = ps_t = 0
+    if table is not None:
+        if table.dtype != torch.float32 or table.dim() != 2 or table.stride(1) != 1:
+            raise ValueError("table must be a float32 [max_pos, rot] tensor")
+        max_pos, rot = table.shape
+        tstride = table.stride(0) if max_pos > 1 else max(table.stride(0), rot)
+        if positions is None or positions.dtype not in (torch.int32, torch.int64):
+            raise ValueError("positions must be an int32 or int64 tensor")
+        if positions.shape == (B, T):
+            ps_b, ps_t = positions.stride()
+        elif x0.dim() == 3 and positions.shape == (B,):
+            ps_b = positions.stride(0)
+        elif x0.dim() == 4 and positions.shape == (T,):
+            ps_t = positions.stride(0)
+        else:
+            raise ValueError(f"positions must be [B, T] = {[B, T]}, or [T], or [B] for one token each")
+    for t in (q, k, positions, table, q_weight, k_weight, *outs):
+        if t is not None and t.device != x0.device:
+            raise ValueError("all tensors must be on one device")
+    if any(x.shape[1] == 0 for x in ins):
+        raise ValueError("q and k must have heads")
+    with launch_on(x0.device, stream):
+        outs = [torch.empty(x.shape, dtype=x.dtype, device=x.device) if x is not None and o is None else o
+                for x, o in zip((q, k), outs)]
+        if B == 0 or T == 0:
+            return outs[0], outs[1]
+        rows = [ctypes.byref(_rows(t)) if t is not None else None for t in (q, k, outs[0], outs[1])]
+        L.check(L.load().hkv_norm_rope(
+            *rows, dt, B, T, HEAD_DIM, q_weight.data_ptr() if q_weight is not None else None,
+            k_weight.data_ptr() if k_weight is not None else None, dtype_code(weights[0].dtype) if weights else 0,
+            float(eps), positions.data_ptr() if rot else None,
+            64 if rot and positions.dtype == torch.int64 else 32, ps_b, ps_t, table.data_ptr() if rot else None,
+            tstride, max_pos, rot, int(bool(adjacent)), _stream()), "hkv_norm_rope")
+    return outs[0], outs[1]

@@ -85,6 +85,7 @@ typedef int hkv_status;
 #define HKV_DEVERR_TIMEOUT 1u
 #define HKV_DEVERR_BAD_PAGE 2u
 #define HKV_DEVERR_CAPACITY 4u
+#define HKV_DEVERR_BAD_POSITION 8u /* a position behind the rotation table */
 
 typedef void* hkv_stream_t; /* cudaStream_t */
 typedef void* hkv_event_t;  /* cudaEvent_t */
@@ -121,6 +122,17 @@ typedef struct hkv_dense_kv {
   int32_t len;            /* rows when lengths == NULL; else an upper bound */
   int32_t reserved;
 } hkv_dense_kv;
+
+/* Rows of head vectors [B][heads][T][128] with element strides (any of which may
+ * be 0 for an input that is broadcast). */
+typedef struct hkv_rows {
+  void* data;
+  int64_t stride_b; /* elements */
+  int64_t stride_h;
+  int64_t stride_t;
+  int32_t heads;
+  int32_t reserved;
+} hkv_rows;
 
 /* ---------------------------------------------------------------- misc */
 const char* hkv_status_str(hkv_status s);
@@ -434,6 +446,65 @@ hkv_status hkv_qk_scores_flat(const void* q, int32_t q_dtype, const uint8_t* cod
  * HKV_ERR_DEVICE, the context still usable. Synchronises `stream`. No
  * counterpart in the reference (it has no device-side waits). */
 hkv_status hkv_selftest_bounded_wait(int64_t limit_ns, int32_t arrive, hkv_stream_t stream);
+
+/* ---------------------------------------------------------------- 5. before the cache
+ * Norm of every query and key head with the position rotation, in one launch
+ * (the step between a layer's projections and hkv_append_kv / hkv_quantize_pack).
+ * Per row x, in fp32 with one rounding at the end: y = x * rsqrt(mean(x^2) + eps)
+ * * weight (weight NULL: y = x), then pair i < rot/2 of y's first `rot` dims,
+ * (a, b) = dims (i, rot/2 + i), or (2i, 2i + 1) with adjacent != 0, becomes
+ * (a c - b s, b c + a s) with c = table[pos][i], s = table[pos][rot/2 + i].
+ * q, k (either may be NULL, with its out): f16 or bf16 rows (one dtype); the outs
+ * may be the inputs themselves (same strides), but must not overlap them
+ * otherwise, nor have a stride of 0. Weights: [128] of weight_dtype, contiguous.
+ * positions: [B][T] int32 (position_bits 32) or int64 (64) on the device with
+ * element strides. A negative position marks a padding row, whose output is not
+ * written; one at or behind max_pos sets HKV_DEVERR_BAD_POSITION, its output not
+ * written either. table: f32 [max_pos][rot], rows table_stride elements apart,
+ * rot even, 2 <= rot <= 128. table NULL: no rotation (rot 0, positions unused).
+ * No counterpart in the reference, which gets rotated queries and keys. */
+hkv_status hkv_norm_rope(const hkv_rows* q, const hkv_rows* k, const hkv_rows* q_out, const hkv_rows* k_out,
+                         int32_t dtype, int32_t B, int32_t T, int32_t D, const void* q_weight,
+                         const void* k_weight, int32_t weight_dtype, float eps, const void* positions,
+                         int32_t position_bits, int64_t pos_stride_b, int64_t pos_stride_t, const float* table,
+                         int64_t table_stride, int32_t max_pos, int32_t rot, int32_t adjacent,
+                         hkv_stream_t stream);
+
+/* ---------------------------------------------------------------- 6. pages of a paged store
+ * Sequences that share pages: page_table (of the store, written here), lengths
+ * [B] and refs [num_pages] (how many table entries name each page; 0 = free) are
+ * device state, and every call is stream-ordered and capturable. The store needs
+ * page_table, lengths and num_pages. The same state gives the same page ids: new
+ * pages are the lowest free ids, in table order. Where the free pages run out,
+ * or a unit's row is full, the entries left over stay -1 and
+ * HKV_DEVERR_CAPACITY is set; a table entry outside the pool sets
+ * HKV_DEVERR_BAD_PAGE and is treated as empty. `workspace`:
+ * hkv_pages_workspace_bytes, 16-byte aligned, not shared by calls that overlap.
+ * No counterpart in the reference (one cache per sequence, chunks never shared). */
+size_t hkv_pages_workspace_bytes(const hkv_int4_store* store, int32_t B, int32_t H);
+
+/* Sequence b becomes what sequence parents[b] (device int32 [B]) was before the
+ * call, for all b at once; -1 empties it. The lowest b with a given parent takes
+ * over the parent's whole row of pages; the others share its full pages and get
+ * their own copy of a partly filled last page (its 128-token blocks in use).
+ * Pages that nobody names any more are free again, for this call's copies too.
+ * A parent outside [-1, B) sets HKV_DEVERR_BAD_PAGE and counts as -1. */
+hkv_status hkv_pages_fork(const hkv_int4_store* store, int32_t B, int32_t H, int32_t* refs, const int32_t* parents,
+                          void* workspace, size_t workspace_bytes, hkv_stream_t stream);
+
+/* Gives every unit the pages it lacks for `tokens` more tokens behind its length
+ * (tokens_of, device int32 [B], lowers that per sequence when not NULL). */
+hkv_status hkv_pages_reserve(const hkv_int4_store* store, int32_t B, int32_t H, int32_t* refs, int32_t tokens,
+                             const int32_t* tokens_of, void* workspace, size_t workspace_bytes, hkv_stream_t stream);
+
+/* Copies the store's pages into another pool of the same format, page size and
+ * units: in order of their first entry in the table they become pages 0, 1, ...
+ * of `into`, whose page_table, lengths and into_refs are rewritten whole; shared
+ * pages stay shared. The bytes of pages that lie behind the length are not
+ * copied, nor is the rest of into's pool written. into->max_pages >=
+ * src->max_pages; src is left as it is; the pools must not overlap. */
+hkv_status hkv_pages_compact(const hkv_int4_store* src, int32_t B, int32_t H, const hkv_int4_store* into,
+                             int32_t* into_refs, void* workspace, size_t workspace_bytes, hkv_stream_t stream);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop
