@@ -15,6 +15,7 @@
 #include "hkv_prefill.cuh"
 #include "hkv_norm_rope.cuh"
 #include "hkv_pages.cuh"
+#include "hkv_shared.cuh"
 
 #define HKV_VERSION 100
 
@@ -554,6 +555,90 @@ hkv_status launch_prefill_f(const hkv::PrefillParams& p, int group, cudaStream_t
     case 128: return launch_prefill_t<FMT, 128>(p, st);
   }
   return HKV_ERR_UNSUPPORTED;
+}
+
+// --------------------------------------------------------------------------- shared prefix
+template <int FMT, int GROUP, int N>
+hkv_status launch_shared_t(const hkv::SharedParams& p, cudaStream_t st) {
+  static std::once_flag once;
+  static cudaError_t attr_err = cudaSuccess;
+  std::call_once(once, [] {
+    attr_err = cudaFuncSetAttribute(hkv::shared_prefix_kernel<FMT, GROUP, N>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    hkv::sh_smem(N));
+  });
+  if (attr_err != cudaSuccess) return cuda_fail(attr_err);
+  const cudaError_t e = launch_pdl(8, hkv::shared_prefix_kernel<FMT, GROUP, N>, dim3(p.C), dim3(hkv::sh_threads(N)),
+                                   hkv::sh_smem(N), st, p);
+  return e == cudaSuccess ? launch_status() : cuda_fail(e);
+}
+template <int FMT, int GROUP>
+hkv_status launch_shared_n(const hkv::SharedParams& p, cudaStream_t st) {
+  switch (p.N) {
+    case 16: return launch_shared_t<FMT, GROUP, 16>(p, st);
+    case 32: return launch_shared_t<FMT, GROUP, 32>(p, st);
+    case 64: return launch_shared_t<FMT, GROUP, 64>(p, st);
+  }
+  return launch_shared_t<FMT, GROUP, 128>(p, st);
+}
+template <int FMT>
+hkv_status launch_shared(const hkv::SharedParams& p, cudaStream_t st) {
+  switch (p.prefix.group) {
+    case 32: return launch_shared_n<FMT, 32>(p, st);
+    case 64: return launch_shared_n<FMT, 64>(p, st);
+  }
+  return launch_shared_n<FMT, 128>(p, st);
+}
+
+// Rows per product, CTAs and workspace of a shared-prefix decode:
+// own part's workspace | its (o, m, l) | the pieces' (o, m, l).
+struct SharedPlan {
+  int N, C;
+  size_t own_ws, own_o, own_ml, part_o, part_ml, bytes;  // offsets
+};
+hkv_status shared_plan(const hkv_int4_store* prefix, const int32_t* start, int P, const hkv_int4_store* body,
+                       const hkv_dense_kv* dense, int B, int Hq, int Hkv, int D, int ctas, SharedPlan* out) {
+  const hkv_status rc = check_store(prefix);
+  if (rc != HKV_OK) return rc;
+  if (!start || P <= 0 || B <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv) return HKV_ERR_ARG;
+  if (D != HKV_D || P > hkv::kShMaxGroups) return HKV_ERR_UNSUPPORTED;
+  const int G = Hq / Hkv;
+  if (start[0] < 0 || start[P] > B) return HKV_ERR_ARG;
+  int64_t rows = 0;
+  for (int g = 0; g < P; ++g) {
+    if (start[g + 1] < start[g]) return HKV_ERR_ARG;
+    rows = std::max<int64_t>(rows, (int64_t)(start[g + 1] - start[g]) * G);
+  }
+  SharedPlan pl;
+  pl.N = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  pl.C = std::min(ctas > 0 ? ctas : device_sms(), 65535);
+  int64_t units = 0, steps = 0;
+  const int64_t cap = (int64_t)prefix->max_pages * (prefix->page_tokens / HKV_BLOCK_TOKENS);
+  for (int g = 0; g < P; ++g) {
+    const int64_t u = Hkv * (((int64_t)(start[g + 1] - start[g]) * G + pl.N - 1) / pl.N);
+    units += u;
+    steps += u * (cap + hkv::kShCharge);
+  }
+  if (steps >= (int64_t(1) << 31) || (units + pl.C) * pl.N >= (int64_t(1) << 31) || (int64_t)B * Hq >= (int64_t(1) << 28) ||
+      (int64_t)prefix->max_pages * prefix->page_tokens >= (int64_t(1) << 31))
+    return HKV_ERR_UNSUPPORTED;
+  size_t at = 0;
+  pl.own_ws = 0;
+  if (body || dense) {
+    Plan dp;
+    const int dummy = 0;  // an address for the argument check: the queries are not read here
+    hkv_status r = check_decode_args(&dummy, HKV_DT_F16, body, dense, B, Hq, Hkv, D);
+    if (r == HKV_OK) r = make_plan(B, Hq, Hkv, body, dense, ctas, &dp);
+    if (r != HKV_OK) return r;
+    at = (dp.ws_bytes + 255) & ~(size_t)255;
+  }
+  const bool own = body || dense;
+  pl.own_o = at;
+  pl.own_ml = pl.own_o + (own ? (size_t)B * Hq * HKV_D * 4 : 0);
+  pl.part_o = (pl.own_ml + (own ? (size_t)B * Hq * 8 : 0) + 255) & ~(size_t)255;
+  pl.part_ml = pl.part_o + (size_t)(units + pl.C) * pl.N * HKV_D * 4;
+  pl.bytes = pl.part_ml + (size_t)(units + pl.C) * pl.N * 8;
+  *out = pl;
+  return HKV_OK;
 }
 
 // --------------------------------------------------------------------------- norm + rotation
@@ -1440,6 +1525,65 @@ hkv_status hkv_pages_compact(const hkv_int4_store* src, int32_t B, int32_t H, co
     e = launch_pdl(8, hkv::pages_compact_apply_kernel,
                    dim3(pages_grid((int64_t)B * H * into->max_pages, std::min<int64_t>(entries, into->num_pages), src->page_stride)),
                    dim3(hkv::kPgThreads), 0, S(stream), p);
+  return e == cudaSuccess ? launch_status() : cuda_fail(e);
+}
+
+// --------------------------------------------------------------------------- shared prefix
+size_t hkv_decode_shared_workspace_bytes(const hkv_int4_store* prefix, const int32_t* group_start, int32_t n_groups,
+                                         const hkv_int4_store* body, const hkv_dense_kv* dense, int32_t B,
+                                         int32_t Hq, int32_t Hkv, int32_t D, int32_t ctas) {
+  SharedPlan pl;
+  return shared_plan(prefix, group_start, n_groups, body, dense, B, Hq, Hkv, D, ctas, &pl) == HKV_OK ? pl.bytes : 0;
+}
+
+hkv_status hkv_decode_shared(const void* q, int32_t q_dtype, int64_t q_stride_b, int64_t q_stride_h,
+                             const hkv_int4_store* prefix, const int32_t* group_start, int32_t n_groups,
+                             const hkv_int4_store* body, const hkv_dense_kv* dense, int32_t B, int32_t Hq,
+                             int32_t Hkv, int32_t D, float sm_scale, int32_t ctas, void* workspace,
+                             size_t workspace_bytes, void* out, int32_t out_dtype, int64_t out_stride_b,
+                             int64_t out_stride_h, hkv_stream_t stream) {
+  if (!q || (q_dtype != HKV_DT_F16 && q_dtype != HKV_DT_BF16) || !out) return HKV_ERR_ARG;
+  if (out_dtype < HKV_DT_F16 || out_dtype > HKV_DT_F32) return HKV_ERR_ARG;
+  if (!(sm_scale > 0.f) || !std::isfinite(sm_scale)) return HKV_ERR_ARG;
+  SharedPlan pl;
+  hkv_status rc = shared_plan(prefix, group_start, n_groups, body, dense, B, Hq, Hkv, D, ctas, &pl);
+  if (rc != HKV_OK) return rc;
+  if (!workspace || workspace_bytes < pl.bytes || !aligned16(workspace)) return HKV_ERR_CAPACITY;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const bool own = body || dense;
+  hkv::SharedParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = q;
+  p.q_dtype = q_dtype;
+  p.q_sb = q_stride_b;
+  p.q_sh = q_stride_h;
+  p.prefix = *prefix;
+  p.P = n_groups;
+  p.Hkv = Hkv;
+  p.G = Hq / Hkv;
+  p.C = pl.C;
+  p.qscale = static_cast<float>(static_cast<double>(sm_scale) * 1.4426950408889634);
+  p.counters = reinterpret_cast<int*>(ws);
+  p.n_counters = own ? B * Hkv : 0;
+  p.part_o = reinterpret_cast<float*>(ws + pl.part_o);
+  p.part_ml = reinterpret_cast<float*>(ws + pl.part_ml);
+  p.own_o = own ? reinterpret_cast<float*>(ws + pl.own_o) : nullptr;
+  p.own_ml = reinterpret_cast<float*>(ws + pl.own_ml);
+  p.out = out;
+  p.out_dtype = out_dtype;
+  p.out_sb = out_stride_b;
+  p.out_sh = out_stride_h;
+  p.B = B;
+  p.N = pl.N;
+  std::memcpy(p.start, group_start, sizeof(int32_t) * (n_groups + 1));
+  rc = prefix->format == HKV_FMT_REF ? launch_shared<HKV_FMT_REF>(p, S(stream)) : launch_shared<HKV_FMT_FP16MIN>(p, S(stream));
+  if (rc != HKV_OK) return rc;
+  if (own) {
+    rc = run_decode(q, q_dtype, q_stride_b, q_stride_h, body, dense, B, Hq, Hkv, D, sm_scale, ctas, ws, pl.own_o, nullptr,
+                    HKV_DT_F32, 0, 0, const_cast<float*>(p.own_o), const_cast<float*>(p.own_ml), S(stream));
+    if (rc != HKV_OK) return rc;
+  }
+  const cudaError_t e = launch_pdl(8, hkv::shared_merge_kernel, dim3(cdiv((int64_t)B * Hq, 8)), dim3(256), 0, S(stream), p);
   return e == cudaSuccess ? launch_status() : cuda_fail(e);
 }
 

@@ -1,0 +1,650 @@
+// Decode attention over an INT4 prefix that several sequences share.
+// Included by hetero_kv.cu.
+//
+// A group of n sequences has one prefix; per KV head its n G query heads are the
+// columns of ONE product over the prefix's tokens, so the packed pages are read
+// and dequantised once per kShN rows instead of once per sequence:
+//   S^T[token][row] = K Q^T,  P = 2^(S qscale - m),  O^T[dim][row] += V^T P
+// on tcgen05 with the tokens (then the dims) as the MMA's M = 128 and the rows as
+// its N = 16 .. 128: a decode batch has few rows, and this way they cost what they
+// are (with the rows as M, 8 rows would cost 128). The running max m and the sum
+// of P are fp32, m moves only when a score beats it by more than 2^8.
+//
+// One persistent CTA per SM; every (group, KV head, row tile) unit's 128-token
+// tiles, with a charge of kShCharge tiles per unit for a piece's start and end,
+// are cut into equal ranges, one per CTA (so a CTA has a few "pieces", runs of
+// tiles of one unit). Each piece leaves an un-normalised partial (O, m, l) at
+// index cta + unit (unique: each next piece raises one of the two), and
+// shared_merge_kernel joins a row's partials with the one of its own tokens.
+//
+// Roles (tile n of the CTA, in order, lives in the buffers n & 1):
+//   producer  one bulk copy per packed 128-token block into a ring of raw slots
+//   K warps   thread = token: dequantised f16 K straight into TMEM (A of S^T, so
+//             K never crosses shared memory again)
+//   V warps   dequantised V^T into shared memory (128-byte swizzle, A of O^T)
+//   MMA warp  S^T(n + 1) ahead of O^T(n)
+//   softmax   thread = token: kShCols columns each of S^T from TMEM, P as f16
+//             rows [token][row] (N-major B of O^T, 128-byte swizzle)
+// Every wait is bounded (HKV_WAIT_NS); on expiry the device error word is set, the
+// CTA's roles leave, and copies and products in flight are waited for before TMEM
+// is freed.
+#pragma once
+#include "hkv_prefill.cuh"
+
+namespace hkv {
+
+constexpr int kShMaxGroups = 512;
+constexpr int kShCharge = 6;
+constexpr int kShRawBytes = 24 * 1024;
+
+constexpr int sh_softmax_groups(int n) { return n <= 32 ? 1 : 2; }
+constexpr int sh_threads(int n) { return 32 * (4 * sh_softmax_groups(n) + 10); }
+constexpr int sh_slots(int n) { return n <= 64 ? 4 : 2; }
+constexpr int sh_p_bytes(int n) { return 128 * 128 * (n <= 64 ? 1 : 2); }  // [token][64 rows] f16 blocks
+constexpr int sh_smem(int n) {  // Q | Vt[2] | P[2] | raw slots | alignment
+  return n * 256 + 2 * kPfTileBytes + 2 * sh_p_bytes(n) + sh_slots(n) * kShRawBytes + 1024;
+}
+constexpr int sh_tmem_cols(int n) { return 128 + 3 * n <= 256 ? 256 : 512; }  // K[2] | S[2] | O
+
+struct SharedParams {
+  const void* q;
+  int q_dtype;
+  int64_t q_sb, q_sh;
+  hkv_int4_store prefix;    // batch = groups
+  int P, Hkv, G, C;         // groups, KV heads, query heads per KV head, CTAs
+  float qscale;             // sm_scale * log2(e)
+  int* counters;            // own part's merge counters, zeroed here
+  int n_counters;
+  float* part_o;            // [C + units][N][128]
+  float* part_ml;           // [C + units][N][2]
+  // merge
+  const float* own_o;       // [B][Hq][128], or NULL
+  const float* own_ml;      // [B][Hq][2]
+  void* out;
+  int out_dtype;
+  int64_t out_sb, out_sh;
+  int B, N;
+  int start[kShMaxGroups + 1];  // sequences [start[p], start[p + 1]) are group p
+};
+
+// The schedule of a launch, from the device lengths: steps before group p.
+__device__ __forceinline__ int sh_tiles(const SharedParams& p, int g) {
+  const int cap = p.prefix.max_pages * (p.prefix.page_tokens / HKV_BLOCK_TOKENS);
+  const int len = max(0, p.prefix.lengths ? p.prefix.lengths[g] : p.prefix.len);
+  return min(cap, (len + HKV_BLOCK_TOKENS - 1) / HKV_BLOCK_TOKENS);
+}
+__device__ __forceinline__ int sh_row_tiles(const SharedParams& p, int g) {
+  return ((p.start[g + 1] - p.start[g]) * p.G + p.N - 1) / p.N;
+}
+__device__ __forceinline__ int sh_units(const SharedParams& p, int g) { return p.Hkv * sh_row_tiles(p, g); }
+
+struct ShGroup {
+  int step, unit;  // steps and units before the group
+};
+// Fills s_g[0 .. P] (one warp); s_g[P].step is the launch's step count.
+__device__ __forceinline__ void sh_schedule(const SharedParams& p, ShGroup* s_g) {
+  const int lane = threadIdx.x & 31;
+  int step = 0, unit = 0;
+  for (int g0 = 0; g0 <= p.P; g0 += 32) {
+    const int g = g0 + lane;
+    int st = 0, un = 0;
+    if (g < p.P) {
+      const int tiles = sh_tiles(p, g);
+      un = sh_units(p, g);
+      st = tiles > 0 ? un * (tiles + kShCharge) : 0;
+    }
+    int si = st, ui = un;
+#pragma unroll
+    for (int k = 1; k < 32; k <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, si, k), b = __shfl_up_sync(0xffffffffu, ui, k);
+      if (lane >= k) si += a, ui += b;
+    }
+    if (g <= p.P) s_g[g] = ShGroup{step + si - st, unit + ui - un};
+    step += __shfl_sync(0xffffffffu, si, 31);
+    unit += __shfl_sync(0xffffffffu, ui, 31);
+  }
+}
+// First step of CTA c's range.
+__device__ __forceinline__ int sh_cut(int total, int C, int c) { return (int)((int64_t)total * c / C); }
+
+struct ShPiece {
+  int g, h, rt;  // group, KV head, row tile
+  int unit;      // ordinal of the unit
+  int t0, n;     // tiles [t0, t0 + n)
+};
+// A unit's tile i is step base + kShCharge + i; the first piece of the steps
+// [at, end) (n == 0: none), `at` moved behind its unit.
+__device__ __forceinline__ ShPiece sh_next(const SharedParams& p, const ShGroup* s_g, int& at, int end) {
+  ShPiece r;
+  r.n = 0;
+  int g = 0;
+  while (at < end) {
+    while (g < p.P && s_g[g + 1].step <= at) ++g;
+    if (g >= p.P) break;
+    const int units = s_g[g + 1].unit - s_g[g].unit;
+    const int per = (s_g[g + 1].step - s_g[g].step) / units;
+    const int u = (at - s_g[g].step) / per, base = s_g[g].step + u * per + kShCharge;
+    const int lo = max(at - base, 0), hi = min(per - kShCharge, end - base);
+    at = base + per - kShCharge;
+    if (hi > lo) {
+      const int rts = units / p.Hkv;
+      r.g = g;
+      r.h = u / rts;
+      r.rt = u - r.h * rts;
+      r.unit = s_g[g].unit + u;
+      r.t0 = lo;
+      r.n = hi - lo;
+      break;
+    }
+  }
+  return r;
+}
+
+// N-major B descriptor: rows of 64 f16 (128 B, 128-byte swizzle), 8 tokens per
+// 1,024-byte group; the second 64 columns 16 KiB further.
+__device__ __forceinline__ uint64_t sh_desc_n(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(16384 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+constexpr uint32_t sh_idesc(int n, bool b_n_major) {
+  return (1u << 4) | (b_n_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void sh_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void sh_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+template <int N>
+__device__ __forceinline__ void sh_ld(uint32_t addr, float (&v)[N]) {  // N columns of this thread's lane
+  static_assert(N == 16 || N == 32, "");
+  if constexpr (N == 32) {
+    tm_ld32(addr, v);
+  } else {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+  }
+}
+template <int N>
+__device__ __forceinline__ void sh_st(uint32_t addr, const float (&v)[N]) {
+  uint32_t r[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) r[i] = __float_as_uint(v[i]);
+  if constexpr (N == 32) tm_st32u(addr, r);
+  else tm_st16u(addr, r);
+}
+__device__ __forceinline__ bool bar_or(int id, int n, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.or.pred p, %2, %3, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)v), "r"(id), "r"(n)
+      : "memory");
+  return r != 0;
+}
+
+// Dims of 16-byte chunk kc (8 values) of Q's and K's common order: value 2 c + e
+// is dim 32 (kc / 4) + 8 c + 2 (kc % 4) + e, the order in which nib8_to_h2 yields
+// a K token's words, so that K needs no shuffling on its way into TMEM.
+__device__ __forceinline__ int sh_dim(int kc, int c) { return 32 * (kc >> 2) + 8 * c + 2 * (kc & 3); }
+
+// K of token t (thread t) of the raw block into TMEM lane t, columns [0, 64).
+// A token's four 16-byte chunks are read in an order rotated by t / 2, so that
+// the 8 threads of a load phase hit 8 distinct bank groups, and rotated back.
+template <int FMT, int GROUP>
+__device__ __forceinline__ void sh_convert_k(const uint8_t* rb, uint32_t tmem, int t, bool valid) {
+  constexpr int NG = HKV_D / GROUP;
+  uint4 v[4], u[4];
+  const int rot = (t >> 1) & 3;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(rb + t * 64 + (((j + rot) & 3) << 4));
+  const bool r1 = rot & 1, r2 = rot & 2;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) u[j] = r1 ? v[(j + 3) & 3] : v[j];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = r2 ? u[(j + 2) & 3] : u[j];
+  const uint8_t* meta = rb + HKV_META_OFF;
+  __half ks[NG], km[NG];
+  if constexpr (FMT == HKV_FMT_FP16MIN) vload_h<NG>(meta + 2 * NG * t, ks), vload_h<NG>(meta + 256 * NG + 2 * NG * t, km);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    uint32_t o[32];
+#pragma unroll
+    for (int w2 = 0; w2 < 2; ++w2) {
+      const int w = 2 * half + w2, g = (32 * w) / GROUP;
+      __half2 s2, m2;
+      uint32_t zlo = 0, zhi = 0;
+      if constexpr (FMT == HKV_FMT_FP16MIN) {
+        s2 = __half2half2(ks[g]);
+        m2 = __half2half2(km[g]);
+      } else {
+        const float s = reinterpret_cast<const float*>(meta)[t * NG + g];
+        const uint32_t z = meta[1024 * NG + t * NG + g];
+        s2 = __float2half2_rn(s);
+        m2 = __float2half2_rn(0.f);
+        zlo = h2u(__float2half2_rn(1024.f + (float)z));
+        zhi = h2u(__float2half2_rn(-64.f - (float)z));
+      }
+      if (!valid) s2 = m2 = __float2half2_rn(0.f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t wd = w == 0 ? v[j].x : w == 1 ? v[j].y : w == 2 ? v[j].z : v[j].w;
+        uint32_t h[4];
+        if constexpr (FMT == HKV_FMT_FP16MIN) nib8_to_h2(wd, h);
+        else nib8_to_h2_z(wd, zlo, zhi, h);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[16 * w2 + 4 * j + c] = h2u(__hfma2(u2h(h[c]), s2, m2));
+      }
+    }
+    tm_st32u(tmem + 32 * half, o);
+  }
+  tm_wait_st();
+}
+
+template <int FMT, int GROUP, int N>
+__global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const __grid_constant__ SharedParams p) {
+  constexpr int SG = sh_softmax_groups(N);   // softmax groups of 128 threads
+  constexpr int COLS = N / SG;               // columns of a softmax thread
+  constexpr int SUB = COLS < 32 ? COLS : 32; // taken at a time
+  constexpr int R = sh_slots(N);
+  constexpr int kThreads = sh_threads(N);
+  constexpr uint32_t kBlock = block_bytes(FMT, GROUP);
+  constexpr uint32_t kCols = sh_tmem_cols(N);
+  extern __shared__ __align__(1024) uint8_t sh_raw[];
+  __shared__ __align__(8) uint64_t raw_full[R], raw_free[R], k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], drain;
+  __shared__ uint32_t s_tmem;
+  __shared__ ShGroup s_g[kShMaxGroups + 1];
+  __shared__ int s_valid[16];        // tokens in use of tile n & 15
+  __shared__ __align__(16) float s_m[N], s_f[N];  // column's running max; its last rescale
+  __shared__ float s_cm[4][N];       // per-warp column maxima, then sums
+  uint8_t* sm = sh_raw + ((1024u - (smem_u32(sh_raw) & 1023u)) & 1023u);
+  uint8_t* sQ = sm;
+  uint8_t* sV = sQ + N * 256;
+  uint8_t* sP = sV + 2 * kPfTileBytes;
+  uint8_t* raw = sP + 2 * sh_p_bytes(N);
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+
+  if (t == 0) {
+    for (int i = 0; i < R; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_free[i], 8);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 4);
+      mbar_init(&v_full[i], 4);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4 * SG);
+      mbar_init(&pv_done[i], 1);
+    }
+    mbar_init(&drain, 1);
+    fence_barrier_init();
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "n"(kCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  griddep_wait();
+  griddep_launch_dependents();
+  for (int i = blockIdx.x * kThreads + t; i < p.n_counters; i += gridDim.x * kThreads) p.counters[i] = 0;
+  if (warp == 1) sh_schedule(p, s_g);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem, tS = tmem + 128, tO = tmem + 128 + 2 * N;
+  const int total = s_g[p.P].step;
+  int at = sh_cut(total, p.C, blockIdx.x);
+  const int end = sh_cut(total, p.C, blockIdx.x + 1);
+  int n0 = 0;       // tiles of the CTA before this piece
+  int issued = 0;   // producer: copies; MMA warp: whether there are products
+  bool ok = true;
+
+  while (true) {
+    const ShPiece pc = sh_next(p, s_g, at, end);
+    if (pc.n == 0) break;
+    // the piece's query rows, in K's dim order
+    const int rows = (p.start[pc.g + 1] - p.start[pc.g]) * p.G - pc.rt * N;
+    for (int c = t; c < N * 16; c += kThreads) {
+      const int n = c >> 4, kc = c & 15;
+      uint32_t o[4] = {0u, 0u, 0u, 0u};
+      if (n < rows) {
+        const int r = pc.rt * N + n, s = r / p.G;
+        const int64_t base = (int64_t)(p.start[pc.g] + s) * p.q_sb + (int64_t)(pc.h * p.G + r - s * p.G) * p.q_sh;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int64_t i = base + sh_dim(kc, e);
+          o[e] = h2u(__floats2half2_rn(load_any(p.q, p.q_dtype, i), load_any(p.q, p.q_dtype, i + 1)));
+        }
+      }
+      *reinterpret_cast<uint4*>(sQ + (kc >> 3) * (N * 128) + n * 128 + (((kc & 7) ^ (n & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    if (t < N) s_m[t] = -1.0e30f;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+
+    if (warp < 4 * SG) {
+      // ---------------- softmax: thread = token, columns [col0, col0 + COLS) ----------------
+      const int sg = warp >> 2, tok = t & 127, col0 = sg * COLS;
+      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+      const float2 qs2 = make_float2(p.qscale, p.qscale);
+      float l[COLS];
+#pragma unroll
+      for (int i = 0; i < COLS; ++i) l[i] = 0.f;
+      for (int j = 0; j < pc.n; ++j) {
+        const int n = n0 + j, buf = n & 1;
+        bool bad = !mbar_wait(&s_full[buf], (n >> 1) & 1);
+        if (n >= 2) bad = !mbar_wait(&pv_done[buf], ((n >> 1) - 1) & 1) || bad;  // P[buf] is free
+        __syncwarp();
+        tc_fence_after();
+        const bool see = tok < s_valid[n & 15];
+#pragma unroll
+        for (int s0 = 0; s0 < COLS; s0 += SUB) {
+          const int c0 = col0 + s0;
+          const uint32_t ts = tS + buf * N + c0 + lanes;
+          float x[SUB];  // S qscale - m
+          auto scores = [&]() {
+            sh_ld<SUB>(ts, x);
+#pragma unroll
+            for (int i = 0; i < SUB; i += 4) {
+              const float4 m = *reinterpret_cast<const float4*>(&s_m[c0 + i]);
+              const float2 a = __ffma2_rn(make_float2(x[i], x[i + 1]), qs2, make_float2(-m.x, -m.y));
+              const float2 b = __ffma2_rn(make_float2(x[i + 2], x[i + 3]), qs2, make_float2(-m.z, -m.w));
+              x[i] = a.x, x[i + 1] = a.y, x[i + 2] = b.x, x[i + 3] = b.y;
+            }
+          };
+          scores();
+          float mx = fmaxf(x[0], x[SUB - 1]);
+#pragma unroll
+          for (int i = 1; i + 1 < SUB; i += 2) mx = fmax3(mx, x[i], x[i + 1]);
+          if (bar_or(1 + sg, 128, (see && mx > kPfLazy) || bad)) {
+            // a column's max moves, or a wait ran out somewhere
+            if (bar_or(1 + sg, 128, bad)) {
+              ok = false;
+              break;
+            }
+            sh_ld<SUB>(ts, x);
+            float mine = -INFINITY;  // the warp's max of column c0 + lane
+#pragma unroll
+            for (int i = 0; i < SUB; ++i) {
+              float v;
+              asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(v) : "f"(see ? x[i] : -INFINITY));
+              if (lane == i) mine = v;
+            }
+            if (lane < SUB) s_cm[warp & 3][c0 + lane] = mine * p.qscale;
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + sg) : "memory");
+            if ((warp & 3) == 0 && lane < SUB) {
+              const int c = c0 + lane;
+              const float top = fmaxf(fmaxf(s_cm[0][c], s_cm[1][c]), fmaxf(s_cm[2][c], s_cm[3][c]));
+              const float old = s_m[c], m = top > old + kPfLazy ? top : old;
+              s_m[c] = m;
+              s_f[c] = fast_exp2(old - m);
+            }
+            // O(n - 1) has to be there before it is rescaled
+            bad = j > 0 && !mbar_wait(&pv_done[buf ^ 1], ((n - 1) >> 1) & 1);
+            __syncwarp();
+            if (bar_or(1 + sg, 128, bad)) {
+              ok = false;
+              break;
+            }
+            if (j > 0) {
+              tc_fence_after();
+              sh_ld<SUB>(tO + c0 + lanes, x);
+#pragma unroll
+              for (int i = 0; i < SUB; ++i) x[i] *= s_f[c0 + i];
+              sh_st<SUB>(tO + c0 + lanes, x);
+              tm_wait_st();
+            }
+#pragma unroll
+            for (int i = 0; i < SUB; ++i) l[s0 + i] *= s_f[c0 + i];
+            scores();
+          }
+          if (!see) {
+#pragma unroll
+            for (int i = 0; i < SUB; ++i) x[i] = -INFINITY;
+          }
+          uint8_t* prow = sP + buf * sh_p_bytes(N) + (c0 >> 6) * 16384 + tok * 128;
+#pragma unroll
+          for (int i = 0; i < SUB; i += 8) {
+            uint32_t pk[4];
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              const float2 y = make_float2(fast_exp2(x[i + e]), fast_exp2(x[i + e + 1]));
+              const float2 z = __fadd2_rn(make_float2(l[s0 + i + e], l[s0 + i + e + 1]), y);
+              l[s0 + i + e] = z.x, l[s0 + i + e + 1] = z.y;
+              pk[e >> 1] = h2u(__floats2half2_rn(y.x, y.y));
+            }
+            *reinterpret_cast<uint4*>(prow + (((((c0 + i) & 63) >> 3) ^ (tok & 7)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+          }
+        }
+        if (!ok) break;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[buf]);
+      }
+      if (ok) {
+        // the piece's partial: O^T from TMEM (lane = dim), m and l per column
+        const int last = n0 + pc.n - 1;
+        const int64_t id = (int64_t)(blockIdx.x + pc.unit) * N;
+        const bool bad = !mbar_wait(&pv_done[last & 1], (last >> 1) & 1);
+        __syncwarp();
+        tc_fence_after();
+        ok = !bar_or(1 + sg, 128, bad);
+        if (ok) {
+#pragma unroll
+          for (int s0 = 0; s0 < COLS; s0 += SUB) {
+            float o[SUB];
+            sh_ld<SUB>(tO + col0 + s0 + lanes, o);
+#pragma unroll
+            for (int i = 0; i < SUB; ++i)
+              if (col0 + s0 + i < rows) p.part_o[(id + col0 + s0 + i) * HKV_D + tok] = o[i];
+            // sums over the warp's tokens: lane ends with column lane % SUB
+#pragma unroll
+            for (int i = 0; i < SUB; ++i) o[i] = l[s0 + i] + (SUB == 16 ? __shfl_xor_sync(0xffffffffu, l[s0 + i], 16) : 0.f);
+#pragma unroll
+            for (int k = SUB / 2; k >= 1; k >>= 1) {
+              const bool up = lane & k;
+#pragma unroll
+              for (int i = 0; i < k; ++i) {
+                const float send = up ? o[i] : o[i + k], keep = up ? o[i + k] : o[i];
+                o[i] = keep + __shfl_xor_sync(0xffffffffu, send, k);
+              }
+            }
+            if (lane < SUB) s_cm[warp & 3][col0 + s0 + lane] = o[0];
+          }
+          asm volatile("bar.sync %0, 128;" ::"r"(1 + sg) : "memory");
+          const int c = col0 + tok;
+          if (tok < COLS && c < rows)
+            *reinterpret_cast<float2*>(p.part_ml + (id + c) * 2) = make_float2(s_m[c], (s_cm[0][c] + s_cm[1][c]) + (s_cm[2][c] + s_cm[3][c]));
+        }
+      }
+    } else if (warp < 4 * SG + 4) {
+      // ---------------- K: thread = token = TMEM lane ----------------
+      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+      for (int j = 0; j < pc.n; ++j) {
+        const int n = n0 + j, buf = n & 1, slot = n % R;
+        bool good = mbar_wait(&raw_full[slot], (n / R) & 1);
+        if (n >= 2) good = mbar_wait(&s_full[buf], ((n >> 1) - 1) & 1) && good;  // S(n - 2) has read K[buf]
+        if (!__all_sync(0xffffffffu, good)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        sh_convert_k<FMT, GROUP>(raw + slot * kShRawBytes, tmem + 64 * buf + lanes, t & 127, (t & 127) < s_valid[n & 15]);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&k_full[buf]);
+          mbar_arrive(&raw_free[slot]);
+        }
+      }
+    } else if (warp < 4 * SG + 8) {
+      // ---------------- V ----------------
+      for (int j = 0; j < pc.n; ++j) {
+        const int n = n0 + j, buf = n & 1, slot = n % R;
+        bool good = mbar_wait(&raw_full[slot], (n / R) & 1);
+        if (n >= 2) good = mbar_wait(&pv_done[buf], ((n >> 1) - 1) & 1) && good;  // O(n - 2) has read Vt[buf]
+        if (!__all_sync(0xffffffffu, good)) {
+          ok = false;
+          break;
+        }
+        pf_convert_v<FMT, GROUP>(raw + slot * kShRawBytes, sV + buf * kPfTileBytes, t & 127, s_valid[n & 15]);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&v_full[buf]);
+          mbar_arrive(&raw_free[slot]);
+        }
+      }
+    } else if (warp == 4 * SG + 8) {
+      // ---------------- producer ----------------
+      const int u = pc.g * p.Hkv + pc.h;
+      const int len = max(0, p.prefix.lengths ? p.prefix.lengths[pc.g] : p.prefix.len);
+      int64_t ids = -1;
+      for (int j = 0; j < pc.n; ++j) {
+        const int n = n0 + j, slot = n % R, tok = (pc.t0 + j) * HKV_BLOCK_TOKENS;
+        if ((j & 31) == 0) ids = j + lane < pc.n ? store_page(p.prefix, u, tok + lane * HKV_BLOCK_TOKENS) : -1;
+        const int64_t page = __shfl_sync(0xffffffffu, ids, j & 31);
+        if (n >= R && !__all_sync(0xffffffffu, mbar_wait(&raw_free[slot], (n / R - 1) & 1, 1000))) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          s_valid[n & 15] = page >= 0 ? min(HKV_BLOCK_TOKENS, len - tok) : 0;
+          if (page >= 0) {
+            const uint8_t* src = static_cast<const uint8_t*>(p.prefix.pages) + page * p.prefix.page_stride +
+                                 (int64_t)((tok % p.prefix.page_tokens) / HKV_BLOCK_TOKENS) * kBlock;
+            mbar_arrive_expect_tx(&raw_full[slot], kBlock);
+            bulk_g2s(raw + slot * kShRawBytes, src, kBlock, &raw_full[slot]);
+          } else {  // no such page: the tile counts as hidden, its bytes are the last tile's
+            hkv_flag_error(HKV_DEVERR_BAD_PAGE);
+            mbar_arrive(&raw_full[slot]);
+          }
+        }
+        __syncwarp();
+        issued = n + 1;
+      }
+      if (!ok)  // copies in flight land before the CTA ends
+        for (int n = max(0, issued - R); n < issued; ++n) mbar_wait(&raw_full[n % R], (n / R) & 1);
+    } else if (lane == 0) {
+      // ---------------- MMA ----------------
+      const uint32_t q0 = smem_u32(sQ), v0 = smem_u32(sV), p0 = smem_u32(sP);
+      auto scores = [&](int n) {  // S^T(n) = K(n) Q^T; its buffer was read before P(n - 2) was announced
+        const int buf = n & 1;
+        if (!mbar_wait(&k_full[buf], (n >> 1) & 1)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          sh_mma_ts(tS + buf * N, tmem + 64 * buf + 8 * kk, pf_desc(q0 + (kk >> 2) * (N * 128) + (kk & 3) * 32),
+                    sh_idesc(N, false), kk > 0);
+        pf_commit(&s_full[buf]);
+        issued = 1;
+        return true;
+      };
+      ok = scores(n0);
+      for (int j = 0; ok && j < pc.n; ++j) {
+        const int n = n0 + j, buf = n & 1;
+        if (j + 1 < pc.n) ok = scores(n + 1);
+        ok = ok && mbar_wait(&v_full[buf], (n >> 1) & 1) && mbar_wait(&p_full[buf], (n >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          sh_mma_ss(tO, pf_desc(v0 + buf * kPfTileBytes + (kk >> 2) * 16384 + (kk & 3) * 32),
+                    sh_desc_n(p0 + buf * sh_p_bytes(N) + kk * 2048), sh_idesc(N, true), j > 0 || kk > 0);
+        pf_commit(&pv_done[buf]);
+      }
+      if (!ok && issued) {  // products in flight end before TMEM is freed
+        pf_commit(&drain);
+        mbar_wait(&drain, 0);
+      }
+    }
+    __syncwarp();
+    ok = __syncthreads_and(ok);
+    n0 += pc.n;
+    if (!ok) break;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kCols));
+  }
+}
+
+// out[b][hq] from the partials of the row's pieces and of its own tokens, one warp
+// per row, lane = dims 4 lane .. 4 lane + 3: sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.
+__global__ void __launch_bounds__(256) shared_merge_kernel(const __grid_constant__ SharedParams p) {
+  __shared__ ShGroup s_g[kShMaxGroups + 1];
+  griddep_wait();
+  griddep_launch_dependents();
+  if (threadIdx.x < 32) sh_schedule(p, s_g);
+  __syncthreads();
+  const int Hq = p.Hkv * p.G, row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= p.B * Hq) return;
+  const int b = row / Hq, hq = row - b * Hq, h = hq / p.G;
+  const int total = s_g[p.P].step;
+  int g = 0;
+  for (int hi = p.P; g < hi;) {  // the first group that ends behind b
+    const int mid = (g + hi) >> 1;
+    if (p.start[mid + 1] > b) hi = mid;
+    else g = mid + 1;
+  }
+  int c0 = 0, c1 = -1, unit = 0, n = 0;
+  if (g < p.P && p.start[g] <= b && s_g[g + 1].step > s_g[g].step) {
+    const int units = s_g[g + 1].unit - s_g[g].unit, per = (s_g[g + 1].step - s_g[g].step) / units, rts = units / p.Hkv;
+    const int r = (b - p.start[g]) * p.G + hq - h * p.G, rt = r / p.N, u = h * rts + rt;
+    n = r - rt * p.N;
+    unit = s_g[g].unit + u;
+    const int first = s_g[g].step + u * per + kShCharge, last = first + per - kShCharge - 1;
+    auto cta = [&](int step) {
+      int c = (int)((int64_t)step * p.C / total);
+      while (c + 1 < p.C && sh_cut(total, p.C, c + 1) <= step) ++c;
+      while (c > 0 && sh_cut(total, p.C, c) > step) --c;
+      return c;
+    };
+    c0 = cta(first);
+    c1 = cta(last);
+  }
+  float M = -1.0e30f, L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](const float* o, float m, float l) {
+    const float4 v = *reinterpret_cast<const float4*>(o + 4 * lane);
+    const float nm = fmaxf(M, m), a = fast_exp2(M - nm), w = fast_exp2(m - nm);
+    M = nm;
+    L = L * a + l * w;
+    acc = make_float4(acc.x * a + v.x * w, acc.y * a + v.y * w, acc.z * a + v.z * w, acc.w * a + v.w * w);
+  };
+  if (p.own_o) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.own_ml + (int64_t)row * 2);
+    if (ml.y != 0.f) add(p.own_o + (int64_t)row * HKV_D, ml.x, ml.y);
+  }
+  for (int c = c0; c <= c1; ++c) {
+    if (sh_cut(total, p.C, c) == sh_cut(total, p.C, c + 1)) continue;  // more CTAs than steps
+    const int64_t id = (int64_t)(c + unit) * p.N + n;
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + id * 2);
+    if (ml.y != 0.f) add(p.part_o + id * HKV_D, ml.x, ml.y);
+  }
+  const float inv = L != 0.f ? 1.f / L : 0.f;  // a NaN stays one
+  const int64_t ob = (int64_t)b * p.out_sb + (int64_t)hq * p.out_sh + 4 * lane;
+  const float v[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) store_any(p.out, p.out_dtype, ob + i, v[i] * inv);
+}
+
+}  // namespace hkv

@@ -10,7 +10,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
-from typing import Optional, Tuple, Union
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -747,3 +747,83 @@ def norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: O
             64 if rot and positions.dtype == torch.int64 else 32, ps_b, ps_t, table.data_ptr() if rot else None,
             tstride, max_pos, rot, int(bool(adjacent)), _stream()), "hkv_norm_rope")
     return outs[0], outs[1]
+
+
+class SharedPrefix:
+    """A prefix shared by groups of a batch's sequences: ``store`` holds one
+    prefix per group (its batch is the number of groups), and the sequences
+    [group_start[p], group_start[p + 1]) attend to prefix p; sequences outside
+    have none. ``group_start``: plain ints, fixed for the object's life (they
+    size the launches); the prefixes may still grow (``store.lengths``)."""
+
+    def __init__(self, store: Int4KVStore, group_start: Sequence[int]):
+        starts = [int(x) for x in group_start]
+        if len(starts) != store.batch + 1:
+            raise ValueError(f"group_start needs {store.batch + 1} entries for {store.batch} prefixes")
+        if starts[0] < 0 or any(b < a for a, b in zip(starts, starts[1:])):
+            raise ValueError("group_start must not decrease, nor be negative")
+        self.store = store
+        self.group_start = starts
+        self._starts = (ctypes.c_int32 * len(starts))(*starts)
+
+
+def decode_shared(q: torch.Tensor, prefix: SharedPrefix, store: Optional[Int4KVStore] = None,
+                  dense: Optional[DenseKV] = None, sm_scale: Optional[float] = None,
+                  out_dtype: torch.dtype = torch.float32, ctas: int = 0, out: Optional[torch.Tensor] = None,
+                  body_len: Optional[int] = None, dense_len: Optional[int] = None, stream=None) -> torch.Tensor:
+    """``decode`` for a batch whose sequences share INT4 prefixes (samples of one
+    prompt, beams, a system prompt): attention of q [B, Hq, 128] (or [B, Hq, 1,
+    128]) over [prefix of the sequence's group ; its INT4 body ; its dense
+    segment], each prefix read once per KV head for its whole group. ``store``
+    and ``dense`` as in ``decode``, or None. Returns [B, Hq, 128] in
+    ``out_dtype``; a row that sees no token is zero."""
+    _require_cuda(q)
+    if q.dim() not in (3, 4) or (q.dim() == 4 and q.shape[2] != 1):
+        raise ValueError("q must be [B, Hq, 128] or [B, Hq, 1, 128]")
+    squeeze = q.dim() == 4
+    if squeeze:
+        q = q[:, :, 0]
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    B, Hq, D = q.shape
+    Hkv = prefix.store.kv_heads
+    for seg in (store, dense):
+        if seg is not None and (seg.batch != B or seg.kv_heads != Hkv):
+            raise ValueError(f"the own segments must hold {B} sequences of {Hkv} KV heads")
+    if prefix.group_start[-1] > B:
+        raise ValueError(f"group_start goes to {prefix.group_start[-1]}, beyond the batch of {B}")
+    if any(t.device != q.device for t in (prefix.store.pool, *((store.pool,) if store else ()), *((dense.k,) if dense else ()))):
+        raise ValueError("q and the caches must be on one device")
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(D)
+    if out is not None and (out.shape != q.shape or out.stride(2) != 1 or out.device != q.device):
+        raise ValueError("out must be [B, Hq, 128] on q's device with a contiguous head dimension")
+    with launch_on(q.device, stream):
+        if out is None:
+            out = torch.empty(B, Hq, D, dtype=out_dtype, device=q.device)
+        G = Hq // Hkv
+        if G > 8 and Hq % Hkv == 0 and (store is not None or dense is not None):
+            gs = max(d for d in range(1, 9) if G % d == 0)  # as in ``decode``
+            qg, og = q.reshape(B, Hkv, G // gs, gs, D), torch.empty(B, Hkv, G // gs, gs, D, dtype=out.dtype, device=q.device)
+            for k in range(G // gs):
+                og[:, :, k] = decode_shared(qg[:, :, k].reshape(B, Hkv * gs, D), prefix, store, dense, sm_scale, out.dtype,
+                                            ctas, None, body_len, dense_len).view(B, Hkv, gs, D)
+            out.copy_(og.view(B, Hq, D))
+            return out[:, :, None, :] if squeeze else out
+        pf = prefix.store.struct()
+        st = store.struct(body_len) if store is not None else None
+        ds = dense.struct(dense_len) if dense is not None else None
+        segs = (ctypes.byref(pf), prefix._starts, prefix.store.batch, ctypes.byref(st) if st is not None else None,
+                ctypes.byref(ds) if ds is not None else None)
+        lib = L.load()
+        nbytes = lib.hkv_decode_shared_workspace_bytes(*segs, B, Hq, Hkv, D, ctas)
+        if nbytes == 0:
+            raise RuntimeError("hkv_decode_shared_workspace_bytes: unsupported decode configuration")
+        # a captured call gets memory of its graph's own, so that graphs replayed side by side do not share it
+        ws = (torch.empty(nbytes, dtype=torch.uint8, device=q.device) if torch.cuda.is_current_stream_capturing()
+              else workspace(nbytes, q.device, kind="shared"))
+        L.check(lib.hkv_decode_shared(
+            q.data_ptr(), dtype_code(q.dtype), q.stride(0), q.stride(1), *segs, B, Hq, Hkv, D, float(sm_scale), ctas,
+            ws.data_ptr(), ws.numel(), out.data_ptr(), dtype_code(out.dtype), out.stride(0), out.stride(1), _stream()),
+            "hkv_decode_shared")
+    return out[:, :, None, :] if squeeze else out

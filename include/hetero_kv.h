@@ -506,6 +506,33 @@ hkv_status hkv_pages_reserve(const hkv_int4_store* store, int32_t B, int32_t H, 
 hkv_status hkv_pages_compact(const hkv_int4_store* src, int32_t B, int32_t H, const hkv_int4_store* into,
                              int32_t* into_refs, void* workspace, size_t workspace_bytes, hkv_stream_t stream);
 
+/* ---------------------------------------------------------------- 7. decode over a shared prefix
+ * hkv_decode_attn for sequences that share INT4 prefixes: the sequences
+ * [group_start[p], group_start[p + 1]) (group_start: HOST array of n_groups + 1
+ * non-decreasing ints in [0, B]) attend to prefix p (units p*Hkv + h of the
+ * store `prefix`, whose lengths are [n_groups]) and to their own body and dense
+ * segment (either or both may be NULL); a sequence outside every group has no
+ * prefix. Attention does not depend on the order of the keys, so the prefix may
+ * stand for any shared tokens. Each prefix is read once per KV head and up to 128
+ * rows (sequences x G) instead of once per sequence. A row that sees no token
+ * gives zeros. G = Hq/Hkv <= 8 with a body or a dense segment, else any.
+ * Precision: as hkv_decode_attn for the own part; for the prefix K, V and P are
+ * f16 (K and V dequantised in f16, a bf16 query rounded to it), sums and the
+ * softmax statistics fp32. Three launches on `stream` (prefix, own part, merge).
+ * Workspace: hkv_decode_shared_workspace_bytes, 16-byte aligned, no initial
+ * contents; calls that overlap on the GPU must use different ones.
+ * n_groups <= HKV_SHARED_MAX_GROUPS. */
+#define HKV_SHARED_MAX_GROUPS 512
+size_t hkv_decode_shared_workspace_bytes(const hkv_int4_store* prefix, const int32_t* group_start, int32_t n_groups,
+                                         const hkv_int4_store* body, const hkv_dense_kv* dense, int32_t B,
+                                         int32_t Hq, int32_t Hkv, int32_t D, int32_t ctas);
+hkv_status hkv_decode_shared(const void* q, int32_t q_dtype, int64_t q_stride_b, int64_t q_stride_h,
+                             const hkv_int4_store* prefix, const int32_t* group_start, int32_t n_groups,
+                             const hkv_int4_store* body, const hkv_dense_kv* dense, int32_t B, int32_t Hq,
+                             int32_t Hkv, int32_t D, float sm_scale, int32_t ctas, void* workspace,
+                             size_t workspace_bytes, void* out, int32_t out_dtype, int64_t out_stride_b,
+                             int64_t out_stride_h, hkv_stream_t stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif
