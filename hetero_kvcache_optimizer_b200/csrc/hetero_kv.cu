@@ -1583,7 +1583,7 @@ hkv_status hkv_decode_shared(const void* q, int32_t q_dtype, int64_t q_stride_b,
                     HKV_DT_F32, 0, 0, const_cast<float*>(p.own_o), const_cast<float*>(p.own_ml), S(stream));
     if (rc != HKV_OK) return rc;
   }
-  const cudaError_t e = launch_pdl(8, hkv::shared_merge_kernel, dim3(cdiv((int64_t)B * Hq, 8)), dim3(256), 0, S(stream), p);
+  const cudaError_t e = launch_pdl(8, hkv::shared_merge_kernel, dim3(B * Hq), dim3(128), 0, S(stream), p);
   return e == cudaSuccess ? launch_status() : cuda_fail(e);
 }
 

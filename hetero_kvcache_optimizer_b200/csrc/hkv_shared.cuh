@@ -37,8 +37,10 @@ constexpr int kShMaxGroups = 512;
 constexpr int kShCharge = 6;
 constexpr int kShRawBytes = 24 * 1024;
 
-constexpr int sh_softmax_groups(int n) { return n <= 32 ? 1 : 2; }
-constexpr int sh_threads(int n) { return 32 * (4 * sh_softmax_groups(n) + 10); }
+// Warps: groups of four softmax warps (kShCols rows each) | K | V | producer, MMA.
+constexpr int sh_softmax_groups(int n) { return n <= 16 ? 1 : n <= 64 ? 2 : 4; }
+constexpr int sh_halves(int n) { return n <= 64 ? 2 : 1; }  // warps that share a token's K (a dim's V)
+constexpr int sh_threads(int n) { return 32 * (4 * sh_softmax_groups(n) + 8 * sh_halves(n) + 2); }
 constexpr int sh_slots(int n) { return n <= 64 ? 4 : 2; }
 constexpr int sh_p_bytes(int n) { return 128 * 128 * (n <= 64 ? 1 : 2); }  // [token][64 rows] f16 blocks
 constexpr int sh_smem(int n) {  // Q | Vt[2] | P[2] | raw slots | alignment
@@ -199,44 +201,52 @@ __device__ __forceinline__ bool bar_or(int id, int n, bool v) {
   return r != 0;
 }
 
+// One lane of a converged warp, in a form by which the compiler knows that a
+// single thread follows: under `lane == 0` each tcgen05.mma was issued through a
+// loop over the active lanes, 57 cycles apiece instead of 10.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e != 0;
+}
+
 // Dims of 16-byte chunk kc (8 values) of Q's and K's common order: value 2 c + e
 // is dim 32 (kc / 4) + 8 c + 2 (kc % 4) + e, the order in which nib8_to_h2 yields
 // a K token's words, so that K needs no shuffling on its way into TMEM.
 __device__ __forceinline__ int sh_dim(int kc, int c) { return 32 * (kc >> 2) + 8 * c + 2 * (kc & 3); }
 
-// K of token t (thread t) of the raw block into TMEM lane t, columns [0, 64).
-// A token's four 16-byte chunks are read in an order rotated by t / 2, so that
-// the 8 threads of a load phase hit 8 distinct bank groups, and rotated back.
-template <int FMT, int GROUP>
-__device__ __forceinline__ void sh_convert_k(const uint8_t* rb, uint32_t tmem, int t, bool valid) {
+// Words 2 half .. 2 half + 1 (HALVES == 2) or all four of each 16-byte chunk of K
+// token t (thread t) of the raw block into TMEM lane t, columns 32 half .. + 31 (all
+// 64). The chunks are read in an order rotated by t / 2, so that a load phase
+// spreads over the banks, and rotated back with selects.
+template <int FMT, int GROUP, int HALVES>
+__device__ __forceinline__ void sh_convert_k(const uint8_t* rb, uint32_t tmem, int t, int half0, bool valid) {
   constexpr int NG = HKV_D / GROUP;
-  uint4 v[4], u[4];
   const int rot = (t >> 1) & 3;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(rb + t * 64 + (((j + rot) & 3) << 4));
   const bool r1 = rot & 1, r2 = rot & 2;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) u[j] = r1 ? v[(j + 3) & 3] : v[j];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = r2 ? u[(j + 2) & 3] : u[j];
   const uint8_t* meta = rb + HKV_META_OFF;
-  __half ks[NG], km[NG];
-  if constexpr (FMT == HKV_FMT_FP16MIN) vload_h<NG>(meta + 2 * NG * t, ks), vload_h<NG>(meta + 256 * NG + 2 * NG * t, km);
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
+  for (int hh = 0; hh < 2 / HALVES; ++hh) {
+    const int half = HALVES == 2 ? half0 : hh;
+    uint2 v[4], u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint2*>(rb + t * 64 + (((j + rot) & 3) << 4) + 8 * half);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u[j].x = r1 ? v[(j + 3) & 3].x : v[j].x, u[j].y = r1 ? v[(j + 3) & 3].y : v[j].y;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j].x = r2 ? u[(j + 2) & 3].x : u[j].x, v[j].y = r2 ? u[(j + 2) & 3].y : u[j].y;
     uint32_t o[32];
 #pragma unroll
-    for (int w2 = 0; w2 < 2; ++w2) {
-      const int w = 2 * half + w2, g = (32 * w) / GROUP;
+    for (int w = 0; w < 2; ++w) {  // dims 32 (2 half + w) .. + 31
+      const int g = (2 * half + w) * 32 / GROUP;
       __half2 s2, m2;
       uint32_t zlo = 0, zhi = 0;
       if constexpr (FMT == HKV_FMT_FP16MIN) {
-        s2 = __half2half2(ks[g]);
-        m2 = __half2half2(km[g]);
+        s2 = __half2half2(reinterpret_cast<const __half*>(meta)[t * NG + g]);
+        m2 = __half2half2(reinterpret_cast<const __half*>(meta + 256 * NG)[t * NG + g]);
       } else {
-        const float s = reinterpret_cast<const float*>(meta)[t * NG + g];
         const uint32_t z = meta[1024 * NG + t * NG + g];
-        s2 = __float2half2_rn(s);
+        s2 = __float2half2_rn(reinterpret_cast<const float*>(meta)[t * NG + g]);
         m2 = __float2half2_rn(0.f);
         zlo = h2u(__float2half2_rn(1024.f + (float)z));
         zhi = h2u(__float2half2_rn(-64.f - (float)z));
@@ -244,12 +254,11 @@ __device__ __forceinline__ void sh_convert_k(const uint8_t* rb, uint32_t tmem, i
       if (!valid) s2 = m2 = __float2half2_rn(0.f);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t wd = w == 0 ? v[j].x : w == 1 ? v[j].y : w == 2 ? v[j].z : v[j].w;
         uint32_t h[4];
-        if constexpr (FMT == HKV_FMT_FP16MIN) nib8_to_h2(wd, h);
-        else nib8_to_h2_z(wd, zlo, zhi, h);
+        if constexpr (FMT == HKV_FMT_FP16MIN) nib8_to_h2(w ? v[j].y : v[j].x, h);
+        else nib8_to_h2_z(w ? v[j].y : v[j].x, zlo, zhi, h);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[16 * w2 + 4 * j + c] = h2u(__hfma2(u2h(h[c]), s2, m2));
+        for (int c = 0; c < 4; ++c) o[16 * w + 4 * j + c] = h2u(__hfma2(u2h(h[c]), s2, m2));
       }
     }
     tm_st32u(tmem + 32 * half, o);
@@ -257,17 +266,72 @@ __device__ __forceinline__ void sh_convert_k(const uint8_t* rb, uint32_t tmem, i
   tm_wait_st();
 }
 
+// V of the raw block into sVt ([dim][token], 128-byte swizzle), as pf_convert_v:
+// thread t has tokens 8 o .. 8 o + 7 (o = t / 8) and chunk i = t % 8 of their four
+// pairs, here words 2 half .. 2 half + 1 of it (HALVES == 2) or all four. Tokens at
+// and behind `valid` become zero (their P is zero and their bytes may be any bits).
+template <int FMT, int GROUP, int HALVES>
+__device__ __forceinline__ void sh_convert_v(const uint8_t* rb, uint8_t* sVt, int t, int half0, int valid) {
+  constexpr int NG = HKV_D / GROUP;
+  const int o = t >> 3, i = t & 7;
+  const uint8_t* meta = rb + HKV_META_OFF;
+#pragma unroll
+  for (int hh = 0; hh < 2 / HALVES; ++hh) {
+    const int half = HALVES == 2 ? half0 : hh;
+    uint2 cw[4];
+#pragma unroll
+    for (int pp = 0; pp < 4; ++pp) cw[pp] = *reinterpret_cast<const uint2*>(rb + HKV_V_CODES_OFF + v_chunk_off(4 * o + pp, i) + 8 * half);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const int k = 2 * half + w, g = 32 * k / GROUP;
+      uint32_t h[4][4];  // [pair][nibble m], then the values
+#pragma unroll
+      for (int pp = 0; pp < 4; ++pp) {
+        const int q = 4 * o + pp;  // tokens 2 q, 2 q + 1
+        __half2 s2, m2;
+        const uint32_t wd = w ? cw[pp].y : cw[pp].x;
+        if constexpr (FMT == HKV_FMT_FP16MIN) {
+          s2 = reinterpret_cast<const __half2*>(meta + 512 * NG)[q * NG + g];
+          m2 = reinterpret_cast<const __half2*>(meta + 768 * NG)[q * NG + g];
+        } else {
+          const float* vs = reinterpret_cast<const float*>(meta + 512 * NG);
+          s2 = __floats2half2_rn(vs[2 * q * NG + g], vs[(2 * q + 1) * NG + g]);
+          m2 = __float2half2_rn(0.f);
+        }
+        if (valid < HKV_BLOCK_TOKENS) {
+          const uint32_t keep = (2 * q < valid ? 0x0000FFFFu : 0u) | (2 * q + 1 < valid ? 0xFFFF0000u : 0u);
+          s2 = u2h(h2u(s2) & keep);
+          m2 = u2h(h2u(m2) & keep);
+        }
+        if constexpr (FMT == HKV_FMT_FP16MIN) {
+          nib8_to_h2(wd, h[pp]);
+        } else {
+          const uint8_t* vz = meta + 1152 * NG;
+          const float za = (float)vz[2 * q * NG + g], zb = (float)vz[(2 * q + 1) * NG + g];
+          nib8_to_h2_z(wd, h2u(__floats2half2_rn(1024.f + za, 1024.f + zb)), h2u(__floats2half2_rn(-64.f - za, -64.f - zb)), h[pp]);
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) h[pp][m] = h2u(__hfma2(u2h(h[pp][m]), s2, m2));
+      }
+#pragma unroll
+      for (int m = 0; m < 4; ++m)  // dim i + 32 k + 8 m
+        *reinterpret_cast<uint4*>(sVt + pf_chunk(i + 32 * k + 8 * m, o)) = make_uint4(h[0][m], h[1][m], h[2][m], h[3][m]);
+    }
+  }
+}
+
 template <int FMT, int GROUP, int N>
 __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const __grid_constant__ SharedParams p) {
   constexpr int SG = sh_softmax_groups(N);   // softmax groups of 128 threads
   constexpr int COLS = N / SG;               // columns of a softmax thread
-  constexpr int SUB = COLS < 32 ? COLS : 32; // taken at a time
+  constexpr int SUB = 16;                    // taken at a time
+  constexpr int KH = sh_halves(N);           // K (and V) warps = 4 KH
   constexpr int R = sh_slots(N);
   constexpr int kThreads = sh_threads(N);
   constexpr uint32_t kBlock = block_bytes(FMT, GROUP);
   constexpr uint32_t kCols = sh_tmem_cols(N);
   extern __shared__ __align__(1024) uint8_t sh_raw[];
-  __shared__ __align__(8) uint64_t raw_full[R], raw_free[R], k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], drain;
+  __shared__ __align__(8) uint64_t raw_full[R], raw_free[R], k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], q_full, drain;
   __shared__ uint32_t s_tmem;
   __shared__ ShGroup s_g[kShMaxGroups + 1];
   __shared__ int s_valid[16];        // tokens in use of tile n & 15
@@ -283,15 +347,16 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
   if (t == 0) {
     for (int i = 0; i < R; ++i) {
       mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_free[i], 8);
+      mbar_init(&raw_free[i], 8 * KH);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&k_full[i], 4);
-      mbar_init(&v_full[i], 4);
+      mbar_init(&k_full[i], 4 * KH);
+      mbar_init(&v_full[i], 4 * KH);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4 * SG);
       mbar_init(&pv_done[i], 1);
     }
+    mbar_init(&q_full, 4 * SG);
     mbar_init(&drain, 1);
     fence_barrier_init();
   }
@@ -310,38 +375,39 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
   const int total = s_g[p.P].step;
   int at = sh_cut(total, p.C, blockIdx.x);
   const int end = sh_cut(total, p.C, blockIdx.x + 1);
-  int n0 = 0;       // tiles of the CTA before this piece
+  int n0 = 0, pieces = 0;  // tiles and pieces of the CTA before this one
   int issued = 0;   // producer: copies; MMA warp: whether there are products
   bool ok = true;
 
   while (true) {
     const ShPiece pc = sh_next(p, s_g, at, end);
     if (pc.n == 0) break;
-    // the piece's query rows, in K's dim order
     const int rows = (p.start[pc.g + 1] - p.start[pc.g]) * p.G - pc.rt * N;
-    for (int c = t; c < N * 16; c += kThreads) {
-      const int n = c >> 4, kc = c & 15;
-      uint32_t o[4] = {0u, 0u, 0u, 0u};
-      if (n < rows) {
-        const int r = pc.rt * N + n, s = r / p.G;
-        const int64_t base = (int64_t)(p.start[pc.g] + s) * p.q_sb + (int64_t)(pc.h * p.G + r - s * p.G) * p.q_sh;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int64_t i = base + sh_dim(kc, e);
-          o[e] = h2u(__floats2half2_rn(load_any(p.q, p.q_dtype, i), load_any(p.q, p.q_dtype, i + 1)));
-        }
-      }
-      *reinterpret_cast<uint4*>(sQ + (kc >> 3) * (N * 128) + n * 128 + (((kc & 7) ^ (n & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-    }
-    if (t < N) s_m[t] = -1.0e30f;
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncthreads();
-
     if (warp < 4 * SG) {
       // ---------------- softmax: thread = token, columns [col0, col0 + COLS) ----------------
       const int sg = warp >> 2, tok = t & 127, col0 = sg * COLS;
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const float2 qs2 = make_float2(p.qscale, p.qscale);
+      // the piece's query rows, in K's dim order
+      for (int c = t; c < N * 16; c += 128 * SG) {
+        const int n = c >> 4, kc = c & 15;
+        uint32_t o[4] = {0u, 0u, 0u, 0u};
+        if (n < rows) {
+          const int r = pc.rt * N + n, sq = r / p.G;
+          const int64_t base = (int64_t)(p.start[pc.g] + sq) * p.q_sb + (int64_t)(pc.h * p.G + r - sq * p.G) * p.q_sh;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int64_t i = base + sh_dim(kc, e);
+            o[e] = h2u(__floats2half2_rn(load_any(p.q, p.q_dtype, i), load_any(p.q, p.q_dtype, i + 1)));
+          }
+        }
+        *reinterpret_cast<uint4*>(sQ + (kc >> 3) * (N * 128) + n * 128 + (((kc & 7) ^ (n & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full);
+      if (tok < COLS) s_m[col0 + tok] = -1.0e30f;
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + sg) : "memory");
       float l[COLS];
 #pragma unroll
       for (int i = 0; i < COLS; ++i) l[i] = 0.f;
@@ -473,9 +539,10 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
             *reinterpret_cast<float2*>(p.part_ml + (id + c) * 2) = make_float2(s_m[c], (s_cm[0][c] + s_cm[1][c]) + (s_cm[2][c] + s_cm[3][c]));
         }
       }
-    } else if (warp < 4 * SG + 4) {
+    } else if (warp < 4 * SG + 4 * KH) {
       // ---------------- K: thread = token = TMEM lane ----------------
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+      const int half = (warp - 4 * SG) >> 2;
       for (int j = 0; j < pc.n; ++j) {
         const int n = n0 + j, buf = n & 1, slot = n % R;
         bool good = mbar_wait(&raw_full[slot], (n / R) & 1);
@@ -485,7 +552,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
           break;
         }
         tc_fence_after();
-        sh_convert_k<FMT, GROUP>(raw + slot * kShRawBytes, tmem + 64 * buf + lanes, t & 127, (t & 127) < s_valid[n & 15]);
+        sh_convert_k<FMT, GROUP, KH>(raw + slot * kShRawBytes, tmem + 64 * buf + lanes, t & 127, half, (t & 127) < s_valid[n & 15]);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
@@ -493,8 +560,9 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
           mbar_arrive(&raw_free[slot]);
         }
       }
-    } else if (warp < 4 * SG + 8) {
+    } else if (warp < 4 * SG + 8 * KH) {
       // ---------------- V ----------------
+      const int half = (warp - 4 * SG - 4 * KH) >> 2;
       for (int j = 0; j < pc.n; ++j) {
         const int n = n0 + j, buf = n & 1, slot = n % R;
         bool good = mbar_wait(&raw_full[slot], (n / R) & 1);
@@ -503,7 +571,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
           ok = false;
           break;
         }
-        pf_convert_v<FMT, GROUP>(raw + slot * kShRawBytes, sV + buf * kPfTileBytes, t & 127, s_valid[n & 15]);
+        sh_convert_v<FMT, GROUP, KH>(raw + slot * kShRawBytes, sV + buf * kPfTileBytes, t & 127, half, s_valid[n & 15]);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) {
@@ -511,7 +579,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
           mbar_arrive(&raw_free[slot]);
         }
       }
-    } else if (warp == 4 * SG + 8) {
+    } else if (warp == 4 * SG + 8 * KH) {
       // ---------------- producer ----------------
       const int u = pc.g * p.Hkv + pc.h;
       const int len = max(0, p.prefix.lengths ? p.prefix.lengths[pc.g] : p.prefix.len);
@@ -541,7 +609,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
       }
       if (!ok)  // copies in flight land before the CTA ends
         for (int n = max(0, issued - R); n < issued; ++n) mbar_wait(&raw_full[n % R], (n / R) & 1);
-    } else if (lane == 0) {
+    } else if (elect_one()) {
       // ---------------- MMA ----------------
       const uint32_t q0 = smem_u32(sQ), v0 = smem_u32(sV), p0 = smem_u32(sP);
       auto scores = [&](int n) {  // S^T(n) = K(n) Q^T; its buffer was read before P(n - 2) was announced
@@ -556,7 +624,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
         issued = 1;
         return true;
       };
-      ok = scores(n0);
+      ok = mbar_wait(&q_full, pieces & 1) && scores(n0);
       for (int j = 0; ok && j < pc.n; ++j) {
         const int n = n0 + j, buf = n & 1;
         if (j + 1 < pc.n) ok = scores(n + 1);
@@ -577,6 +645,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
     __syncwarp();
     ok = __syncthreads_and(ok);
     n0 += pc.n;
+    ++pieces;
     if (!ok) break;
   }
   tc_fence_before();
@@ -587,16 +656,19 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
   }
 }
 
-// out[b][hq] from the partials of the row's pieces and of its own tokens, one warp
-// per row, lane = dims 4 lane .. 4 lane + 3: sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.
-__global__ void __launch_bounds__(256) shared_merge_kernel(const __grid_constant__ SharedParams p) {
+// out[b][hq] from the partials of the row's pieces and of its own tokens:
+// sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i. Four warps per row, each a quarter
+// of the partials (lane = dims 4 lane .. 4 lane + 3), all (m, l) and then several
+// O loaded at once: the launch is a few round trips to L2, not one per partial.
+__global__ void __launch_bounds__(128) shared_merge_kernel(const __grid_constant__ SharedParams p) {
   __shared__ ShGroup s_g[kShMaxGroups + 1];
+  __shared__ float4 s_o[4][32];
+  __shared__ float2 s_ml[4];
   griddep_wait();
   griddep_launch_dependents();
   if (threadIdx.x < 32) sh_schedule(p, s_g);
   __syncthreads();
-  const int Hq = p.Hkv * p.G, row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= p.B * Hq) return;
+  const int Hq = p.Hkv * p.G, row = blockIdx.x, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int b = row / Hq, hq = row - b * Hq, h = hq / p.G;
   const int total = s_g[p.P].step;
   int g = 0;
@@ -621,24 +693,58 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const __grid_constant
     c0 = cta(first);
     c1 = cta(last);
   }
+  // partial k: the own part (k = 0, when there is one), then the CTAs c0 .. c1
+  const int own = p.own_o ? 1 : 0, parts = own + c1 - c0 + 1;
   float M = -1.0e30f, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](const float* o, float m, float l) {
-    const float4 v = *reinterpret_cast<const float4*>(o + 4 * lane);
-    const float nm = fmaxf(M, m), a = fast_exp2(M - nm), w = fast_exp2(m - nm);
+  for (int k0 = w; k0 < parts; k0 += 128) {  // up to 32 partials of this warp: k0, k0 + 4, ...
+    const int k = k0 + 4 * lane, c = c0 + k - own;
+    float2 ml = make_float2(-1.0e30f, 0.f);
+    const float* src = nullptr;
+    if (k < own) {
+      ml = *reinterpret_cast<const float2*>(p.own_ml + (int64_t)row * 2);
+      src = p.own_o + (int64_t)row * HKV_D;
+    } else if (k < parts && sh_cut(total, p.C, c) < sh_cut(total, p.C, c + 1)) {  // else: more CTAs than steps
+      const int64_t id = (int64_t)(c + unit) * p.N + n;
+      ml = *reinterpret_cast<const float2*>(p.part_ml + id * 2);
+      src = p.part_o + id * HKV_D;
+    }
+    if (ml.y == 0.f) ml.x = -1.0e30f, src = nullptr;  // saw nothing
+    float nm = fmaxf(M, ml.x);
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, x));
+    const float a = fast_exp2(M - nm), wt = src ? fast_exp2(ml.x - nm) : 0.f;
+    float l = src ? ml.y * wt : 0.f;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
     M = nm;
-    L = L * a + l * w;
-    acc = make_float4(acc.x * a + v.x * w, acc.y * a + v.y * w, acc.z * a + v.z * w, acc.w * a + v.w * w);
-  };
-  if (p.own_o) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.own_ml + (int64_t)row * 2);
-    if (ml.y != 0.f) add(p.own_o + (int64_t)row * HKV_D, ml.x, ml.y);
+    L = L * a + l;
+    acc = make_float4(acc.x * a, acc.y * a, acc.z * a, acc.w * a);
+    const int m = min(32, (parts - k0 + 3) / 4);
+#pragma unroll 4
+    for (int i = 0; i < m; ++i) {
+      const float* o = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), i));
+      const float x = __shfl_sync(0xffffffffu, wt, i);
+      if (o) {
+        const float4 v = *reinterpret_cast<const float4*>(o + 4 * lane);
+        acc = make_float4(acc.x + v.x * x, acc.y + v.y * x, acc.z + v.z * x, acc.w + v.w * x);
+      }
+    }
   }
-  for (int c = c0; c <= c1; ++c) {
-    if (sh_cut(total, p.C, c) == sh_cut(total, p.C, c + 1)) continue;  // more CTAs than steps
-    const int64_t id = (int64_t)(c + unit) * p.N + n;
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + id * 2);
-    if (ml.y != 0.f) add(p.part_o + id * HKV_D, ml.x, ml.y);
+  s_o[w][lane] = acc;
+  if (lane == 0) s_ml[w] = make_float2(M, L);
+  __syncthreads();
+  if (w) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) M = fmaxf(M, s_ml[i].x);
+  L = 0.f;
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float x = fast_exp2(s_ml[i].x - M);
+    const float4 v = s_o[i][lane];
+    L += s_ml[i].y * x;
+    acc = make_float4(acc.x + v.x * x, acc.y + v.y * x, acc.z + v.z * x, acc.w + v.w * x);
   }
   const float inv = L != 0.f ? 1.f / L : 0.f;  // a NaN stays one
   const int64_t ob = (int64_t)b * p.out_sb + (int64_t)hq * p.out_sh + 4 * lane;
