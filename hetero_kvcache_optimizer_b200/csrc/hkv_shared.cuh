@@ -39,7 +39,7 @@ constexpr int kShRawBytes = 24 * 1024;
 
 // Warps: groups of four softmax warps (kShCols rows each) | K | V | producer, MMA.
 constexpr int sh_softmax_groups(int n) { return n <= 16 ? 1 : n <= 64 ? 2 : 4; }
-constexpr int sh_halves(int n) { return n <= 64 ? 2 : 1; }  // warps that share a token's K (a dim's V)
+constexpr int sh_halves(int n) { return n <= 64 ? 2 : 1; }  // sets of four K and of four V warps
 constexpr int sh_threads(int n) { return 32 * (4 * sh_softmax_groups(n) + 8 * sh_halves(n) + 2); }
 constexpr int sh_slots(int n) { return n <= 64 ? 4 : 2; }
 constexpr int sh_p_bytes(int n) { return 128 * 128 * (n <= 64 ? 1 : 2); }  // [token][64 rows] f16 blocks
@@ -210,40 +210,51 @@ __device__ __forceinline__ bool elect_one() {
   return e != 0;
 }
 
+// The kernel's bounded wait: a pending warp sleeps (woken by the phase) instead of
+// polling, since 26 warps that poll take issue slots from those that work.
+__device__ __forceinline__ bool sh_wait(uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, 2000); }
+
 // Dims of 16-byte chunk kc (8 values) of Q's and K's common order: value 2 c + e
 // is dim 32 (kc / 4) + 8 c + 2 (kc % 4) + e, the order in which nib8_to_h2 yields
 // a K token's words, so that K needs no shuffling on its way into TMEM.
 __device__ __forceinline__ int sh_dim(int kc, int c) { return 32 * (kc >> 2) + 8 * c + 2 * (kc & 3); }
 
-// Words 2 half .. 2 half + 1 (HALVES == 2) or all four of each 16-byte chunk of K
-// token t (thread t) of the raw block into TMEM lane t, columns 32 half .. + 31 (all
-// 64). The chunks are read in an order rotated by t / 2, so that a load phase
-// spreads over the banks, and rotated back with selects.
-template <int FMT, int GROUP, int HALVES>
-__device__ __forceinline__ void sh_convert_k(const uint8_t* rb, uint32_t tmem, int t, int half0, bool valid) {
+// K of token t (thread t) of the raw block into TMEM lane t, columns 0 .. 63. The
+// token's four 16-byte chunks are read in an order rotated by t / 2, so that the 8
+// threads of a load phase hit 8 distinct bank groups, and rotated back with selects.
+template <int FMT, int GROUP>
+__device__ __forceinline__ void sh_convert_k(const uint8_t* rb, uint32_t tmem, int t, bool valid) {
   constexpr int NG = HKV_D / GROUP;
   const int rot = (t >> 1) & 3;
   const bool r1 = rot & 1, r2 = rot & 2;
   const uint8_t* meta = rb + HKV_META_OFF;
+  uint32_t v[4][4], u[4][4];
 #pragma unroll
-  for (int hh = 0; hh < 2 / HALVES; ++hh) {
-    const int half = HALVES == 2 ? half0 : hh;
-    uint2 v[4], u[4];
+  for (int j = 0; j < 4; ++j) {
+    const uint4 c = *reinterpret_cast<const uint4*>(rb + t * 64 + (((j + rot) & 3) << 4));
+    v[j][0] = c.x, v[j][1] = c.y, v[j][2] = c.z, v[j][3] = c.w;
+  }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint2*>(rb + t * 64 + (((j + rot) & 3) << 4) + 8 * half);
+  for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) u[j].x = r1 ? v[(j + 3) & 3].x : v[j].x, u[j].y = r1 ? v[(j + 3) & 3].y : v[j].y;
+    for (int w = 0; w < 4; ++w) u[j][w] = r1 ? v[(j + 3) & 3][w] : v[j][w];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j].x = r2 ? u[(j + 2) & 3].x : u[j].x, v[j].y = r2 ? u[(j + 2) & 3].y : u[j].y;
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) v[j][w] = r2 ? u[(j + 2) & 3][w] : u[j][w];
+  __half ks[NG], km[NG];
+  if constexpr (FMT == HKV_FMT_FP16MIN) vload_h<NG>(meta + 2 * NG * t, ks), vload_h<NG>(meta + 256 * NG + 2 * NG * t, km);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
     uint32_t o[32];
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {  // dims 32 (2 half + w) .. + 31
-      const int g = (2 * half + w) * 32 / GROUP;
+    for (int w2 = 0; w2 < 2; ++w2) {  // dims 32 w .. + 31
+      const int w = 2 * half + w2, g = w * 32 / GROUP;
       __half2 s2, m2;
       uint32_t zlo = 0, zhi = 0;
       if constexpr (FMT == HKV_FMT_FP16MIN) {
-        s2 = __half2half2(reinterpret_cast<const __half*>(meta)[t * NG + g]);
-        m2 = __half2half2(reinterpret_cast<const __half*>(meta + 256 * NG)[t * NG + g]);
+        s2 = __half2half2(ks[g]);
+        m2 = __half2half2(km[g]);
       } else {
         const uint32_t z = meta[1024 * NG + t * NG + g];
         s2 = __float2half2_rn(reinterpret_cast<const float*>(meta)[t * NG + g]);
@@ -255,10 +266,10 @@ __device__ __forceinline__ void sh_convert_k(const uint8_t* rb, uint32_t tmem, i
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint32_t h[4];
-        if constexpr (FMT == HKV_FMT_FP16MIN) nib8_to_h2(w ? v[j].y : v[j].x, h);
-        else nib8_to_h2_z(w ? v[j].y : v[j].x, zlo, zhi, h);
+        if constexpr (FMT == HKV_FMT_FP16MIN) nib8_to_h2(v[j][w], h);
+        else nib8_to_h2_z(v[j][w], zlo, zhi, h);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[16 * w + 4 * j + c] = h2u(__hfma2(u2h(h[c]), s2, m2));
+        for (int c = 0; c < 4; ++c) o[16 * w2 + 4 * j + c] = h2u(__hfma2(u2h(h[c]), s2, m2));
       }
     }
     tm_st32u(tmem + 32 * half, o);
@@ -266,24 +277,26 @@ __device__ __forceinline__ void sh_convert_k(const uint8_t* rb, uint32_t tmem, i
   tm_wait_st();
 }
 
-// V of the raw block into sVt ([dim][token], 128-byte swizzle), as pf_convert_v:
-// thread t has tokens 8 o .. 8 o + 7 (o = t / 8) and chunk i = t % 8 of their four
-// pairs, here words 2 half .. 2 half + 1 of it (HALVES == 2) or all four. Tokens at
-// and behind `valid` become zero (their P is zero and their bytes may be any bits).
-template <int FMT, int GROUP, int HALVES>
-__device__ __forceinline__ void sh_convert_v(const uint8_t* rb, uint8_t* sVt, int t, int half0, int valid) {
+// V of the raw block into sVt ([dim][token], 128-byte swizzle): thread (o, k2, i) has
+// tokens 8 o .. 8 o + 7 and words 2 k2, 2 k2 + 1 of chunk i of their four pairs, so the
+// 16 threads of a load phase read a pair's 128 bytes and the 8 of a store phase hit
+// 8 chunks apart; KH == 1 has 128 threads, which take both k2. Word k of chunk i
+// holds dims i + 32 k + 8 m (nibble m) of a pair's two tokens. Tokens at and behind
+// `valid` become zero (their P is zero and their bytes may be any bits).
+template <int FMT, int GROUP, int KH>
+__device__ __forceinline__ void sh_convert_v(const uint8_t* rb, uint8_t* sVt, int t, int valid) {
   constexpr int NG = HKV_D / GROUP;
-  const int o = t >> 3, i = t & 7;
+  const int i = t & 7, o0 = t >> 4, k2 = (t >> 3) & 1;
   const uint8_t* meta = rb + HKV_META_OFF;
 #pragma unroll
-  for (int hh = 0; hh < 2 / HALVES; ++hh) {
-    const int half = HALVES == 2 ? half0 : hh;
+  for (int rep = 0; rep < 2 / KH; ++rep) {
+    const int o = o0 + 8 * rep;
     uint2 cw[4];
 #pragma unroll
-    for (int pp = 0; pp < 4; ++pp) cw[pp] = *reinterpret_cast<const uint2*>(rb + HKV_V_CODES_OFF + v_chunk_off(4 * o + pp, i) + 8 * half);
+    for (int pp = 0; pp < 4; ++pp) cw[pp] = *reinterpret_cast<const uint2*>(rb + HKV_V_CODES_OFF + v_chunk_off(4 * o + pp, i) + 8 * k2);
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-      const int k = 2 * half + w, g = 32 * k / GROUP;
+      const int k = 2 * k2 + w, g = 32 * k / GROUP;
       uint32_t h[4][4];  // [pair][nibble m], then the values
 #pragma unroll
       for (int pp = 0; pp < 4; ++pp) {
@@ -314,8 +327,8 @@ __device__ __forceinline__ void sh_convert_v(const uint8_t* rb, uint8_t* sVt, in
         for (int m = 0; m < 4; ++m) h[pp][m] = h2u(__hfma2(u2h(h[pp][m]), s2, m2));
       }
 #pragma unroll
-      for (int m = 0; m < 4; ++m)  // dim i + 32 k + 8 m
-        *reinterpret_cast<uint4*>(sVt + pf_chunk(i + 32 * k + 8 * m, o)) = make_uint4(h[0][m], h[1][m], h[2][m], h[3][m]);
+      for (int m = 0; m < 4; ++m)  // dim i + 32 k + 8 m: its row is 0 mod 8 plus i
+        *reinterpret_cast<uint4*>(sVt + pf_chunk(i, o) + (32 * k + 8 * m) * 128) = make_uint4(h[0][m], h[1][m], h[2][m], h[3][m]);
     }
   }
 }
@@ -325,7 +338,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
   constexpr int SG = sh_softmax_groups(N);   // softmax groups of 128 threads
   constexpr int COLS = N / SG;               // columns of a softmax thread
   constexpr int SUB = 16;                    // taken at a time
-  constexpr int KH = sh_halves(N);           // K (and V) warps = 4 KH
+  constexpr int KH = sh_halves(N);           // sets of four K warps (a tile each in turn); V warps = 4 KH
   constexpr int R = sh_slots(N);
   constexpr int kThreads = sh_threads(N);
   constexpr uint32_t kBlock = block_bytes(FMT, GROUP);
@@ -347,10 +360,10 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
   if (t == 0) {
     for (int i = 0; i < R; ++i) {
       mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_free[i], 8 * KH);
+      mbar_init(&raw_free[i], 4 + 4 * KH);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&k_full[i], 4 * KH);
+      mbar_init(&k_full[i], 4);
       mbar_init(&v_full[i], 4 * KH);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4 * SG);
@@ -413,9 +426,16 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
       for (int i = 0; i < COLS; ++i) l[i] = 0.f;
       for (int j = 0; j < pc.n; ++j) {
         const int n = n0 + j, buf = n & 1;
-        bool bad = !mbar_wait(&s_full[buf], (n >> 1) & 1);
-        if (n >= 2) bad = !mbar_wait(&pv_done[buf], ((n >> 1) - 1) & 1) || bad;  // P[buf] is free
-        __syncwarp();
+        // One warp of a role polls the mbarriers and the others sleep at a named
+        // barrier: with every warp polling, two thirds of the instructions were polls.
+        bool good = true;
+        if ((warp & 3) == 0) {
+          good = sh_wait(&s_full[buf], (n >> 1) & 1);
+          if (n >= 2) good = sh_wait(&pv_done[buf], ((n >> 1) - 1) & 1) && good;  // P[buf] is free
+          __syncwarp();
+        }
+        ok = bar_and(1 + sg, 128, good);
+        if (!ok) break;
         tc_fence_after();
         const bool see = tok < s_valid[n & 15];
 #pragma unroll
@@ -437,12 +457,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
           float mx = fmaxf(x[0], x[SUB - 1]);
 #pragma unroll
           for (int i = 1; i + 1 < SUB; i += 2) mx = fmax3(mx, x[i], x[i + 1]);
-          if (bar_or(1 + sg, 128, (see && mx > kPfLazy) || bad)) {
-            // a column's max moves, or a wait ran out somewhere
-            if (bar_or(1 + sg, 128, bad)) {
-              ok = false;
-              break;
-            }
+          if (bar_or(1 + sg, 128, see && mx > kPfLazy)) {  // a column's max moves
             sh_ld<SUB>(ts, x);
             float mine = -INFINITY;  // the warp's max of column c0 + lane
 #pragma unroll
@@ -461,12 +476,10 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
               s_f[c] = fast_exp2(old - m);
             }
             // O(n - 1) has to be there before it is rescaled
-            bad = j > 0 && !mbar_wait(&pv_done[buf ^ 1], ((n - 1) >> 1) & 1);
+            good = (warp & 3) != 0 || j == 0 || sh_wait(&pv_done[buf ^ 1], ((n - 1) >> 1) & 1);
             __syncwarp();
-            if (bar_or(1 + sg, 128, bad)) {
-              ok = false;
-              break;
-            }
+            ok = bar_and(1 + sg, 128, good);
+            if (!ok) break;
             if (j > 0) {
               tc_fence_after();
               sh_ld<SUB>(tO + c0 + lanes, x);
@@ -507,10 +520,10 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
         // the piece's partial: O^T from TMEM (lane = dim), m and l per column
         const int last = n0 + pc.n - 1;
         const int64_t id = (int64_t)(blockIdx.x + pc.unit) * N;
-        const bool bad = !mbar_wait(&pv_done[last & 1], (last >> 1) & 1);
+        const bool good = (warp & 3) != 0 || sh_wait(&pv_done[last & 1], (last >> 1) & 1);
         __syncwarp();
+        ok = bar_and(1 + sg, 128, good);
         tc_fence_after();
-        ok = !bar_or(1 + sg, 128, bad);
         if (ok) {
 #pragma unroll
           for (int s0 = 0; s0 < COLS; s0 += SUB) {
@@ -542,17 +555,19 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
     } else if (warp < 4 * SG + 4 * KH) {
       // ---------------- K: thread = token = TMEM lane ----------------
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-      const int half = (warp - 4 * SG) >> 2;
-      for (int j = 0; j < pc.n; ++j) {
+      const int set = (warp - 4 * SG) >> 2;  // takes the tiles of its parity (KH == 2)
+      for (int j = KH == 2 ? (n0 ^ set) & 1 : 0; j < pc.n; j += KH) {
         const int n = n0 + j, buf = n & 1, slot = n % R;
-        bool good = mbar_wait(&raw_full[slot], (n / R) & 1);
-        if (n >= 2) good = mbar_wait(&s_full[buf], ((n >> 1) - 1) & 1) && good;  // S(n - 2) has read K[buf]
-        if (!__all_sync(0xffffffffu, good)) {
-          ok = false;
-          break;
+        bool good = true;
+        if ((warp & 3) == 0) {
+          good = sh_wait(&raw_full[slot], (n / R) & 1);
+          if (n >= 2) good = sh_wait(&s_full[buf], ((n >> 1) - 1) & 1) && good;  // S(n - 2) has read K[buf]
+          __syncwarp();
         }
+        ok = bar_and(5 + set, 128, good);
+        if (!ok) break;
         tc_fence_after();
-        sh_convert_k<FMT, GROUP, KH>(raw + slot * kShRawBytes, tmem + 64 * buf + lanes, t & 127, half, (t & 127) < s_valid[n & 15]);
+        sh_convert_k<FMT, GROUP>(raw + slot * kShRawBytes, tmem + 64 * buf + lanes, t & 127, (t & 127) < s_valid[n & 15]);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
@@ -562,16 +577,18 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
       }
     } else if (warp < 4 * SG + 8 * KH) {
       // ---------------- V ----------------
-      const int half = (warp - 4 * SG - 4 * KH) >> 2;
+      const int vt = t - 128 * (SG + KH);
       for (int j = 0; j < pc.n; ++j) {
         const int n = n0 + j, buf = n & 1, slot = n % R;
-        bool good = mbar_wait(&raw_full[slot], (n / R) & 1);
-        if (n >= 2) good = mbar_wait(&pv_done[buf], ((n >> 1) - 1) & 1) && good;  // O(n - 2) has read Vt[buf]
-        if (!__all_sync(0xffffffffu, good)) {
-          ok = false;
-          break;
+        bool good = true;
+        if (vt < 32) {
+          good = sh_wait(&raw_full[slot], (n / R) & 1);
+          if (n >= 2) good = sh_wait(&pv_done[buf], ((n >> 1) - 1) & 1) && good;  // O(n - 2) has read Vt[buf]
+          __syncwarp();
         }
-        sh_convert_v<FMT, GROUP, KH>(raw + slot * kShRawBytes, sV + buf * kPfTileBytes, t & 127, half, s_valid[n & 15]);
+        ok = bar_and(7, 128 * KH, good);
+        if (!ok) break;
+        sh_convert_v<FMT, GROUP, KH>(raw + slot * kShRawBytes, sV + buf * kPfTileBytes, vt, s_valid[n & 15]);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) {
@@ -588,7 +605,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
         const int n = n0 + j, slot = n % R, tok = (pc.t0 + j) * HKV_BLOCK_TOKENS;
         if ((j & 31) == 0) ids = j + lane < pc.n ? store_page(p.prefix, u, tok + lane * HKV_BLOCK_TOKENS) : -1;
         const int64_t page = __shfl_sync(0xffffffffu, ids, j & 31);
-        if (n >= R && !__all_sync(0xffffffffu, mbar_wait(&raw_free[slot], (n / R - 1) & 1, 1000))) {
+        if (n >= R && !__all_sync(0xffffffffu, sh_wait(&raw_free[slot], (n / R - 1) & 1))) {
           ok = false;
           break;
         }
@@ -608,13 +625,13 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
         issued = n + 1;
       }
       if (!ok)  // copies in flight land before the CTA ends
-        for (int n = max(0, issued - R); n < issued; ++n) mbar_wait(&raw_full[n % R], (n / R) & 1);
+        for (int n = max(0, issued - R); n < issued; ++n) sh_wait(&raw_full[n % R], (n / R) & 1);
     } else if (elect_one()) {
       // ---------------- MMA ----------------
       const uint32_t q0 = smem_u32(sQ), v0 = smem_u32(sV), p0 = smem_u32(sP);
       auto scores = [&](int n) {  // S^T(n) = K(n) Q^T; its buffer was read before P(n - 2) was announced
         const int buf = n & 1;
-        if (!mbar_wait(&k_full[buf], (n >> 1) & 1)) return false;
+        if (!sh_wait(&k_full[buf], (n >> 1) & 1)) return false;
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
@@ -624,11 +641,11 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
         issued = 1;
         return true;
       };
-      ok = mbar_wait(&q_full, pieces & 1) && scores(n0);
+      ok = sh_wait(&q_full, pieces & 1) && scores(n0);
       for (int j = 0; ok && j < pc.n; ++j) {
         const int n = n0 + j, buf = n & 1;
         if (j + 1 < pc.n) ok = scores(n + 1);
-        ok = ok && mbar_wait(&v_full[buf], (n >> 1) & 1) && mbar_wait(&p_full[buf], (n >> 1) & 1);
+        ok = ok && sh_wait(&v_full[buf], (n >> 1) & 1) && sh_wait(&p_full[buf], (n >> 1) & 1);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
@@ -639,7 +656,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
       }
       if (!ok && issued) {  // products in flight end before TMEM is freed
         pf_commit(&drain);
-        mbar_wait(&drain, 0);
+        sh_wait(&drain, 0);
       }
     }
     __syncwarp();
