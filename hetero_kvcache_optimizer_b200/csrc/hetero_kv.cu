@@ -567,7 +567,7 @@ hkv_status launch_shared_t(const hkv::SharedParams& p, cudaStream_t st) {
                                     hkv::sh_smem(N));
   });
   if (attr_err != cudaSuccess) return cuda_fail(attr_err);
-  const cudaError_t e = launch_pdl(8, hkv::shared_prefix_kernel<FMT, GROUP, N>, dim3(p.C), dim3(hkv::sh_threads(N)),
+  const cudaError_t e = launch_pdl(16, hkv::shared_prefix_kernel<FMT, GROUP, N>, dim3(p.C), dim3(hkv::sh_threads(N)),
                                    hkv::sh_smem(N), st, p);
   return e == cudaSuccess ? launch_status() : cuda_fail(e);
 }
@@ -618,7 +618,7 @@ hkv_status shared_plan(const hkv_int4_store* prefix, const int32_t* start, int P
     units += u;
     steps += u * (cap + hkv::kShCharge);
   }
-  if (steps >= (int64_t(1) << 31) || (units + pl.C) * pl.N >= (int64_t(1) << 31) || (int64_t)B * Hq >= (int64_t(1) << 28) ||
+  if (steps >= (int64_t(1) << 31) || (units + pl.C) * pl.N >= (int64_t(1) << 30) || (int64_t)B * Hq >= (int64_t(1) << 28) ||
       (int64_t)prefix->max_pages * prefix->page_tokens >= (int64_t(1) << 31))
     return HKV_ERR_UNSUPPORTED;
   size_t at = 0;
@@ -635,8 +635,9 @@ hkv_status shared_plan(const hkv_int4_store* prefix, const int32_t* start, int P
   pl.own_o = at;
   pl.own_ml = pl.own_o + (own ? (size_t)B * Hq * HKV_D * 4 : 0);
   pl.part_o = (pl.own_ml + (own ? (size_t)B * Hq * 8 : 0) + 255) & ~(size_t)255;
-  pl.part_ml = pl.part_o + (size_t)(units + pl.C) * pl.N * HKV_D * 4;
-  pl.bytes = pl.part_ml + (size_t)(units + pl.C) * pl.N * 8;
+  const size_t parts = (size_t)(units + pl.C) * hkv::sh_streams(pl.N) * pl.N;
+  pl.part_ml = pl.part_o + parts * HKV_D * 4;
+  pl.bytes = pl.part_ml + parts * 8;
   *out = pl;
   return HKV_OK;
 }
@@ -1583,7 +1584,7 @@ hkv_status hkv_decode_shared(const void* q, int32_t q_dtype, int64_t q_stride_b,
                     HKV_DT_F32, 0, 0, const_cast<float*>(p.own_o), const_cast<float*>(p.own_ml), S(stream));
     if (rc != HKV_OK) return rc;
   }
-  const cudaError_t e = launch_pdl(8, hkv::shared_merge_kernel, dim3(B * Hq), dim3(128), 0, S(stream), p);
+  const cudaError_t e = launch_pdl(32, hkv::shared_merge_kernel, dim3(B * Hq), dim3(128), 0, S(stream), p);
   return e == cudaSuccess ? launch_status() : cuda_fail(e);
 }
 

@@ -37,16 +37,20 @@ constexpr int kShMaxGroups = 512;
 constexpr int kShCharge = 6;
 constexpr int kShRawBytes = 24 * 1024;
 
-// Warps: groups of four softmax warps (kShCols rows each) | K | V | producer, MMA.
-constexpr int sh_softmax_groups(int n) { return n <= 16 ? 1 : n <= 64 ? 2 : 4; }
-constexpr int sh_halves(int n) { return n <= 64 ? 2 : 1; }  // sets of four K and of four V warps
+// Up to 64 rows, even and odd tiles of a CTA are two streams, each with its own
+// softmax warps, running max, O and partial: two tiles' softmax are in flight at a
+// time, neither waiting for the other's rescale. At 128 rows TMEM has room for one.
+constexpr int sh_streams(int n) { return n <= 64 ? 2 : 1; }
+constexpr int sh_col_groups(int n) { return n <= 32 ? 1 : n <= 64 ? 2 : 4; }  // softmax groups that share a tile's rows
+constexpr int sh_softmax_groups(int n) { return sh_streams(n) * sh_col_groups(n); }
+constexpr int sh_halves(int n) { return n <= 32 ? 2 : 1; }  // sets of four K and of four V warps
 constexpr int sh_threads(int n) { return 32 * (4 * sh_softmax_groups(n) + 8 * sh_halves(n) + 2); }
 constexpr int sh_slots(int n) { return n <= 64 ? 4 : 2; }
 constexpr int sh_p_bytes(int n) { return 128 * 128 * (n <= 64 ? 1 : 2); }  // [token][64 rows] f16 blocks
 constexpr int sh_smem(int n) {  // Q | Vt[2] | P[2] | raw slots | alignment
   return n * 256 + 2 * kPfTileBytes + 2 * sh_p_bytes(n) + sh_slots(n) * kShRawBytes + 1024;
 }
-constexpr int sh_tmem_cols(int n) { return 128 + 3 * n <= 256 ? 256 : 512; }  // K[2] | S[2] | O
+constexpr int sh_tmem_cols(int n) { return 128 + (2 + sh_streams(n)) * n <= 256 ? 256 : 512; }  // K[2] | S[2] | O[streams]
 
 struct SharedParams {
   const void* q;
@@ -57,8 +61,8 @@ struct SharedParams {
   float qscale;             // sm_scale * log2(e)
   int* counters;            // own part's merge counters, zeroed here
   int n_counters;
-  float* part_o;            // [C + units][N][128]
-  float* part_ml;           // [C + units][N][2]
+  float* part_o;            // [C + units][streams][N][128]
+  float* part_ml;           // [C + units][streams][N][2]
   // merge
   const float* own_o;       // [B][Hq][128], or NULL
   const float* own_ml;      // [B][Hq][2]
@@ -210,9 +214,9 @@ __device__ __forceinline__ bool elect_one() {
   return e != 0;
 }
 
-// The kernel's bounded wait: a pending warp sleeps (woken by the phase) instead of
-// polling, since 26 warps that poll take issue slots from those that work.
-__device__ __forceinline__ bool sh_wait(uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, 2000); }
+// Bounded wait for the phase that tile n's use of a buffer completes (the buffers
+// of `ring` tiles are used in turn; n counts the CTA's tiles).
+__device__ __forceinline__ bool sh_wait(uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity & 1u); }
 
 // Dims of 16-byte chunk kc (8 values) of Q's and K's common order: value 2 c + e
 // is dim 32 (kc / 4) + 8 c + 2 (kc % 4) + e, the order in which nib8_to_h2 yields
@@ -278,22 +282,34 @@ __device__ __forceinline__ void sh_convert_k(const uint8_t* rb, uint32_t tmem, i
 }
 
 // V of the raw block into sVt ([dim][token], 128-byte swizzle): thread (o, k2, i) has
-// tokens 8 o .. 8 o + 7 and words 2 k2, 2 k2 + 1 of chunk i of their four pairs, so the
-// 16 threads of a load phase read a pair's 128 bytes and the 8 of a store phase hit
-// 8 chunks apart; KH == 1 has 128 threads, which take both k2. Word k of chunk i
-// holds dims i + 32 k + 8 m (nibble m) of a pair's two tokens. Tokens at and behind
+// tokens 8 o .. 8 o + 7 (and 64 on) and words 2 k2, 2 k2 + 1 of chunk i of their four
+// pairs, so the 16 threads of a load phase read a pair's 128 bytes and the 8 of a
+// store phase hit 8 chunks apart. Word k of chunk i holds dims i + 32 k + 8 m (nibble m) of a pair's two tokens. Tokens at and behind
 // `valid` become zero (their P is zero and their bytes may be any bits).
-template <int FMT, int GROUP, int KH>
+template <int FMT, int GROUP>
 __device__ __forceinline__ void sh_convert_v(const uint8_t* rb, uint8_t* sVt, int t, int valid) {
   constexpr int NG = HKV_D / GROUP;
   const int i = t & 7, o0 = t >> 4, k2 = (t >> 3) & 1;
   const uint8_t* meta = rb + HKV_META_OFF;
 #pragma unroll
-  for (int rep = 0; rep < 2 / KH; ++rep) {
+  for (int rep = 0; rep < 2; ++rep) {
     const int o = o0 + 8 * rep;
     uint2 cw[4];
+    __half2 vs2[4][2], vm2[4][2];  // fp16min: scales and mins of the pairs in the groups of words 2 k2, 2 k2 + 1
 #pragma unroll
-    for (int pp = 0; pp < 4; ++pp) cw[pp] = *reinterpret_cast<const uint2*>(rb + HKV_V_CODES_OFF + v_chunk_off(4 * o + pp, i) + 8 * k2);
+    for (int pp = 0; pp < 4; ++pp) {
+      cw[pp] = *reinterpret_cast<const uint2*>(rb + HKV_V_CODES_OFF + v_chunk_off(4 * o + pp, i) + 8 * k2);
+      if constexpr (FMT == HKV_FMT_FP16MIN) {
+        const uint8_t* mp = meta + 512 * NG + 4 * ((4 * o + pp) * NG + 64 * k2 / GROUP);
+        if constexpr (NG == 4) {
+          vload_h2<2>(mp, vs2[pp]);
+          vload_h2<2>(mp + 256 * NG, vm2[pp]);
+        } else {
+          vs2[pp][0] = vs2[pp][1] = *reinterpret_cast<const __half2*>(mp);
+          vm2[pp][0] = vm2[pp][1] = *reinterpret_cast<const __half2*>(mp + 256 * NG);
+        }
+      }
+    }
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       const int k = 2 * k2 + w, g = 32 * k / GROUP;
@@ -304,8 +320,8 @@ __device__ __forceinline__ void sh_convert_v(const uint8_t* rb, uint8_t* sVt, in
         __half2 s2, m2;
         const uint32_t wd = w ? cw[pp].y : cw[pp].x;
         if constexpr (FMT == HKV_FMT_FP16MIN) {
-          s2 = reinterpret_cast<const __half2*>(meta + 512 * NG)[q * NG + g];
-          m2 = reinterpret_cast<const __half2*>(meta + 768 * NG)[q * NG + g];
+          s2 = vs2[pp][w];
+          m2 = vm2[pp][w];
         } else {
           const float* vs = reinterpret_cast<const float*>(meta + 512 * NG);
           s2 = __floats2half2_rn(vs[2 * q * NG + g], vs[(2 * q + 1) * NG + g]);
@@ -335,10 +351,11 @@ __device__ __forceinline__ void sh_convert_v(const uint8_t* rb, uint8_t* sVt, in
 
 template <int FMT, int GROUP, int N>
 __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const __grid_constant__ SharedParams p) {
-  constexpr int SG = sh_softmax_groups(N);   // softmax groups of 128 threads
-  constexpr int COLS = N / SG;               // columns of a softmax thread
+  constexpr int NS = sh_streams(N), CG = sh_col_groups(N);
+  constexpr int SG = NS * CG;                // softmax groups of 128 threads
+  constexpr int COLS = N / CG;               // columns of a softmax thread
   constexpr int SUB = 16;                    // taken at a time
-  constexpr int KH = sh_halves(N);           // sets of four K warps (a tile each in turn); V warps = 4 KH
+  constexpr int KH = sh_halves(N);           // sets of four K and of four V warps (a tile each in turn)
   constexpr int R = sh_slots(N);
   constexpr int kThreads = sh_threads(N);
   constexpr uint32_t kBlock = block_bytes(FMT, GROUP);
@@ -348,8 +365,8 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
   __shared__ uint32_t s_tmem;
   __shared__ ShGroup s_g[kShMaxGroups + 1];
   __shared__ int s_valid[16];        // tokens in use of tile n & 15
-  __shared__ __align__(16) float s_m[N], s_f[N];  // column's running max; its last rescale
-  __shared__ float s_cm[4][N];       // per-warp column maxima, then sums
+  __shared__ __align__(16) float s_ms[NS][N], s_fs[NS][N];  // column's running max; its last rescale
+  __shared__ float s_cms[NS][4][N];  // per-warp column maxima, then sums
   uint8_t* sm = sh_raw + ((1024u - (smem_u32(sh_raw) & 1023u)) & 1023u);
   uint8_t* sQ = sm;
   uint8_t* sV = sQ + N * 256;
@@ -360,13 +377,13 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
   if (t == 0) {
     for (int i = 0; i < R; ++i) {
       mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_free[i], 4 + 4 * KH);
+      mbar_init(&raw_free[i], 8);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 4);
-      mbar_init(&v_full[i], 4 * KH);
+      mbar_init(&v_full[i], 4);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4 * SG);
+      mbar_init(&p_full[i], 4 * CG);
       mbar_init(&pv_done[i], 1);
     }
     mbar_init(&q_full, 4 * SG);
@@ -388,8 +405,8 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
   const int total = s_g[p.P].step;
   int at = sh_cut(total, p.C, blockIdx.x);
   const int end = sh_cut(total, p.C, blockIdx.x + 1);
-  int n0 = 0, pieces = 0;  // tiles and pieces of the CTA before this one
-  int issued = 0;   // producer: copies; MMA warp: whether there are products
+  uint32_t n0 = 0, pieces = 0;  // tiles and pieces of the CTA before this one
+  uint32_t issued = 0;   // producer: copies; MMA warp: whether there are products
   bool ok = true;
 
   while (true) {
@@ -397,11 +414,17 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
     if (pc.n == 0) break;
     const int rows = (p.start[pc.g + 1] - p.start[pc.g]) * p.G - pc.rt * N;
     if (warp < 4 * SG) {
-      // ---------------- softmax: thread = token, columns [col0, col0 + COLS) ----------------
-      const int sg = warp >> 2, tok = t & 127, col0 = sg * COLS;
+      // ---------------- softmax: thread = token, columns [col0, col0 + COLS) of the stream's tiles ----------------
+      const int sg = warp >> 2, tok = t & 127, col0 = sg % CG * COLS, stream = sg / CG;
+      float *s_m = s_ms[stream], *s_f = s_fs[stream];
+      auto s_cm = s_cms[stream];
+      const uint32_t tOs = tO + stream * N;
+      const int j0 = NS == 2 ? (n0 ^ stream) & 1 : 0;  // the stream's first tile
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const float2 qs2 = make_float2(p.qscale, p.qscale);
-      // the piece's query rows, in K's dim order
+      // every group is through with the last piece's scores: its query rows make room
+      // for this one's, in K's dim order (a group that gave up says so here)
+      if (!bar_and(9, 128 * SG, ok)) break;
       for (int c = t; c < N * 16; c += 128 * SG) {
         const int n = c >> 4, kc = c & 15;
         uint32_t o[4] = {0u, 0u, 0u, 0u};
@@ -424,14 +447,14 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
       float l[COLS];
 #pragma unroll
       for (int i = 0; i < COLS; ++i) l[i] = 0.f;
-      for (int j = 0; j < pc.n; ++j) {
-        const int n = n0 + j, buf = n & 1;
+      for (int j = j0; j < pc.n; j += NS) {
+        const uint32_t n = n0 + j, buf = n & 1;
         // One warp of a role polls the mbarriers and the others sleep at a named
         // barrier: with every warp polling, two thirds of the instructions were polls.
         bool good = true;
         if ((warp & 3) == 0) {
-          good = sh_wait(&s_full[buf], (n >> 1) & 1);
-          if (n >= 2) good = sh_wait(&pv_done[buf], ((n >> 1) - 1) & 1) && good;  // P[buf] is free
+          good = sh_wait(&s_full[buf], n >> 1);
+          if (n >= 2) good = sh_wait(&pv_done[buf], (n >> 1) - 1) && good;  // P[buf] is free
           __syncwarp();
         }
         ok = bar_and(1 + sg, 128, good);
@@ -475,17 +498,18 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
               s_m[c] = m;
               s_f[c] = fast_exp2(old - m);
             }
-            // O(n - 1) has to be there before it is rescaled
-            good = (warp & 3) != 0 || j == 0 || sh_wait(&pv_done[buf ^ 1], ((n - 1) >> 1) & 1);
+            // the stream's last O has to be there before it is rescaled (with two streams
+            // that is O(n - 2), waited for above)
+            good = NS == 2 || (warp & 3) != 0 || j == 0 || sh_wait(&pv_done[buf ^ 1], (n - 1) >> 1);
             __syncwarp();
             ok = bar_and(1 + sg, 128, good);
             if (!ok) break;
-            if (j > 0) {
+            if (j > j0) {
               tc_fence_after();
-              sh_ld<SUB>(tO + c0 + lanes, x);
+              sh_ld<SUB>(tOs + c0 + lanes, x);
 #pragma unroll
               for (int i = 0; i < SUB; ++i) x[i] *= s_f[c0 + i];
-              sh_st<SUB>(tO + c0 + lanes, x);
+              sh_st<SUB>(tOs + c0 + lanes, x);
               tm_wait_st();
             }
 #pragma unroll
@@ -518,9 +542,9 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
       }
       if (ok) {
         // the piece's partial: O^T from TMEM (lane = dim), m and l per column
-        const int last = n0 + pc.n - 1;
-        const int64_t id = (int64_t)(blockIdx.x + pc.unit) * N;
-        const bool good = (warp & 3) != 0 || sh_wait(&pv_done[last & 1], (last >> 1) & 1);
+        const int last = (int)(n0 + pc.n - 1) - (NS == 2 ? (int)((n0 + pc.n - 1) ^ stream) & 1 : 0);  // the stream's last tile
+        const int64_t id = ((int64_t)(blockIdx.x + pc.unit) * NS + stream) * N;
+        const bool any = last >= (int)n0, good = (warp & 3) != 0 || !any || sh_wait(&pv_done[last & 1], last >> 1);
         __syncwarp();
         ok = bar_and(1 + sg, 128, good);
         tc_fence_after();
@@ -528,10 +552,10 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
 #pragma unroll
           for (int s0 = 0; s0 < COLS; s0 += SUB) {
             float o[SUB];
-            sh_ld<SUB>(tO + col0 + s0 + lanes, o);
+            sh_ld<SUB>(tOs + col0 + s0 + lanes, o);
 #pragma unroll
             for (int i = 0; i < SUB; ++i)
-              if (col0 + s0 + i < rows) p.part_o[(id + col0 + s0 + i) * HKV_D + tok] = o[i];
+              if (any && col0 + s0 + i < rows) p.part_o[(id + col0 + s0 + i) * HKV_D + tok] = o[i];
             // sums over the warp's tokens: lane ends with column lane % SUB
 #pragma unroll
             for (int i = 0; i < SUB; ++i) o[i] = l[s0 + i] + (SUB == 16 ? __shfl_xor_sync(0xffffffffu, l[s0 + i], 16) : 0.f);
@@ -557,11 +581,11 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const int set = (warp - 4 * SG) >> 2;  // takes the tiles of its parity (KH == 2)
       for (int j = KH == 2 ? (n0 ^ set) & 1 : 0; j < pc.n; j += KH) {
-        const int n = n0 + j, buf = n & 1, slot = n % R;
+        const uint32_t n = n0 + j, buf = n & 1, slot = n % R;
         bool good = true;
         if ((warp & 3) == 0) {
-          good = sh_wait(&raw_full[slot], (n / R) & 1);
-          if (n >= 2) good = sh_wait(&s_full[buf], ((n >> 1) - 1) & 1) && good;  // S(n - 2) has read K[buf]
+          good = sh_wait(&raw_full[slot], n / R);
+          if (n >= 2) good = sh_wait(&s_full[buf], (n >> 1) - 1) && good;  // S(n - 2) has read K[buf]
           __syncwarp();
         }
         ok = bar_and(5 + set, 128, good);
@@ -577,18 +601,18 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
       }
     } else if (warp < 4 * SG + 8 * KH) {
       // ---------------- V ----------------
-      const int vt = t - 128 * (SG + KH);
-      for (int j = 0; j < pc.n; ++j) {
-        const int n = n0 + j, buf = n & 1, slot = n % R;
+      const int set = (warp - 4 * SG - 4 * KH) >> 2, vt = t & 127;
+      for (int j = KH == 2 ? (n0 ^ set) & 1 : 0; j < pc.n; j += KH) {
+        const uint32_t n = n0 + j, buf = n & 1, slot = n % R;
         bool good = true;
-        if (vt < 32) {
-          good = sh_wait(&raw_full[slot], (n / R) & 1);
-          if (n >= 2) good = sh_wait(&pv_done[buf], ((n >> 1) - 1) & 1) && good;  // O(n - 2) has read Vt[buf]
+        if ((warp & 3) == 0) {
+          good = sh_wait(&raw_full[slot], n / R);
+          if (n >= 2) good = sh_wait(&pv_done[buf], (n >> 1) - 1) && good;  // O(n - 2) has read Vt[buf]
           __syncwarp();
         }
-        ok = bar_and(7, 128 * KH, good);
+        ok = bar_and(7 + set, 128, good);
         if (!ok) break;
-        sh_convert_v<FMT, GROUP, KH>(raw + slot * kShRawBytes, sV + buf * kPfTileBytes, vt, s_valid[n & 15]);
+        sh_convert_v<FMT, GROUP>(raw + slot * kShRawBytes, sV + buf * kPfTileBytes, vt, s_valid[n & 15]);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) {
@@ -602,10 +626,11 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
       const int len = max(0, p.prefix.lengths ? p.prefix.lengths[pc.g] : p.prefix.len);
       int64_t ids = -1;
       for (int j = 0; j < pc.n; ++j) {
-        const int n = n0 + j, slot = n % R, tok = (pc.t0 + j) * HKV_BLOCK_TOKENS;
+        const uint32_t n = n0 + j, slot = n % R;
+        const int tok = (pc.t0 + j) * HKV_BLOCK_TOKENS;
         if ((j & 31) == 0) ids = j + lane < pc.n ? store_page(p.prefix, u, tok + lane * HKV_BLOCK_TOKENS) : -1;
         const int64_t page = __shfl_sync(0xffffffffu, ids, j & 31);
-        if (n >= R && !__all_sync(0xffffffffu, sh_wait(&raw_free[slot], (n / R - 1) & 1))) {
+        if (n >= R && !__all_sync(0xffffffffu, sh_wait(&raw_free[slot], n / R - 1))) {
           ok = false;
           break;
         }
@@ -625,13 +650,14 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
         issued = n + 1;
       }
       if (!ok)  // copies in flight land before the CTA ends
-        for (int n = max(0, issued - R); n < issued; ++n) sh_wait(&raw_full[n % R], (n / R) & 1);
+        for (uint32_t n = issued > R ? issued - R : 0; n < issued; ++n) sh_wait(&raw_full[n % R], n / R);
     } else if (elect_one()) {
-      // ---------------- MMA ----------------
+      // ---------------- MMA: O of a stream is overwritten once P of its first tile says
+      // that its groups have read the last piece's ----------------
       const uint32_t q0 = smem_u32(sQ), v0 = smem_u32(sV), p0 = smem_u32(sP);
-      auto scores = [&](int n) {  // S^T(n) = K(n) Q^T; its buffer was read before P(n - 2) was announced
-        const int buf = n & 1;
-        if (!sh_wait(&k_full[buf], (n >> 1) & 1)) return false;
+      auto scores = [&](uint32_t n) {  // S^T(n) = K(n) Q^T; its buffer was read before P(n - 2) was announced
+        const uint32_t buf = n & 1;
+        if (!sh_wait(&k_full[buf], n >> 1)) return false;
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
@@ -641,17 +667,17 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
         issued = 1;
         return true;
       };
-      ok = sh_wait(&q_full, pieces & 1) && scores(n0);
+      ok = sh_wait(&q_full, pieces) && scores(n0);
       for (int j = 0; ok && j < pc.n; ++j) {
-        const int n = n0 + j, buf = n & 1;
+        const uint32_t n = n0 + j, buf = n & 1;
         if (j + 1 < pc.n) ok = scores(n + 1);
-        ok = ok && sh_wait(&v_full[buf], (n >> 1) & 1) && sh_wait(&p_full[buf], (n >> 1) & 1);
+        ok = ok && sh_wait(&v_full[buf], n >> 1) && sh_wait(&p_full[buf], n >> 1);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
-          sh_mma_ss(tO, pf_desc(v0 + buf * kPfTileBytes + (kk >> 2) * 16384 + (kk & 3) * 32),
-                    sh_desc_n(p0 + buf * sh_p_bytes(N) + kk * 2048), sh_idesc(N, true), j > 0 || kk > 0);
+          sh_mma_ss(tO + (NS == 2 ? buf * N : 0), pf_desc(v0 + buf * kPfTileBytes + (kk >> 2) * 16384 + (kk & 3) * 32),
+                    sh_desc_n(p0 + buf * sh_p_bytes(N) + kk * 2048), sh_idesc(N, true), j >= NS || kk > 0);
         pf_commit(&pv_done[buf]);
       }
       if (!ok && issued) {  // products in flight end before TMEM is freed
@@ -660,10 +686,10 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
       }
     }
     __syncwarp();
-    ok = __syncthreads_and(ok);
     n0 += pc.n;
     ++pieces;
-    if (!ok) break;
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok && warp >= 4 * SG) break;
   }
   tc_fence_before();
   __syncthreads();
@@ -710,19 +736,19 @@ __global__ void __launch_bounds__(128) shared_merge_kernel(const __grid_constant
     c0 = cta(first);
     c1 = cta(last);
   }
-  // partial k: the own part (k = 0, when there is one), then the CTAs c0 .. c1
-  const int own = p.own_o ? 1 : 0, parts = own + c1 - c0 + 1;
+  // partial k: the own part (k = 0, when there is one), then the streams of the CTAs c0 .. c1
+  const int own = p.own_o ? 1 : 0, ns = sh_streams(p.N), parts = own + (c1 - c0 + 1) * ns;
   float M = -1.0e30f, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int k0 = w; k0 < parts; k0 += 128) {  // up to 32 partials of this warp: k0, k0 + 4, ...
-    const int k = k0 + 4 * lane, c = c0 + k - own;
+    const int k = k0 + 4 * lane, c = c0 + (k - own) / ns;
     float2 ml = make_float2(-1.0e30f, 0.f);
     const float* src = nullptr;
     if (k < own) {
       ml = *reinterpret_cast<const float2*>(p.own_ml + (int64_t)row * 2);
       src = p.own_o + (int64_t)row * HKV_D;
     } else if (k < parts && sh_cut(total, p.C, c) < sh_cut(total, p.C, c + 1)) {  // else: more CTAs than steps
-      const int64_t id = (int64_t)(c + unit) * p.N + n;
+      const int64_t id = ((int64_t)(c + unit) * ns + (k - own) % ns) * p.N + n;
       ml = *reinterpret_cast<const float2*>(p.part_ml + id * 2);
       src = p.part_o + id * HKV_D;
     }
