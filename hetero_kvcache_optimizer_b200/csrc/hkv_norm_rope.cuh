@@ -35,9 +35,12 @@ struct NormRopeParams {
   const float* table;      // [max_pos][rot]: cos | sin
   int64_t table_stride;    // elements
   int max_pos, rot;
+  int table_vec;           // table rows and their halves 16-byte aligned
   float eps;
   int B, T;
-  int chunks[2];           // warps' head chunks per token of q and of k
+  uint32_t items;          // warps' pieces of work
+  int per_warp;            // heads of one token a warp takes
+  int chunks[2];           // warps per token of q and of k
 };
 
 constexpr int kNrThreads = 256;
@@ -69,31 +72,62 @@ __device__ __forceinline__ uint4 nr_load(const T* p, bool vec) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// kHeads: heads of one token a warp takes (even).
-template <typename T, int MODE, int kHeads>
-__global__ void __launch_bounds__(kNrThreads) norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
-  const int lane = threadIdx.x & 31, l = lane & 15, hi = lane >> 4;
-  const int per = p.chunks[0] + p.chunks[1];
-  const int64_t item = (int64_t)blockIdx.x * (kNrThreads / 32) + (threadIdx.x >> 5);
-  griddep_wait();
-  griddep_launch_dependents();
-  if (item >= (int64_t)p.B * p.T * per) return;
-  const int64_t tok = item / per;
+__device__ __forceinline__ void nr_ld4(const float* p, float* v) {
+  const float4 x = __ldg(reinterpret_cast<const float4*>(p));
+  v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+}
+
+// The place of a warp's work: heads h0 .. h0 + kHeads - 1 of side 0 (q) or 1 (k) of a token.
+struct NrItem {
+  int side, h0, b, t;
+};
+template <int kHeads>
+__device__ __forceinline__ NrItem nr_item(const NormRopeParams& p, uint32_t item) {
+  const uint32_t per = p.chunks[0] + p.chunks[1], tok = item / per;
   const int c = (int)(item - tok * per);
-  const int b = (int)(tok / p.T), t = (int)(tok - (int64_t)b * p.T);
-  const int side = c >= p.chunks[0];
-  const int h0 = (side ? c - p.chunks[0] : c) * kHeads;
-  const int64_t pi = (int64_t)b * p.ps_b + (int64_t)t * p.ps_t;
-  const int64_t pos = !p.pos ? 0 : p.pos64 ? static_cast<const int64_t*>(p.pos)[pi] : (int64_t) static_cast<const int32_t*>(p.pos)[pi];
-  const T* x = static_cast<const T*>(p.x[side]) + b * p.xs[side][0] + t * p.xs[side][2] + 8 * l;
-  T* y = static_cast<T*>(p.y[side]) + b * p.ys[side][0] + t * p.ys[side][2] + 8 * l;
-  const bool vec = p.vec[side];
-  uint4 raw[kHeads / 2];
+  NrItem r;
+  r.side = c >= p.chunks[0];
+  r.h0 = (r.side ? c - p.chunks[0] : c) * kHeads;
+  r.b = (int)(tok / (uint32_t)p.T);
+  r.t = (int)(tok - (uint32_t)r.b * p.T);
+  return r;
+}
+// This lane's 16 bytes of every second head from h0 + (lane / 16), and the token's position.
+template <typename T, int kHeads>
+__device__ __forceinline__ int64_t nr_fetch(const NormRopeParams& p, const NrItem& m, int lane, uint4 (&raw)[kHeads / 2]) {
+  const int64_t* st = p.xs[m.side];
+  const T* x = static_cast<const T*>(p.x[m.side]) + m.b * st[0] + m.t * st[2] + 8 * (lane & 15);
 #pragma unroll
   for (int i = 0; i < kHeads / 2; ++i) {
-    const int h = h0 + 2 * i + hi;
-    raw[i] = h < p.H[side] ? nr_load(x + h * p.xs[side][1], vec) : make_uint4(0, 0, 0, 0);
+    const int h = m.h0 + 2 * i + (lane >> 4);
+    raw[i] = h < p.H[m.side] ? nr_load(x + h * st[1], p.vec[m.side]) : make_uint4(0, 0, 0, 0);
   }
+  if (!p.pos) return 0;
+  const int64_t pi = (int64_t)m.b * p.ps_b + (int64_t)m.t * p.ps_t;
+  return p.pos64 ? static_cast<const int64_t*>(p.pos)[pi] : (int64_t) static_cast<const int32_t*>(p.pos)[pi];
+}
+
+// One warp: heads h0 .. h1 - 1 of side SIDE (0 q, 1 k) of token (b, t): at most kHeads
+// of them, or with LOOP kHeads at a time, the next ones' loads out before these are
+// worked on. With
+// u = x w and rn the row's factor, out = rn (x (w c) + x' (w' s)), x' and w' the
+// pair's other half: the products with the weights are made once for all heads, and
+// x' is exchanged as it was loaded (16 bits), beside the sum of squares.
+template <typename T, int MODE, int kHeads, bool LOOP, int SIDE>
+__device__ __forceinline__ void nr_rows(const NormRopeParams& p, int b, int t, int h0, int h1, int lane) {
+  const int l = lane & 15, hi = lane >> 4;
+  const int64_t pi = (int64_t)b * p.ps_b + (int64_t)t * p.ps_t;
+  const int64_t pos = !p.pos ? 0 : p.pos64 ? static_cast<const int64_t*>(p.pos)[pi] : (int64_t) static_cast<const int32_t*>(p.pos)[pi];
+  const T* x = static_cast<const T*>(p.x[SIDE]) + b * p.xs[SIDE][0] + t * p.xs[SIDE][2] + (int64_t)(h0 + hi) * p.xs[SIDE][1] + 8 * l;
+  const int64_t xstep = 2 * p.xs[SIDE][1];
+  const bool vec = p.vec[SIDE];
+  uint4 raw[kHeads / 2], nraw[LOOP ? kHeads / 2 : 1];
+  const T* xn = x;
+  auto fetch = [&](int h, uint4* v) {
+#pragma unroll
+    for (int i = 0; i < kHeads / 2; ++i, xn += xstep) v[i] = h + 2 * i + hi < h1 ? nr_load(xn, vec) : make_uint4(0, 0, 0, 0);
+  };
+  fetch(h0, LOOP ? nraw : raw);
   if (pos < 0) return;  // a padding row: not written
   if (pos >= p.max_pos) {
     if (lane == 0) hkv_flag_error(HKV_DEVERR_BAD_POSITION);
@@ -101,87 +135,148 @@ __global__ void __launch_bounds__(kNrThreads) norm_rope_kernel(const __grid_cons
   }
   const int r = p.rot >> 1;
   const float* row = p.table + pos * p.table_stride;
-  float w[8], cs[8], sn[8];  // adjacent: cs/sn[0..3] serve the lane's four pairs
+  const void* wp = p.w[SIDE];
+  float w[8], cs[8], sn[8];  // adjacent: cs/sn[0 .. 3] serve the lane's four pairs
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = 1.f;
-  if (p.w[side]) {
-    if (p.w_dtype[side] == DT<T>::id && (reinterpret_cast<uintptr_t>(p.w[side]) & 15) == 0) {
-      nr_unpack<T>(__ldg(reinterpret_cast<const uint4*>(p.w[side]) + l), w);
+  for (int e = 0; e < 8; ++e) w[e] = cs[e] = 1.f, sn[e] = 0.f;
+  if (wp) {
+    if (p.w_dtype[SIDE] == DT<T>::id && (reinterpret_cast<uintptr_t>(wp) & 15) == 0) {
+      nr_unpack<T>(__ldg(reinterpret_cast<const uint4*>(wp) + l), w);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = load_any(p.w[side], p.w_dtype[side], 8 * l + e);
+      for (int e = 0; e < 8; ++e) w[e] = load_any(wp, p.w_dtype[SIDE], 8 * l + e);
     }
   }
+  const int k = r >> 3;  // kNrLane: lanes between the halves of a pair
+  const int from = (lane & 16) | (l < k ? l + k : l < 2 * k ? l - k : l);
+  const bool turned = MODE == kNrAdjacent ? 4 * l < r : 8 * l < 2 * r;  // some of the lane's values
   if constexpr (MODE == kNrAdjacent) {
+    if (p.table_vec) {  // r is a multiple of 4: the lane's four pairs turn together or not at all
+      if (turned) {
+        nr_ld4(row + 4 * l, cs);
+        nr_ld4(row + r + 4 * l, sn);
+      }
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = 4 * l + e;
-      cs[e] = i < r ? __ldg(row + i) : 1.f;
-      sn[e] = i < r ? __ldg(row + r + i) : 0.f;
+      for (int e = 0; e < 4; ++e)
+        if (4 * l + e < r) cs[e] = __ldg(row + 4 * l + e), sn[e] = __ldg(row + r + 4 * l + e);
+    }
+  } else if (MODE == kNrLane && p.table_vec) {  // r is a multiple of 8: a lane's values are in one half
+    if (turned) {
+      const float* c = row + (8 * l < r ? 8 * l : 8 * l - r);
+      nr_ld4(c, cs);
+      nr_ld4(c + 4, cs + 4);
+      nr_ld4(c + r, sn);
+      nr_ld4(c + r + 4, sn + 4);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sn[e] = 8 * l < r ? -sn[e] : sn[e];
     }
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int d = 8 * l + e, i = d < r ? d : d - r;
-      cs[e] = d < 2 * r ? __ldg(row + i) : 1.f;
-      sn[e] = d < r ? -__ldg(row + r + i) : d < 2 * r ? __ldg(row + r + i) : 0.f;
+      if (d < 2 * r) cs[e] = __ldg(row + i), sn[e] = d < r ? -__ldg(row + r + i) : __ldg(row + r + i);
     }
   }
+  // the weights into the rotation
+  if constexpr (MODE == kNrLane) {
 #pragma unroll
-  for (int i = 0; i < kHeads / 2; ++i) {
-    const int h = h0 + 2 * i + hi;
-    float v[8];
-    nr_unpack<T>(raw[i], v);
-    float rn = 1.f;
-    if (p.w[side]) {
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s = fmaf(v[e], v[e], s);
-#pragma unroll
-      for (int k = 1; k < 16; k <<= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
-      rn = rsqrtf(s * (1.f / HKV_D) + p.eps);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= rn * w[e];
+    for (int e = 0; e < 8; ++e) {
+      sn[e] *= __shfl_sync(0xffffffffu, w[e], from);
+      cs[e] *= w[e];
     }
-    float o[8];
-    if constexpr (MODE == kNrAdjacent) {
+  } else if constexpr (MODE == kNrAny) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool turned = 4 * l + e < r;  // the rest passes through, infinities included
-        o[2 * e] = turned ? v[2 * e] * cs[e] - v[2 * e + 1] * sn[e] : v[2 * e];
-        o[2 * e + 1] = turned ? v[2 * e + 1] * cs[e] + v[2 * e] * sn[e] : v[2 * e + 1];
+    for (int e = 0; e < 8; ++e) {
+      const int d = 8 * l + e;
+      if (wp && d < 2 * r) sn[e] *= load_any(wp, p.w_dtype[SIDE], d < r ? d + r : d - r);
+      cs[e] *= w[e];
+    }
+  }
+  T* yi = static_cast<T*>(p.y[SIDE]) + b * p.ys[SIDE][0] + t * p.ys[SIDE][2] + (int64_t)(h0 + hi) * p.ys[SIDE][1] + 8 * l;
+  const int64_t ystep = 2 * p.ys[SIDE][1];
+  const T* xi = x - 8 * l;
+#pragma unroll 1
+  for (int h = h0;; h += kHeads) {
+    if constexpr (LOOP) {
+#pragma unroll
+      for (int i = 0; i < kHeads / 2; ++i) raw[i] = nraw[i];
+      if (h + kHeads < h1) fetch(h + kHeads, nraw);
+    }
+#pragma unroll
+    for (int i = 0; i < kHeads / 2; ++i, yi += ystep, xi += xstep) {
+      const bool on = h + 2 * i + hi < h1;
+      float v[8], o[8];
+      nr_unpack<T>(raw[i], v);
+      float rn = 1.f;
+      if (wp) {
+        float2 s2 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) s2 = __ffma2_rn(make_float2(v[e], v[e + 1]), make_float2(v[e], v[e + 1]), s2);
+        float s = s2.x + s2.y;
+#pragma unroll
+        for (int q = 1; q < 16; q <<= 1) s += __shfl_xor_sync(0xffffffffu, s, q);
+        rn = rsqrtf(s * (1.f / HKV_D) + p.eps);
       }
-    } else if constexpr (MODE == kNrLane) {
-      const int k = r >> 3;  // lanes between the halves of a pair
-      const int from = l < k ? l + k : l < 2 * k ? l - k : l;
+      if constexpr (MODE == kNrAdjacent) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float other = __shfl_sync(0xffffffffu, v[e], (lane & 16) | from);
-        o[e] = l < 2 * k ? v[e] * cs[e] + other * sn[e] : v[e];
-      }
-    } else {
-      const T* xr = x - 8 * l + (int64_t)h * p.xs[side][1];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int d = 8 * l + e, q = d < r ? d + r : d < 2 * r ? d - r : d;
-        float other = 0.f;
-        if (h < p.H[side] && d < 2 * r) {
-          other = to_f32(xr[q]);
-          if (p.w[side]) other *= rn * load_any(p.w[side], p.w_dtype[side], q);
+        for (int e = 0; e < 4; ++e) {
+          const float a = v[2 * e] * w[2 * e], c = v[2 * e + 1] * w[2 * e + 1];
+          const bool on_pair = 4 * l + e < r;  // the rest passes through, infinities included
+          o[2 * e] = on_pair ? a * cs[e] - c * sn[e] : a;
+          o[2 * e + 1] = on_pair ? c * cs[e] + a * sn[e] : c;
         }
-        o[e] = d < 2 * r ? v[e] * cs[e] + other * sn[e] : v[e];
-      }
-      __syncwarp();  // in place: the row's values are all read before the first is written
-    }
-    if (h >= p.H[side]) continue;
-    T* yr = y + h * p.ys[side][1];
-    if (vec) {
-      *reinterpret_cast<uint4*>(yr) = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]), pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));
-    } else {
+      } else if constexpr (MODE == kNrLane) {
+        uint4 po;  // the pairs' other halves; nothing (not an infinity) where a lane passes through
+        po.x = __shfl_sync(0xffffffffu, raw[i].x, from);
+        po.y = __shfl_sync(0xffffffffu, raw[i].y, from);
+        po.z = __shfl_sync(0xffffffffu, raw[i].z, from);
+        po.w = __shfl_sync(0xffffffffu, raw[i].w, from);
+        if (!turned) po = make_uint4(0, 0, 0, 0);
+        nr_unpack<T>(po, o);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) yr[e] = from_f32<T>(o[e]);
+        for (int e = 0; e < 8; e += 2) {
+          const float2 z = __fmul2_rn(make_float2(o[e], o[e + 1]), make_float2(sn[e], sn[e + 1]));
+          const float2 u = __ffma2_rn(make_float2(v[e], v[e + 1]), make_float2(cs[e], cs[e + 1]), z);
+          o[e] = u.x, o[e + 1] = u.y;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int d = 8 * l + e;
+          o[e] = v[e] * cs[e];
+          if (on && d < 2 * r) o[e] = fmaf(to_f32(xi[d < r ? d + r : d - r]), sn[e], o[e]);
+        }
+        __syncwarp();  // in place: the row's values are all read before the first is written
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float2 u = __fmul2_rn(make_float2(o[e], o[e + 1]), make_float2(rn, rn));
+        o[e] = u.x, o[e + 1] = u.y;
+      }
+      if (!on) continue;
+      if (vec) {
+        *reinterpret_cast<uint4*>(yi) = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]), pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) yi[e] = from_f32<T>(o[e]);
+      }
     }
+    if (!LOOP || h + kHeads >= h1) break;
   }
+}
+
+template <typename T, int MODE, int kHeads, bool LOOP>
+__global__ void __launch_bounds__(kNrThreads, MODE == kNrAny ? 2 : LOOP ? 3 : 4) norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
+  const uint32_t item = blockIdx.x * (kNrThreads / 32) + (threadIdx.x >> 5);
+  griddep_wait();
+  griddep_launch_dependents();
+  if (item >= p.items) return;
+  const uint32_t per = p.chunks[0] + p.chunks[1], tok = item / per;
+  const int c = (int)(item - tok * per), b = (int)(tok / (uint32_t)p.T), t = (int)(tok - (uint32_t)b * p.T), lane = threadIdx.x & 31;
+  const int h0 = (c < p.chunks[0] ? c : c - p.chunks[0]) * p.per_warp;
+  if (c < p.chunks[0]) nr_rows<T, MODE, kHeads, LOOP, 0>(p, b, t, h0, min(p.H[0], h0 + p.per_warp), lane);
+  else nr_rows<T, MODE, kHeads, LOOP, 1>(p, b, t, h0, min(p.H[1], h0 + p.per_warp), lane);
 }
 
 }  // namespace hkv

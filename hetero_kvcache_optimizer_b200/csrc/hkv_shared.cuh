@@ -22,7 +22,8 @@
 //   K warps   thread = token: dequantised f16 K straight into TMEM (A of S^T, so
 //             K never crosses shared memory again)
 //   V warps   dequantised V^T into shared memory (128-byte swizzle, A of O^T)
-//   MMA warp  S^T(n + 1) ahead of O^T(n)
+//   two MMA warps  one issues S^T, up to two tiles ahead, the other O^T: one thread for
+//             both held S^T(n + 2) back until P(n) was written
 //   softmax   thread = token: kShCols columns each of S^T from TMEM, P as f16
 //             rows [token][row] (N-major B of O^T, 128-byte swizzle)
 // Every wait is bounded (HKV_WAIT_NS); on expiry the device error word is set, the
@@ -35,7 +36,7 @@ namespace hkv {
 
 constexpr int kShMaxGroups = 512;
 constexpr int kShCharge = 6;
-constexpr int kShRawBytes = 24 * 1024;
+constexpr int kShRawBytes = 21504;  // the largest block (ref, group 32)
 
 // Up to 64 rows, even and odd tiles of a CTA are two streams, each with its own
 // softmax warps, running max, O and partial: two tiles' softmax are in flight at a
@@ -44,11 +45,13 @@ constexpr int sh_streams(int n) { return n <= 64 ? 2 : 1; }
 constexpr int sh_col_groups(int n) { return n <= 32 ? 1 : n <= 64 ? 2 : 4; }  // softmax groups that share a tile's rows
 constexpr int sh_softmax_groups(int n) { return sh_streams(n) * sh_col_groups(n); }
 constexpr int sh_halves(int n) { return n <= 32 ? 2 : 1; }  // sets of four K and of four V warps
-constexpr int sh_threads(int n) { return 32 * (4 * sh_softmax_groups(n) + 8 * sh_halves(n) + 2); }
-constexpr int sh_slots(int n) { return n <= 64 ? 4 : 2; }
-constexpr int sh_p_bytes(int n) { return 128 * 128 * (n <= 64 ? 1 : 2); }  // [token][64 rows] f16 blocks
-constexpr int sh_smem(int n) {  // Q | Vt[2] | P[2] | raw slots | alignment
-  return n * 256 + 2 * kPfTileBytes + 2 * sh_p_bytes(n) + sh_slots(n) * kShRawBytes + 1024;
+constexpr int sh_threads(int n) { return 32 * (4 * sh_softmax_groups(n) + 8 * sh_halves(n) + 3); }
+constexpr int sh_slots(int n) { return n <= 32 ? 4 : n <= 64 ? 3 : 2; }
+constexpr int sh_v_bufs(int n) { return n <= 64 ? 3 : 2; }
+constexpr int sh_p_row(int n) { return n <= 32 ? 64 : 128; }  // bytes of a token's row of P, swizzled as wide
+constexpr int sh_p_bytes(int n) { return 128 * sh_p_row(n) * (n <= 64 ? 1 : 2); }  // [row block of 64][token]
+constexpr int sh_smem(int n) {  // Q | Vt | P[2] | raw slots | alignment
+  return n * 256 + sh_v_bufs(n) * kPfTileBytes + 2 * sh_p_bytes(n) + sh_slots(n) * kShRawBytes + 1024;
 }
 constexpr int sh_tmem_cols(int n) { return 128 + (2 + sh_streams(n)) * n <= 256 ? 256 : 512; }  // K[2] | S[2] | O[streams]
 
@@ -146,11 +149,11 @@ __device__ __forceinline__ ShPiece sh_next(const SharedParams& p, const ShGroup*
   return r;
 }
 
-// N-major B descriptor: rows of 64 f16 (128 B, 128-byte swizzle), 8 tokens per
-// 1,024-byte group; the second 64 columns 16 KiB further.
-__device__ __forceinline__ uint64_t sh_desc_n(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(16384 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// N-major B descriptor: a token's row of 64 f16 (128 bytes, 128-byte swizzle; the
+// second 64 columns 16 KiB further) or of 32 (64 bytes, 64-byte swizzle), 8 rows a group.
+__device__ __forceinline__ uint64_t sh_desc_n(uint32_t addr, int row) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(16384 >> 4) << 16) | ((uint64_t)(row * 8 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)(row == 64 ? 4 : 2) << 61);
 }
 constexpr uint32_t sh_idesc(int n, bool b_n_major) {
   return (1u << 4) | (b_n_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
@@ -355,13 +358,15 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
   constexpr int SG = NS * CG;                // softmax groups of 128 threads
   constexpr int COLS = N / CG;               // columns of a softmax thread
   constexpr int SUB = 16;                    // taken at a time
+  constexpr int VB = sh_v_bufs(N), PR = sh_p_row(N);
   constexpr int KH = sh_halves(N);           // sets of four K and of four V warps (a tile each in turn)
   constexpr int R = sh_slots(N);
   constexpr int kThreads = sh_threads(N);
   constexpr uint32_t kBlock = block_bytes(FMT, GROUP);
   constexpr uint32_t kCols = sh_tmem_cols(N);
   extern __shared__ __align__(1024) uint8_t sh_raw[];
-  __shared__ __align__(8) uint64_t raw_full[R], raw_free[R], k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], q_full, drain;
+  __shared__ __align__(8) uint64_t raw_full[R], raw_free[R], k_full[2], v_full[VB], v_free[VB], s_full[2], s_free[2];
+  __shared__ __align__(8) uint64_t p_full[2], pv_done[2], q_full, drain[2];
   __shared__ uint32_t s_tmem;
   __shared__ ShGroup s_g[kShMaxGroups + 1];
   __shared__ int s_valid[16];        // tokens in use of tile n & 15
@@ -370,7 +375,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
   uint8_t* sm = sh_raw + ((1024u - (smem_u32(sh_raw) & 1023u)) & 1023u);
   uint8_t* sQ = sm;
   uint8_t* sV = sQ + N * 256;
-  uint8_t* sP = sV + 2 * kPfTileBytes;
+  uint8_t* sP = sV + VB * kPfTileBytes;
   uint8_t* raw = sP + 2 * sh_p_bytes(N);
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
 
@@ -379,15 +384,20 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
       mbar_init(&raw_full[i], 1);
       mbar_init(&raw_free[i], 8);
     }
+    for (int i = 0; i < VB; ++i) {
+      mbar_init(&v_full[i], 4);
+      mbar_init(&v_free[i], 1);
+    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 4);
-      mbar_init(&v_full[i], 4);
+      mbar_init(&s_free[i], 4 * CG);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4 * CG);
       mbar_init(&pv_done[i], 1);
     }
     mbar_init(&q_full, 4 * SG);
-    mbar_init(&drain, 1);
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
     fence_barrier_init();
   }
   if (warp == 0) {
@@ -520,7 +530,13 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
 #pragma unroll
             for (int i = 0; i < SUB; ++i) x[i] = -INFINITY;
           }
-          uint8_t* prow = sP + buf * sh_p_bytes(N) + (c0 >> 6) * 16384 + tok * 128;
+          if (s0 + SUB == COLS) {  // the last scores of the tile are read
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_free[buf]);
+          }
+          uint8_t* prow = sP + buf * sh_p_bytes(N) + (c0 >> 6) * 16384 + tok * PR;
+          const int turn = PR == 64 ? (tok >> 1) & 3 : tok & 7;
 #pragma unroll
           for (int i = 0; i < SUB; i += 8) {
             uint32_t pk[4];
@@ -531,7 +547,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
               l[s0 + i + e] = z.x, l[s0 + i + e + 1] = z.y;
               pk[e >> 1] = h2u(__floats2half2_rn(y.x, y.y));
             }
-            *reinterpret_cast<uint4*>(prow + (((((c0 + i) & 63) >> 3) ^ (tok & 7)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            *reinterpret_cast<uint4*>(prow + (((((c0 + i) & 63) >> 3) ^ turn) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
           }
         }
         if (!ok) break;
@@ -603,20 +619,20 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
       // ---------------- V ----------------
       const int set = (warp - 4 * SG - 4 * KH) >> 2, vt = t & 127;
       for (int j = KH == 2 ? (n0 ^ set) & 1 : 0; j < pc.n; j += KH) {
-        const uint32_t n = n0 + j, buf = n & 1, slot = n % R;
+        const uint32_t n = n0 + j, vb = n % VB, slot = n % R;
         bool good = true;
         if ((warp & 3) == 0) {
           good = sh_wait(&raw_full[slot], n / R);
-          if (n >= 2) good = sh_wait(&pv_done[buf], (n >> 1) - 1) && good;  // O(n - 2) has read Vt[buf]
+          if (n >= VB) good = sh_wait(&v_free[vb], n / VB - 1) && good;  // O(n - VB) has read Vt[vb]
           __syncwarp();
         }
         ok = bar_and(7 + set, 128, good);
         if (!ok) break;
-        sh_convert_v<FMT, GROUP>(raw + slot * kShRawBytes, sV + buf * kPfTileBytes, vt, s_valid[n & 15]);
+        sh_convert_v<FMT, GROUP>(raw + slot * kShRawBytes, sV + vb * kPfTileBytes, vt, s_valid[n & 15]);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&v_full[buf]);
+          mbar_arrive(&v_full[vb]);
           mbar_arrive(&raw_free[slot]);
         }
       }
@@ -651,38 +667,48 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
       }
       if (!ok)  // copies in flight land before the CTA ends
         for (uint32_t n = issued > R ? issued - R : 0; n < issued; ++n) sh_wait(&raw_full[n % R], n / R);
-    } else if (elect_one()) {
-      // ---------------- MMA: O of a stream is overwritten once P of its first tile says
-      // that its groups have read the last piece's ----------------
-      const uint32_t q0 = smem_u32(sQ), v0 = smem_u32(sV), p0 = smem_u32(sP);
-      auto scores = [&](uint32_t n) {  // S^T(n) = K(n) Q^T; its buffer was read before P(n - 2) was announced
-        const uint32_t buf = n & 1;
-        if (!sh_wait(&k_full[buf], n >> 1)) return false;
-        tc_fence_after();
+    } else if (warp == 4 * SG + 8 * KH + 1) {
+      // ---------------- S^T(n) = K(n) Q^T, up to two tiles ahead of the softmax ----------------
+      if (elect_one()) {
+        const uint32_t q0 = smem_u32(sQ);
+        ok = sh_wait(&q_full, pieces);
+        for (int j = 0; ok && j < pc.n; ++j) {
+          const uint32_t n = n0 + j, buf = n & 1;
+          ok = sh_wait(&k_full[buf], n >> 1) && (n < 2 || sh_wait(&s_free[buf], (n >> 1) - 1));
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          sh_mma_ts(tS + buf * N, tmem + 64 * buf + 8 * kk, pf_desc(q0 + (kk >> 2) * (N * 128) + (kk & 3) * 32),
-                    sh_idesc(N, false), kk > 0);
-        pf_commit(&s_full[buf]);
-        issued = 1;
-        return true;
-      };
-      ok = sh_wait(&q_full, pieces) && scores(n0);
-      for (int j = 0; ok && j < pc.n; ++j) {
-        const uint32_t n = n0 + j, buf = n & 1;
-        if (j + 1 < pc.n) ok = scores(n + 1);
-        ok = ok && sh_wait(&v_full[buf], n >> 1) && sh_wait(&p_full[buf], n >> 1);
+          for (int kk = 0; kk < 8; ++kk)
+            sh_mma_ts(tS + buf * N, tmem + 64 * buf + 8 * kk, pf_desc(q0 + (kk >> 2) * (N * 128) + (kk & 3) * 32),
+                      sh_idesc(N, false), kk > 0);
+          pf_commit(&s_full[buf]);
+          issued = 1;
+        }
+        if (!ok && issued) {  // products in flight end before TMEM is freed
+          pf_commit(&drain[0]);
+          sh_wait(&drain[0], 0);
+        }
+      }
+    } else if (elect_one()) {
+      // ---------------- O^T += V^T P; a stream's O is overwritten once P of a piece's first
+      // tile says that its groups have read the last piece's ----------------
+      const uint32_t v0 = smem_u32(sV), p0 = smem_u32(sP);
+      for (int j = 0; j < pc.n; ++j) {
+        const uint32_t n = n0 + j, buf = n & 1, vb = n % VB;
+        ok = sh_wait(&v_full[vb], n / VB) && sh_wait(&p_full[buf], n >> 1);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
-          sh_mma_ss(tO + (NS == 2 ? buf * N : 0), pf_desc(v0 + buf * kPfTileBytes + (kk >> 2) * 16384 + (kk & 3) * 32),
-                    sh_desc_n(p0 + buf * sh_p_bytes(N) + kk * 2048), sh_idesc(N, true), j >= NS || kk > 0);
+          sh_mma_ss(tO + (NS == 2 ? buf * N : 0), pf_desc(v0 + vb * kPfTileBytes + (kk >> 2) * 16384 + (kk & 3) * 32),
+                    sh_desc_n(p0 + buf * sh_p_bytes(N) + kk * 16 * PR, PR), sh_idesc(N, true), j >= NS || kk > 0);
         pf_commit(&pv_done[buf]);
+        pf_commit(&v_free[vb]);
+        issued = 1;
       }
-      if (!ok && issued) {  // products in flight end before TMEM is freed
-        pf_commit(&drain);
-        sh_wait(&drain, 0);
+      if (!ok && issued) {
+        pf_commit(&drain[1]);
+        sh_wait(&drain[1], 0);
       }
     }
     __syncwarp();

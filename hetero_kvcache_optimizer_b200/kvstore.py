@@ -658,12 +658,12 @@ def rope_table(max_pos: int, rot_dim: int = HEAD_DIM, base: float = 10000.0, sca
     return torch.cat((ang.cos(), ang.sin()), dim=1).to(torch.float32)
 
 
-def _rows(x: torch.Tensor) -> L.HkvRows:
-    r = L.HkvRows()
-    r.data, r.heads = x.data_ptr(), x.shape[1]
-    r.stride_b, r.stride_h = x.stride(0), x.stride(1)
-    r.stride_t = x.stride(2) if x.dim() == 4 else 0
-    return r
+def _rows(x: Optional[torch.Tensor]):
+    """The C view of head vectors [B, H, T, 128] or [B, H, 128] (None: none)."""
+    if x is None:
+        return None
+    st = x.stride()
+    return L.HkvRows(x.data_ptr(), st[0], st[1], st[2] if len(st) == 4 else 0, x.shape[1], 0)
 
 
 def norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: Optional[torch.Tensor] = None,
@@ -684,36 +684,44 @@ def norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: O
     ``table``: f32 [max_pos, rot] of cos | sin (``rope_table``); None: no
     rotation. ``q_out`` / ``k_out``: where to write, e.g. q and k themselves.
     Either of q and k may be None. Returns (q_out, k_out)."""
-    ins = [x for x in (q, k) if x is not None]
-    if not ins:
+    x0 = q if q is not None else k
+    if x0 is None:
         raise ValueError("norm_rope needs q or k")
-    _require_cuda(*(t for t in (q, k, positions, table, q_weight, k_weight, q_out, k_out) if t is not None))
-    x0 = ins[0]
-    if x0.dim() not in (3, 4) or x0.shape[-1] != HEAD_DIM:
+    shape = x0.shape
+    if len(shape) not in (3, 4) or shape[-1] != HEAD_DIM:
         raise ValueError("q and k must be [B, H, T, 128] or [B, H, 128]")
-    B, T = x0.shape[0], (x0.shape[2] if x0.dim() == 4 else 1)
-    outs = []
-    for x, o, name in ((q, q_out, "q"), (k, k_out, "k")):
-        if x is None:
-            if o is not None:
-                raise ValueError(f"{name}_out without {name}")
-            outs.append(None)
-            continue
-        if x.dim() != x0.dim() or x.shape[0] != B or x.shape[2:] != x0.shape[2:] or x.dtype != x0.dtype:
-            raise ValueError("q and k must have one batch, length, head size and dtype")
-        if o is not None and (o.shape != x.shape or o.dtype != x.dtype):
-            raise ValueError(f"{name}_out must have the shape and dtype of {name}")
-        if x.stride(-1) != 1 or (o is not None and o.stride(-1) != 1):
-            raise ValueError("the head dimension must be contiguous")
-        outs.append(o)
-    dt = dtype_code(x0.dtype)
+    B, T = shape[0], (shape[2] if len(shape) == 4 else 1)
+    dtype, device = x0.dtype, x0.device
+    dt = dtype_code(dtype)
     if dt == L.DT_F32:
         raise TypeError("norm_rope takes float16 or bfloat16")
-    weights = [w for w in (q_weight, k_weight) if w is not None]
-    for w in weights:
-        if w.shape != (HEAD_DIM,) or not w.is_contiguous() or w.dtype != weights[0].dtype:
-            raise ValueError("norm weights must be contiguous [128] tensors of one dtype")
-    rot = max_pos = tstride = ps_b = ps_t = 0
+    for t in (q, k, positions, table, q_weight, k_weight, q_out, k_out):
+        if t is not None and t.device != device:
+            _require_cuda(t)
+            raise ValueError("all tensors must be on one device")
+    _require_cuda(x0)
+    for x, o in ((q, q_out), (k, k_out)):
+        if x is None:
+            if o is not None:
+                raise ValueError("an output without its input")
+            continue
+        s = x.shape
+        if len(s) != len(shape) or s[0] != B or s[2:] != shape[2:] or x.dtype != dtype:
+            raise ValueError("q and k must have one batch, length, head size and dtype")
+        if s[1] == 0:
+            raise ValueError("q and k must have heads")
+        if x.stride(-1) != 1 or (o is not None and o.stride(-1) != 1):
+            raise ValueError("the head dimension must be contiguous")
+        if o is not None and (o.shape != s or o.dtype != dtype):
+            raise ValueError("q_out and k_out must have the shape and dtype of q and k")
+    wdt = None
+    for w in (q_weight, k_weight):
+        if w is not None:
+            if w.shape != (HEAD_DIM,) or not w.is_contiguous() or (wdt is not None and w.dtype != wdt):
+                raise ValueError("norm weights must be contiguous [128] tensors of one dtype")
+            wdt = w.dtype
+    rot = max_pos = tstride = ps_b = ps_t = tptr = pptr = 0
+    bits = 32
     if table is not None:
         if table.dtype != torch.float32 or table.dim() != 2 or table.stride(1) != 1:
             raise ValueError("table must be a float32 [max_pos, rot] tensor")
@@ -723,30 +731,26 @@ def norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: O
             raise ValueError("positions must be an int32 or int64 tensor")
         if positions.shape == (B, T):
             ps_b, ps_t = positions.stride()
-        elif x0.dim() == 3 and positions.shape == (B,):
+        elif len(shape) == 3 and positions.shape == (B,):
             ps_b = positions.stride(0)
-        elif x0.dim() == 4 and positions.shape == (T,):
+        elif len(shape) == 4 and positions.shape == (T,):
             ps_t = positions.stride(0)
         else:
             raise ValueError(f"positions must be [B, T] = {[B, T]}, or [T], or [B] for one token each")
-    for t in (q, k, positions, table, q_weight, k_weight, *outs):
-        if t is not None and t.device != x0.device:
-            raise ValueError("all tensors must be on one device")
-    if any(x.shape[1] == 0 for x in ins):
-        raise ValueError("q and k must have heads")
-    with launch_on(x0.device, stream):
-        outs = [torch.empty(x.shape, dtype=x.dtype, device=x.device) if x is not None and o is None else o
-                for x, o in zip((q, k), outs)]
-        if B == 0 or T == 0:
-            return outs[0], outs[1]
-        rows = [ctypes.byref(_rows(t)) if t is not None else None for t in (q, k, outs[0], outs[1])]
-        L.check(L.load().hkv_norm_rope(
-            *rows, dt, B, T, HEAD_DIM, q_weight.data_ptr() if q_weight is not None else None,
-            k_weight.data_ptr() if k_weight is not None else None, dtype_code(weights[0].dtype) if weights else 0,
-            float(eps), positions.data_ptr() if rot else None,
-            64 if rot and positions.dtype == torch.int64 else 32, ps_b, ps_t, table.data_ptr() if rot else None,
-            tstride, max_pos, rot, int(bool(adjacent)), _stream()), "hkv_norm_rope")
-    return outs[0], outs[1]
+        bits = 64 if positions.dtype == torch.int64 else 32
+        tptr, pptr = table.data_ptr(), positions.data_ptr()
+    with launch_on(device, stream):
+        if q is not None and q_out is None:
+            q_out = torch.empty(q.shape, dtype=dtype, device=device)
+        if k is not None and k_out is None:
+            k_out = torch.empty(k.shape, dtype=dtype, device=device)
+        if B and T:
+            L.check(L.load().hkv_norm_rope(
+                _rows(q), _rows(k), _rows(q_out), _rows(k_out), dt, B, T, HEAD_DIM,
+                q_weight.data_ptr() if q_weight is not None else 0, k_weight.data_ptr() if k_weight is not None else 0,
+                dtype_code(wdt) if wdt is not None else 0, eps, pptr, bits, ps_b, ps_t, tptr, tstride, max_pos, rot,
+                1 if adjacent else 0, _stream()), "hkv_norm_rope")
+    return q_out, k_out
 
 
 class SharedPrefix:
