@@ -1453,7 +1453,7 @@ void pages_params(hkv::PagesParams& p, const hkv_int4_store* s, int B, int H, in
 int pages_grid(int64_t entries, int64_t copies, int64_t page_bytes) {
   const int64_t work = std::max((entries + 4 * hkv::kPgThreads - 1) / (4 * hkv::kPgThreads),
                                 copies * ((page_bytes + hkv::kPgChunk - 1) / hkv::kPgChunk));
-  return (int)std::max<int64_t>(1, std::min<int64_t>(work, (int64_t)device_sms() * 6));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(work, (int64_t)device_sms() * 64));
 }
 }  // namespace
 
@@ -1527,11 +1527,12 @@ hkv_status hkv_pages_compact(const hkv_int4_store* src, int32_t B, int32_t H, co
   p.max_pages = into->max_pages;
   p.num_pages = into->num_pages;
   const int64_t entries = (int64_t)B * H * src->max_pages;
-  cudaError_t e = cudaMemsetAsync(p.first, 0x7f, (size_t)src->num_pages * 4, S(stream));
-  if (e == cudaSuccess) e = cudaMemsetAsync(into_refs, 0, (size_t)into->num_pages * 4, S(stream));
-  if (e == cudaSuccess)
-    e = launch_pdl(8, hkv::pages_compact_map_kernel, dim3(pages_grid(entries, 0, 1)), dim3(hkv::kPgThreads), 0, S(stream), p);
-  if (e == cudaSuccess) e = launch_pdl(8, hkv::pages_compact_give_kernel, dim3(1), dim3(hkv::kPgGive), 0, S(stream), p);
+  const dim3 threads(hkv::kPgThreads), spans(cdiv(entries, hkv::kPgSpan));
+  cudaError_t e = launch_pdl(8, hkv::pages_compact_clear_kernel, dim3(pages_grid(std::max(src->num_pages, into->num_pages), 0, 1)),
+                             threads, 0, S(stream), p);
+  if (e == cudaSuccess) e = launch_pdl(8, hkv::pages_compact_map_kernel, dim3(pages_grid(entries, 0, 1)), threads, 0, S(stream), p);
+  if (e == cudaSuccess && spans.x > 1) e = launch_pdl(8, hkv::pages_compact_count_kernel, spans, dim3(hkv::kPgGive), 0, S(stream), p);
+  if (e == cudaSuccess) e = launch_pdl(8, hkv::pages_compact_give_kernel, spans, dim3(hkv::kPgGive), 0, S(stream), p);
   if (e == cudaSuccess)
     e = launch_pdl(8, hkv::pages_compact_apply_kernel,
                    dim3(pages_grid((int64_t)B * H * into->max_pages, std::min<int64_t>(entries, into->num_pages), src->page_stride)),

@@ -6,12 +6,16 @@
 // page; a page with refs == 0 is free. Every operation gives the same ids for
 // the same state: new pages are the lowest free ids, handed out in table order.
 //
-// Three launches each (with programmatic dependent launch): map (parallel over
+// A few launches each (with programmatic dependent launch): map (parallel over
 // the table: what changes, reference counts, which entries want a page), give
-// (one CTA: ranks the wants and the free pages against each other), apply (the
-// new table, and the page bytes, copied by every SM).
-// Bound: HBM for the copies (a 16-byte load and store per 16 bytes, kPgUnroll
-// of them in flight a thread); launch latency for a few pages.
+// (ranks the wants and the free pages against each other), apply (the new table,
+// and the page bytes, copied by every SM).
+// Bound: HBM for the copies, launch latency for a few pages. A copy item is 16 KB,
+// kPgUnroll 16-byte loads a thread before their stores; measured for 16,128 pages
+// of 40 KB (1.32 GB moved): 220 us = 6.0 TB/s, 210 of them copying, with up to 64
+// CTAs queued per SM (245 us with 8 per SM that loop: their ends do not line up),
+// the same with 8 loads a thread. 4 samples of a short prompt: 7.8 us, 64 of eight
+// long ones (18 MB copied): 12.9 us, both launch latency.
 #pragma once
 #include "hkv_common.cuh"
 
@@ -19,7 +23,7 @@ namespace hkv {
 
 constexpr int kPgThreads = 256;    // map and apply
 constexpr int kPgGive = 1024;      // give: one CTA
-constexpr int kPgUnroll = 8;
+constexpr int kPgUnroll = 4;
 constexpr int kPgChunk = kPgThreads * kPgUnroll * 16;  // bytes of a copy item
 
 struct PagesParams {
@@ -232,7 +236,20 @@ __global__ void __launch_bounds__(kPgThreads) pages_fork_apply_kernel(const __gr
 
 // ---------------------------------------------------------------- compact
 // The source's pages in order of their first table entry become pages 0, 1, ...
-// of another pool. first[] starts at 0x7f7f7f7f.
+// of another pool. The ranking is spread over CTAs of kPgSpan entries (one CTA
+// took 38 us of 256 for 16,128 pages): with more than one, each first publishes how
+// many first entries it has, then adds up those before it.
+constexpr int kPgSpan = kPgPages * kPgGive;
+
+__global__ void __launch_bounds__(kPgThreads) pages_compact_clear_kernel(const __grid_constant__ PagesParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  for (int i = blockIdx.x * kPgThreads + threadIdx.x; i < max(p.src_num_pages, p.num_pages); i += gridDim.x * kPgThreads) {
+    if (i < p.src_num_pages) p.first[i] = 0x7fffffff;
+    if (i < p.num_pages) p.refs[i] = 0;
+  }
+}
+
 __global__ void __launch_bounds__(kPgThreads) pages_compact_map_kernel(const __grid_constant__ PagesParams p) {
   griddep_wait();
   griddep_launch_dependents();
@@ -244,38 +261,53 @@ __global__ void __launch_bounds__(kPgThreads) pages_compact_map_kernel(const __g
   }
 }
 
-// Ranks the first entries: want[e] is the new id of the page that entry e names
-// first. Pages behind the sequence's length keep their place but are not copied.
-__global__ void __launch_bounds__(kPgGive) pages_compact_give_kernel(const __grid_constant__ PagesParams p) {
-  __shared__ int s_warp[32];
+// Which of the thread's kPgPages entries from e1 on name a page first.
+__device__ __forceinline__ unsigned pg_firsts(const PagesParams& p, int e1, int n, int (&page)[kPgPages]) {
+  unsigned mask = 0;
+#pragma unroll
+  for (int j = 0; j < kPgPages; ++j) page[j] = e1 + j < n ? p.src_table[e1 + j] : -1;
+#pragma unroll
+  for (int j = 0; j < kPgPages; ++j)
+    if (pg_ok(page[j], p.src_num_pages) && p.first[page[j]] == e1 + j) mask |= 1u << j;
+  return mask;
+}
+
+__global__ void __launch_bounds__(kPgGive) pages_compact_count_kernel(const __grid_constant__ PagesParams p) {
   griddep_wait();
   griddep_launch_dependents();
-  const int n = p.B * p.H * p.src_max_pages;
-  int live = 0;
-  for (int e0 = 0; e0 < n; e0 += kPgPages * kPgGive) {
-    const int e1 = e0 + kPgPages * threadIdx.x;
-    int page[kPgPages];
-    unsigned mask = 0;
+  __shared__ int s_warp[32];
+  int page[kPgPages], total;
+  const unsigned mask = pg_firsts(p, blockIdx.x * kPgSpan + kPgPages * threadIdx.x, p.B * p.H * p.src_max_pages, page);
+  pg_scan(__popc(mask), total, s_warp);
+  if (threadIdx.x == 0) p.from[blockIdx.x] = total;
+}
+
+// list[3 r]: the page of rank r, want[e]: the rank at its first entry e. Pages behind
+// the sequence's length keep their place but are not copied (list[3 r + 2] = 0).
+__global__ void __launch_bounds__(kPgGive) pages_compact_give_kernel(const __grid_constant__ PagesParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  __shared__ int s_warp[32];
+  const int n = p.B * p.H * p.src_max_pages, e1 = blockIdx.x * kPgSpan + kPgPages * threadIdx.x;
+  int before = 0, total;
+  for (int i = threadIdx.x; i < blockIdx.x; i += kPgGive) before += p.from[i];
+  pg_scan(before, total, s_warp);
+  before = total;
+  int page[kPgPages];
+  const unsigned mask = pg_firsts(p, e1, n, page);
+  int r = before + pg_scan(__popc(mask), total, s_warp);
 #pragma unroll
-    for (int j = 0; j < kPgPages; ++j) page[j] = e1 + j < n ? p.src_table[e1 + j] : -1;
-#pragma unroll
-    for (int j = 0; j < kPgPages; ++j)
-      if (pg_ok(page[j], p.src_num_pages) && p.first[page[j]] == e1 + j) mask |= 1u << j;
-    int total;
-    int r = live + pg_scan(__popc(mask), total, s_warp);
-#pragma unroll
-    for (int j = 0; j < kPgPages; ++j)
-      if (mask >> j & 1) {
-        const int e = e1 + j, u = e / p.src_max_pages, i = e - u * p.src_max_pages;
-        p.want[e] = r;
-        p.list[3 * r] = page[j];
-        p.list[3 * r + 1] = r;
-        p.list[3 * r + 2] = (int64_t)i * p.page_tokens < p.src_lengths[u / p.H] ? p.page_tokens / HKV_BLOCK_TOKENS * (p.block_bytes >> 4) : 0;
-        ++r;
-      }
-    live += total;
-  }
-  if (threadIdx.x == 0) {
+  for (int j = 0; j < kPgPages; ++j)
+    if (mask >> j & 1) {
+      const int e = e1 + j, u = e / p.src_max_pages, i = e - u * p.src_max_pages;
+      p.want[e] = r;
+      p.list[3 * r] = page[j];
+      p.list[3 * r + 1] = r;
+      p.list[3 * r + 2] = (int64_t)i * p.page_tokens < p.src_lengths[u / p.H] ? p.page_tokens / HKV_BLOCK_TOKENS * (p.block_bytes >> 4) : 0;
+      ++r;
+    }
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
+    const int live = before + total;
     p.count[0] = min(live, p.num_pages);
     if (live > p.num_pages) hkv_flag_error(HKV_DEVERR_CAPACITY);
   }

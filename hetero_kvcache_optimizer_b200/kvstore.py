@@ -53,6 +53,12 @@ def launch_on(device: torch.device, stream: Optional[torch.cuda.Stream] = None):
     return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
+def raw_stream(device: torch.device) -> int:
+    """Handle of the device's current stream, without making a Stream object
+    (4 us of a call's time on the host)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def page_bytes(fmt: str, group: int, page_tokens: int) -> int:
     n = L.load().hkv_page_bytes(FORMATS[fmt], group, page_tokens)
     if n <= 0:
@@ -749,7 +755,7 @@ def norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: O
                 _rows(q), _rows(k), _rows(q_out), _rows(k_out), dt, B, T, HEAD_DIM,
                 q_weight.data_ptr() if q_weight is not None else 0, k_weight.data_ptr() if k_weight is not None else 0,
                 dtype_code(wdt) if wdt is not None else 0, eps, pptr, bits, ps_b, ps_t, tptr, tstride, max_pos, rot,
-                1 if adjacent else 0, _stream()), "hkv_norm_rope")
+                1 if adjacent else 0, raw_stream(device)), "hkv_norm_rope")
     return q_out, k_out
 
 
@@ -828,6 +834,6 @@ def decode_shared(q: torch.Tensor, prefix: SharedPrefix, store: Optional[Int4KVS
               else workspace(nbytes, q.device, kind="shared"))
         L.check(lib.hkv_decode_shared(
             q.data_ptr(), dtype_code(q.dtype), q.stride(0), q.stride(1), *segs, B, Hq, Hkv, D, float(sm_scale), ctas,
-            ws.data_ptr(), ws.numel(), out.data_ptr(), dtype_code(out.dtype), out.stride(0), out.stride(1), _stream()),
+            ws.data_ptr(), ws.numel(), out.data_ptr(), dtype_code(out.dtype), out.stride(0), out.stride(1), raw_stream(q.device)),
             "hkv_decode_shared")
     return out[:, :, None, :] if squeeze else out

@@ -52,7 +52,7 @@ class PagePool:
         st = self.store
         s = st.struct()
         L.check(getattr(L.load(), name)(ctypes.byref(s), st.batch, st.kv_heads, *args, self._ws.data_ptr(),
-                                        self._ws.numel(), kv._stream()), name)
+                                        self._ws.numel(), kv.raw_stream(self.refs.device)), name)
 
     def _per_sequence(self, x: Union[torch.Tensor, Sequence[int]], name: str) -> torch.Tensor:
         if not isinstance(x, torch.Tensor):
