@@ -50,7 +50,9 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // (a chunked prefill's launches overlap their start with the previous one's
 // drain: 4.82 -> 4.68 ms for config 2's 896 chunk launches); the append kernel,
 // whose blocks would wait resident beside the decode kernel's, measured slower
-// with it (2.608 ms) and launches normally. HKV_PDL (bit mask: 1 decode,
+// with it (2.608 ms) and launches normally, as do the three launches of a
+// shared-prefix decode (72 KB to 222 KB of shared memory keep them from overlapping;
+// 8 samples of a 32K prompt: 59.6 us with it, 55.8 us without). HKV_PDL (bit mask: 1 decode,
 // 2 append, 4 quantise-pack, 8 norm + rotation and page operations; default 13)
 // overrides this for experiments.
 bool pdl_enabled(int which) {
@@ -244,7 +246,7 @@ hkv_status launch_decode_t(const hkv::DecodeParams& p, int smem, cudaStream_t st
                                     cudaFuncAttributeMaxDynamicSharedMemorySize, kDynSmemBudget);
   });
   if (attr_err != cudaSuccess) return cuda_fail(attr_err);
-  const cudaError_t e = launch_pdl(1, hkv::decode_kernel<FMT, GROUP, DTy, STATS, APPEND>, dim3(p.sc.C),
+  const cudaError_t e = launch_pdl(p.alone ? 0 : 1, hkv::decode_kernel<FMT, GROUP, DTy, STATS, APPEND>, dim3(p.sc.C),
                                    dim3(hkv::decode_threads(FMT, APPEND)), smem, st, p);
   if (e != cudaSuccess) return cuda_fail(e);
   return launch_status();
@@ -370,7 +372,8 @@ hkv_status run_decode(const void* q, int q_dtype, int64_t q_sb, int64_t q_sh, co
                       const hkv_dense_kv* dense, int B, int Hq, int Hkv, int D, float sm_scale, int ctas,
                       void* workspace, size_t workspace_bytes, void* out, int out_dtype, int64_t out_sb,
                       int64_t out_sh, float* out_o, float* out_ml, cudaStream_t st, float* tile_stats = nullptr,
-                      int stat_tiles = 0, float* unit_ml = nullptr, const AppendArgs* app = nullptr) {
+                      int stat_tiles = 0, float* unit_ml = nullptr, const AppendArgs* app = nullptr,
+                      bool alone = false) {
   hkv_status rc = check_decode_args(q, q_dtype, body, dense, B, Hq, Hkv, D);
   if (rc != HKV_OK) return rc;
   if (!(sm_scale > 0.f) || !std::isfinite(sm_scale)) return HKV_ERR_ARG;
@@ -416,6 +419,7 @@ hkv_status run_decode(const void* q, int q_dtype, int64_t q_sb, int64_t q_sh, co
   p.tile_stats = tile_stats;
   p.stat_tiles = stat_tiles;
   p.unit_ml = unit_ml;
+  p.alone = alone;
   if (app) {
     p.k_new = app->k_new;
     p.v_new = app->v_new;
@@ -567,14 +571,25 @@ hkv_status launch_shared_t(const hkv::SharedParams& p, cudaStream_t st) {
                                     hkv::sh_smem(N));
   });
   if (attr_err != cudaSuccess) return cuda_fail(attr_err);
-  const cudaError_t e = launch_pdl(16, hkv::shared_prefix_kernel<FMT, GROUP, N>, dim3(p.C), dim3(hkv::sh_threads(N)),
-                                   hkv::sh_smem(N), st, p);
-  return e == cudaSuccess ? launch_status() : cuda_fail(e);
+  hkv::shared_prefix_kernel<FMT, GROUP, N><<<p.C, hkv::sh_threads(N), hkv::sh_smem(N), st>>>(p);
+  return launch_status();
+}
+template <int FMT, int GROUP>
+hkv_status launch_rows_t(const hkv::SharedParams& p, cudaStream_t st) {
+  static std::once_flag once;
+  static cudaError_t attr_err = cudaSuccess;
+  std::call_once(once, [] {
+    attr_err = cudaFuncSetAttribute(hkv::shared_rows_kernel<FMT, GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    hkv::kRowsSmem);
+  });
+  if (attr_err != cudaSuccess) return cuda_fail(attr_err);
+  hkv::shared_rows_kernel<FMT, GROUP><<<p.C, hkv::kRowsThreads, hkv::kRowsSmem, st>>>(p);
+  return launch_status();
 }
 template <int FMT, int GROUP>
 hkv_status launch_shared_n(const hkv::SharedParams& p, cudaStream_t st) {
   switch (p.N) {
-    case 16: return launch_shared_t<FMT, GROUP, 16>(p, st);
+    case 16: return launch_rows_t<FMT, GROUP>(p, st);
     case 32: return launch_shared_t<FMT, GROUP, 32>(p, st);
     case 64: return launch_shared_t<FMT, GROUP, 64>(p, st);
   }
@@ -592,7 +607,7 @@ hkv_status launch_shared(const hkv::SharedParams& p, cudaStream_t st) {
 // Rows per product, CTAs and workspace of a shared-prefix decode:
 // own part's workspace | its (o, m, l) | the pieces' (o, m, l).
 struct SharedPlan {
-  int N, C;
+  int N, ns, C;
   size_t own_ws, own_o, own_ml, part_o, part_ml, bytes;  // offsets
 };
 hkv_status shared_plan(const hkv_int4_store* prefix, const int32_t* start, int P, const hkv_int4_store* body,
@@ -609,7 +624,10 @@ hkv_status shared_plan(const hkv_int4_store* prefix, const int32_t* start, int P
     rows = std::max<int64_t>(rows, (int64_t)(start[g + 1] - start[g]) * G);
   }
   SharedPlan pl;
+  // Rows of a unit that share its dequantised tiles: the narrowest product that holds the
+  // largest group (its cost grows with its width); at most 16 rows run on shared_rows_kernel.
   pl.N = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  pl.ns = pl.N == 16 ? 1 : hkv::sh_streams(pl.N);
   pl.C = std::min(ctas > 0 ? ctas : device_sms(), 65535);
   int64_t units = 0, steps = 0;
   const int64_t cap = (int64_t)prefix->max_pages * (prefix->page_tokens / HKV_BLOCK_TOKENS);
@@ -635,7 +653,7 @@ hkv_status shared_plan(const hkv_int4_store* prefix, const int32_t* start, int P
   pl.own_o = at;
   pl.own_ml = pl.own_o + (own ? (size_t)B * Hq * HKV_D * 4 : 0);
   pl.part_o = (pl.own_ml + (own ? (size_t)B * Hq * 8 : 0) + 255) & ~(size_t)255;
-  const size_t parts = (size_t)(units + pl.C) * hkv::sh_streams(pl.N) * pl.N;
+  const size_t parts = (size_t)(units + pl.C) * pl.ns * pl.N;
   pl.part_ml = pl.part_o + parts * HKV_D * 4;
   pl.bytes = pl.part_ml + parts * 8;
   *out = pl;
@@ -1587,16 +1605,18 @@ hkv_status hkv_decode_shared(const void* q, int32_t q_dtype, int64_t q_stride_b,
   p.out_sh = out_stride_h;
   p.B = B;
   p.N = pl.N;
+  p.ns = pl.ns;
   std::memcpy(p.start, group_start, sizeof(int32_t) * (n_groups + 1));
   rc = prefix->format == HKV_FMT_REF ? launch_shared<HKV_FMT_REF>(p, S(stream)) : launch_shared<HKV_FMT_FP16MIN>(p, S(stream));
   if (rc != HKV_OK) return rc;
   if (own) {
     rc = run_decode(q, q_dtype, q_stride_b, q_stride_h, body, dense, B, Hq, Hkv, D, sm_scale, ctas, ws, pl.own_o, nullptr,
-                    HKV_DT_F32, 0, 0, const_cast<float*>(p.own_o), const_cast<float*>(p.own_ml), S(stream));
+                    HKV_DT_F32, 0, 0, const_cast<float*>(p.own_o), const_cast<float*>(p.own_ml), S(stream), nullptr, 0,
+                    nullptr, nullptr, /*alone=*/true);
     if (rc != HKV_OK) return rc;
   }
-  const cudaError_t e = launch_pdl(32, hkv::shared_merge_kernel, dim3(B * Hq), dim3(128), 0, S(stream), p);
-  return e == cudaSuccess ? launch_status() : cuda_fail(e);
+  hkv::shared_merge_kernel<<<B * Hq, 128, 0, S(stream)>>>(p);
+  return launch_status();
 }
 
 }  // extern "C"

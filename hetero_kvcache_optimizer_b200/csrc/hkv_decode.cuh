@@ -118,6 +118,7 @@ struct DecodeParams {
   int out_dtype;
   int64_t out_sb, out_sh;
   float* out_o;    // [B][Hq][128] f32 (partial mode, when non-null)
+  int alone;       // launched without programmatic stream serialization
   float* out_ml;   // [B][Hq][2]
   // where the attention mass fell (optional, normalised mode): per INT4 body tile
   // k < stat_tiles of unit u, per consumer warp and head, (sum of the warp's

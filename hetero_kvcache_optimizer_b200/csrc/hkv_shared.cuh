@@ -64,15 +64,15 @@ struct SharedParams {
   float qscale;             // sm_scale * log2(e)
   int* counters;            // own part's merge counters, zeroed here
   int n_counters;
-  float* part_o;            // [C + units][streams][N][128]
-  float* part_ml;           // [C + units][streams][N][2]
+  float* part_o;            // [C + units][ns][N][128]
+  float* part_ml;           // [C + units][ns][N][2]
   // merge
   const float* own_o;       // [B][Hq][128], or NULL
   const float* own_ml;      // [B][Hq][2]
   void* out;
   int out_dtype;
   int64_t out_sb, out_sh;
-  int B, N;
+  int B, N, ns;             // N: rows of a row tile; ns: partials of a piece
   int start[kShMaxGroups + 1];  // sequences [start[p], start[p + 1]) are group p
 };
 
@@ -404,8 +404,6 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "n"(kCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
-  griddep_wait();
-  griddep_launch_dependents();
   for (int i = blockIdx.x * kThreads + t; i < p.n_counters; i += gridDim.x * kThreads) p.counters[i] = 0;
   if (warp == 1) sh_schedule(p, s_g);
   tc_fence_before();
@@ -725,6 +723,430 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
   }
 }
 
+// ---------------------------------------------------------------- few rows
+// The same partials for at most 16 rows on mma.sync (m16n8k16), tokens as M, two
+// column blocks of 8 rows. Few rows are bound by unpacking the codes, and here they
+// meet the tensor cores almost as they are stored:
+//   S = sum_g s_g (sum_{d in g} (1024 + n_d) q_d - 1024 sum q_d) + sum_g min_g sum q_d:
+//     K's codes are OR-ed into f16 numbers 1024 + n (or + 16 n, against q / 16), one
+//     instruction per pair; the accumulator starts at -1024 sum q, exact as the
+//     products are; the group's scale multiplies in fp32 afterwards; fp16min's mins
+//     are one more product, against sum q_d in f16 high and low parts;
+//   O^T += (n V^T) (s_g P)^T: the codes as exact integers, their scale in P's operand
+//     (rounded to f16 with it), fp16min's mins one more product into an accumulator
+//     of its own. The ref format's zero points enter as z sum q_d and as n - z.
+// So nothing of K is rounded, and no operand crosses shared memory twice. Two groups
+// of four consumer warps take every second tile, 32 tokens a warp.
+constexpr int kRowsThreads = 320;  // 8 consumer warps, 2 producers
+constexpr int kRowsSlots = 6;
+constexpr int kRowsPitch = HKV_D + 4;
+constexpr int kRowsSmem = kRowsSlots * kShRawBytes + 16 * 256 + 8 * 16 * kRowsPitch * 4;  // raw slots | query fragments | O per warp
+
+template <int FMT, int GROUP>
+__global__ void __launch_bounds__(kRowsThreads, 1) shared_rows_kernel(const __grid_constant__ SharedParams p) {
+  constexpr int ROWS = 16, NG = HKV_D / GROUP, WPG = 4 / NG, NB = 2, R = kRowsSlots;
+  constexpr uint32_t kBlock = block_bytes(FMT, GROUP);
+  extern __shared__ __align__(1024) uint8_t sh_raw[];
+  __shared__ __align__(8) uint64_t raw_full[R], raw_free[R];
+  __shared__ ShGroup s_g[kShMaxGroups + 1];
+  __shared__ int s_valid[16];
+  __shared__ float s_ps[ROWS][4], s_pb[ROWS][4];                  // per row and 32 dims: sums of q, and of q as multiplied
+  __shared__ __align__(8) float s_nb[4][ROWS], s_qs[4][ROWS];    // per group and row: -1024 sum, sum
+  __shared__ float s_wm[8][16], s_wl[8][16];                     // per warp and row: m, l
+  uint8_t* ring = sh_raw;
+  uint4* sQ = reinterpret_cast<uint4*>(ring + R * kShRawBytes);  // [ROWS / 8][4][32 lanes]
+  float* comb = reinterpret_cast<float*>(ring + R * kShRawBytes + ROWS * 256);
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  if (t == 0) {
+    for (int i = 0; i < R; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_free[i], 4);
+    }
+    fence_barrier_init();
+  }
+  for (int i = blockIdx.x * kRowsThreads + t; i < p.n_counters; i += gridDim.x * kRowsThreads) p.counters[i] = 0;
+  if (warp == 0) sh_schedule(p, s_g);
+  __syncthreads();
+  const int total = s_g[p.P].step;
+  int at = sh_cut(total, p.C, blockIdx.x);
+  const int end = sh_cut(total, p.C, blockIdx.x + 1);
+  uint32_t n0 = 0;  // tiles of the CTA before this piece
+
+  if (warp >= 8) {
+    // ---------------- producers: the tiles of the warp's parity ----------------
+    const int par = warp - 8;
+    bool ok = true;
+    uint32_t last = 0;  // behind the last tile issued
+    while (ok) {
+      const ShPiece pc = sh_next(p, s_g, at, end);
+      if (pc.n == 0) break;
+      const int u = pc.g * p.Hkv + pc.h, len = max(0, p.prefix.lengths ? p.prefix.lengths[pc.g] : p.prefix.len);
+      int64_t ids = -1;
+      int i = 0;
+      for (int j = (n0 ^ par) & 1; j < pc.n; j += 2, ++i) {
+        const uint32_t n = n0 + j, slot = n % R;
+        const int tok = (pc.t0 + j) * HKV_BLOCK_TOKENS;
+        if ((i & 31) == 0) ids = j + 2 * lane < pc.n ? store_page(p.prefix, u, tok + 2 * lane * HKV_BLOCK_TOKENS) : -1;
+        const int64_t page = __shfl_sync(0xffffffffu, ids, i & 31);
+        if (n >= R && !__all_sync(0xffffffffu, mbar_wait(&raw_free[slot], (n / R - 1) & 1))) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          s_valid[n & 15] = page >= 0 ? min(HKV_BLOCK_TOKENS, len - tok) : 0;
+          if (page >= 0) {
+            const uint8_t* src = static_cast<const uint8_t*>(p.prefix.pages) + page * p.prefix.page_stride +
+                                 (int64_t)((tok % p.prefix.page_tokens) / HKV_BLOCK_TOKENS) * kBlock;
+            mbar_arrive_expect_tx(&raw_full[slot], kBlock);
+            bulk_g2s(ring + slot * kShRawBytes, src, kBlock, &raw_full[slot]);
+          } else {  // no such page: the tile counts as hidden
+            hkv_flag_error(HKV_DEVERR_BAD_PAGE);
+            mbar_arrive(&raw_full[slot]);
+          }
+        }
+        __syncwarp();
+        last = n + 1;
+      }
+      n0 += pc.n;
+    }
+    // every copy this warp issued lands before the CTA ends (its parity's slots: R is even)
+    static_assert(R % 2 == 0, "a slot belongs to one producer");
+    for (uint32_t n = last > R ? last - R : 0; n < last; ++n)
+      if ((n & 1) == (uint32_t)par) mbar_wait(&raw_full[n % R], (n / R) & 1);
+    return;
+  }
+
+  // ---------------- consumers ----------------
+  const int grp = warp >> 2, wg = warp & 3, r = lane >> 2, j4 = lane & 3, t0 = 32 * wg;
+  const float qs = p.qscale;
+  bool ok = true;
+  while (ok) {
+    const ShPiece pc = sh_next(p, s_g, at, end);
+    if (pc.n == 0) break;
+    const int rows = (p.start[pc.g + 1] - p.start[pc.g]) * p.G - pc.rt * ROWS;
+    // query fragments: block b, word w, lane (r, j4): q of row 8 b + r at dims 32 w + 2 j4 + {0, 1},
+    // (+ {8, 9}) / 16, + {16, 17}, (+ {24, 25}) / 16; sums of 32 dims beside them
+    {
+      const int c = warp, b = c >> 2, w = c & 3, n = 8 * b + r;
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (n < rows) {
+        const int row = pc.rt * ROWS + n, sq = row / p.G;
+        const int64_t base = (int64_t)(p.start[pc.g] + sq) * p.q_sb + (int64_t)(pc.h * p.G + row - sq * p.G) * p.q_sh + 32 * w + 2 * j4;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = load_any(p.q, p.q_dtype, base + 8 * (e >> 1) + (e & 1));
+      }
+      float ps = 0.f, pb = 0.f;
+      uint32_t f[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float d = e & 1 ? 0.0625f : 1.f, up = e & 1 ? 16.f : 1.f;
+        const __half a = __float2half_rn(to_f32(__float2half_rn(v[2 * e])) * d), q2 = __float2half_rn(to_f32(__float2half_rn(v[2 * e + 1])) * d);
+        f[e] = (uint32_t)__half_as_ushort(a) | ((uint32_t)__half_as_ushort(q2) << 16);
+        const float sum = __half2float(a) + __half2float(q2);
+        pb += sum;
+        ps += up * sum;
+      }
+      sQ[c * 32 + lane] = make_uint4(f[0], f[1], f[2], f[3]);
+#pragma unroll
+      for (int k = 1; k < 4; k <<= 1) {
+        ps += __shfl_xor_sync(0xffffffffu, ps, k);
+        pb += __shfl_xor_sync(0xffffffffu, pb, k);
+      }
+      if (j4 == 0) s_ps[n][w] = ps, s_pb[n][w] = pb;
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    for (int c = t; c < NG * ROWS; c += 256) {
+      const int g = c / ROWS, n = c - g * ROWS;
+      float a = 0.f, b = 0.f;
+      for (int w = g * WPG; w < (g + 1) * WPG; ++w) a += s_ps[n][w], b += s_pb[n][w];
+      s_qs[g][n] = a;
+      s_nb[g][n] = -1024.f * b;
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    uint32_t qbias[NB] = {0u, 0u};  // fp16min: sum q_d of the groups, f16 high then low parts, as a B operand
+    if constexpr (FMT == HKV_FMT_FP16MIN) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int n = 8 * b + r;
+        auto part = [&](int i) -> uint32_t {  // part i < NG: high of group i, else low of group i - NG
+          const float v = i < 2 * NG ? s_qs[i % NG][n] : 0.f;
+          const __half hi = __float2half_rn(v);
+          return i < 2 * NG ? __half_as_ushort(i < NG ? hi : __float2half_rn(v - __half2float(hi))) : 0u;
+        };
+        qbias[b] = part(2 * j4) | (part(2 * j4 + 1) << 16);
+      }
+    }
+    float o[NB][8][4], zc[NB][4], m[NB][2], l[NB][2];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[b][i][0] = o[b][i][1] = o[b][i][2] = o[b][i][3] = 0.f;
+      zc[b][0] = zc[b][1] = zc[b][2] = zc[b][3] = l[b][0] = l[b][1] = 0.f;
+      m[b][0] = m[b][1] = -1.0e30f;
+    }
+    for (int j = (n0 ^ grp) & 1; j < pc.n; j += 2) {
+      const uint32_t n = n0 + j, slot = n % R;
+      if (!__all_sync(0xffffffffu, mbar_wait(&raw_full[slot], (n / R) & 1))) {
+        ok = false;
+        break;
+      }
+      const uint8_t* blk = ring + slot * kShRawBytes;
+      const uint8_t* meta = blk + HKV_META_OFF;
+      const int nv = s_valid[n & 15] - t0;  // tokens of this warp's 32 in use
+      if (nv > 0) {
+        // ---- scores x[s][b]: tokens 16 s + r and 16 s + r + 8, rows 2 j4 and 2 j4 + 1 of block b
+        uint32_t kw[2][2][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4 c = *reinterpret_cast<const uint4*>(blk + (t0 + 8 * i + r) * HKV_CODE_BYTES + 16 * j4);
+          kw[i >> 1][i & 1][0] = c.x, kw[i >> 1][i & 1][1] = c.y, kw[i >> 1][i & 1][2] = c.z, kw[i >> 1][i & 1][3] = c.w;
+        }
+        float sc[2][2][NG], x[2][NB][4];
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) {
+          const int tk = t0 + 16 * s2;
+#pragma unroll
+          for (int b = 0; b < NB; ++b) x[s2][b][0] = x[s2][b][1] = x[s2][b][2] = x[s2][b][3] = 0.f;
+          if constexpr (FMT == HKV_FMT_FP16MIN) {
+            const __half* ks = reinterpret_cast<const __half*>(meta) + (tk + r) * NG;
+            ld_row_h<NG>(ks, 0, sc[s2][0]);
+            ld_row_h<NG>(ks, 8, sc[s2][1]);
+            // mins of tokens r and r + 8, groups (2 j4, 2 j4 + 1) mod NG, against qbias
+            const uint8_t* km = meta + 256 * NG + tk * NG * 2;
+            uint32_t m0 = 0u, m1 = 0u;
+            if constexpr (NG == 4) {
+              m0 = reinterpret_cast<const uint32_t*>(km)[2 * r + (j4 & 1)];
+              m1 = reinterpret_cast<const uint32_t*>(km)[2 * (r + 8) + (j4 & 1)];
+            } else if constexpr (NG == 2) {
+              if (j4 < 2) m0 = reinterpret_cast<const uint32_t*>(km)[r], m1 = reinterpret_cast<const uint32_t*>(km)[r + 8];
+            } else if (j4 == 0) {
+              m0 = reinterpret_cast<const uint16_t*>(km)[r] * 0x10001u;
+              m1 = reinterpret_cast<const uint16_t*>(km)[r + 8] * 0x10001u;
+            }
+            const uint32_t ab[4] = {m0, m1, 0u, 0u};
+#pragma unroll
+            for (int b = 0; b < NB; ++b) mma16816<__half>(x[s2][b], ab, qbias[b], 0u);
+          } else {
+            const float* ks = reinterpret_cast<const float*>(meta) + (tk + r) * NG;
+            ld_row<NG>(ks, 0, sc[s2][0]);
+            ld_row<NG>(ks, 8, sc[s2][1]);
+          }
+        }
+        float c[2][NB][4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int g = w / WPG;
+          uint32_t a0[2][4], a1[2][4];
+#pragma unroll
+          for (int s2 = 0; s2 < 2; ++s2) {
+            const uint32_t wa = kw[s2][0][w], wb = kw[s2][1][w], wa8 = wa >> 8, wb8 = wb >> 8;
+            a0[s2][0] = biased1(wa), a0[s2][1] = biased1(wb), a0[s2][2] = biased16(wa), a0[s2][3] = biased16(wb);
+            a1[s2][0] = biased1(wa8), a1[s2][1] = biased1(wb8), a1[s2][2] = biased16(wa8), a1[s2][3] = biased16(wb8);
+          }
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            const uint4 f = sQ[(b * 4 + w) * 32 + lane];
+            if (w % WPG == 0) {
+              const float2 nb = *reinterpret_cast<const float2*>(&s_nb[g][8 * b + 2 * j4]);
+              const float ci[4] = {nb.x, nb.y, nb.x, nb.y};
+              mma16816_c(c[0][b], a0[0], f.x, f.y, ci);
+              mma16816_c(c[1][b], a0[1], f.x, f.y, ci);
+            } else {
+              mma16816<__half>(c[0][b], a0[0], f.x, f.y);
+              mma16816<__half>(c[1][b], a0[1], f.x, f.y);
+            }
+            mma16816<__half>(c[0][b], a1[0], f.z, f.w);
+            mma16816<__half>(c[1][b], a1[1], f.z, f.w);
+            if (w % WPG == WPG - 1) {
+#pragma unroll
+              for (int s2 = 0; s2 < 2; ++s2) {
+                float *xx = x[s2][b], *cc = c[s2][b];
+                if constexpr (FMT == HKV_FMT_REF) {  // minus the zero points' share
+                  const float2 q2 = *reinterpret_cast<const float2*>(&s_qs[g][8 * b + 2 * j4]);
+                  const uint8_t* kz = meta + 1024 * NG + (t0 + 16 * s2 + r) * NG + g;
+                  const float za = -(float)kz[0], zb = -(float)kz[8 * NG];
+                  cc[0] = fmaf(za, q2.x, cc[0]), cc[1] = fmaf(za, q2.y, cc[1]);
+                  cc[2] = fmaf(zb, q2.x, cc[2]), cc[3] = fmaf(zb, q2.y, cc[3]);
+                }
+                const float2 lo = __ffma2_rn(make_float2(sc[s2][0][g], sc[s2][0][g]), make_float2(cc[0], cc[1]), make_float2(xx[0], xx[1]));
+                const float2 hi = __ffma2_rn(make_float2(sc[s2][1][g], sc[s2][1][g]), make_float2(cc[2], cc[3]), make_float2(xx[2], xx[3]));
+                xx[0] = lo.x, xx[1] = lo.y, xx[2] = hi.x, xx[3] = hi.y;
+              }
+            }
+          }
+        }
+        // ---- softmax: the warp's own running max, moved when a score beats it by 2^8
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            float* xx = x[s2][b];
+            const float2 lo = __fmul2_rn(make_float2(xx[0], xx[1]), make_float2(qs, qs)), hi = __fmul2_rn(make_float2(xx[2], xx[3]), make_float2(qs, qs));
+            xx[0] = lo.x, xx[1] = lo.y, xx[2] = hi.x, xx[3] = hi.y;
+          }
+        if (nv < 32) {  // the prefix ends in here
+#pragma unroll
+          for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (16 * s2 + r + 4 * (i & 2) >= nv) x[s2][b][i] = -INFINITY;
+        }
+        float top[NB][2];
+        bool need = false;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            top[b][e] = fmax3(fmaxf(x[0][b][e], x[0][b][e + 2]), x[1][b][e], x[1][b][e + 2]);
+            need |= top[b][e] > m[b][e] + kPfLazy;
+          }
+        if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float v = top[b][e];
+#pragma unroll
+              for (int k = 4; k < 32; k <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, k));
+              const float nm = fmaxf(m[b][e], v), a = fast_exp2(m[b][e] - nm);
+              m[b][e] = nm;
+              l[b][e] *= a;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) o[b][i][e] *= a, o[b][i][e + 2] *= a;
+              zc[b][e] *= a, zc[b][e + 2] *= a;
+            }
+        }
+        uint32_t pt[2][NB][2];  // P / 16 (below f16's largest) in f16, transposed: row r, tokens 2 j4, 2 j4 + 1 (+ 8)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const float m0 = m[b][0] + 4.f, m1 = m[b][1] + 4.f;
+#pragma unroll
+          for (int s2 = 0; s2 < 2; ++s2) {
+            float* xx = x[s2][b];
+            xx[0] = fast_exp2(xx[0] - m0), xx[1] = fast_exp2(xx[1] - m1);
+            xx[2] = fast_exp2(xx[2] - m0), xx[3] = fast_exp2(xx[3] - m1);
+            l[b][0] += xx[0] + xx[2];
+            l[b][1] += xx[1] + xx[3];
+            pt[s2][b][0] = movmatrix_t(pack2<__half>(xx[0], xx[1]));
+            pt[s2][b][1] = movmatrix_t(pack2<__half>(xx[2], xx[3]));
+          }
+        }
+        // ---- O^T += V^T P^T
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) {
+          const int q0 = (t0 + 16 * s2) / 2, left = nv - 16 * s2;  // the subtile's first pair; its tokens in use
+          uint32_t vs[2][NG], vz[2][NG];  // pairs j4 and 4 + j4: scales; ref: zero points
+          uint32_t zmin[2] = {0u, 0u};
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int q = q0 + 4 * e + j4;
+            if constexpr (FMT == HKV_FMT_FP16MIN) {
+              ld_row_u<NG>(reinterpret_cast<const uint32_t*>(meta + 512 * NG), q, vs[e]);
+              zmin[e] = r < NG ? reinterpret_cast<const uint32_t*>(meta + 768 * NG)[q * NG + r] : 0u;
+            } else {
+              float fa[NG], fb[NG];
+              ld_row<NG>(reinterpret_cast<const float*>(meta + 512 * NG), 2 * q, fa);
+              ld_row<NG>(reinterpret_cast<const float*>(meta + 512 * NG), 2 * q + 1, fb);
+              const uint8_t* zp = meta + 1152 * NG + 2 * q * NG;
+#pragma unroll
+              for (int g = 0; g < NG; ++g) {
+                vs[e][g] = pack2<__half>(fa[g], fb[g]);
+                vz[e][g] = (uint32_t)zp[g] | ((uint32_t)zp[NG + g] << 16);
+              }
+            }
+          }
+          if (left < 16) {  // unused tokens' metadata may be any bits: P = 0 has to meet 0
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int tk = 8 * e + 2 * j4;
+              const uint32_t keep = (tk < left ? 0x0000FFFFu : 0u) | (tk + 1 < left ? 0xFFFF0000u : 0u);
+              zmin[e] &= keep;
+#pragma unroll
+              for (int g = 0; g < NG; ++g) vs[e][g] &= keep;
+            }
+          }
+          if constexpr (FMT == HKV_FMT_FP16MIN) {
+            const uint32_t ab[4] = {zmin[0], 0u, zmin[1], 0u};
+#pragma unroll
+            for (int b = 0; b < NB; ++b) mma16816<__half>(zc[b], ab, pt[s2][b][0], pt[s2][b][1]);
+          }
+          uint32_t vw[2][4];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint4 c4 = *reinterpret_cast<const uint4*>(blk + HKV_V_CODES_OFF + v_chunk_off(q0 + 4 * e + j4, r));
+            vw[e][0] = c4.x, vw[e][1] = c4.y, vw[e][2] = c4.z, vw[e][3] = c4.w;
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int g = k / WPG;
+            uint32_t ha[4], hb[4];
+            if constexpr (FMT == HKV_FMT_REF) {  // 1024 + z and -64 - z in f16 are one addition to the bits
+              nib8_to_h2_z(vw[0][k], 0x64006400u + vz[0][g], 0xD400D400u + 16u * vz[0][g], ha);
+              nib8_to_h2_z(vw[1][k], 0x64006400u + vz[1][g], 0xD400D400u + 16u * vz[1][g], hb);
+            } else {
+              nib8_to_h2(vw[0][k], ha);
+              nib8_to_h2(vw[1][k], hb);
+            }
+            const uint32_t a0[4] = {ha[0], ha[1], hb[0], hb[1]}, a1[4] = {ha[2], ha[3], hb[2], hb[3]};
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              const uint32_t p0 = hmul2(pt[s2][b][0], vs[0][g]), p1 = hmul2(pt[s2][b][1], vs[1][g]);
+              mma16816<__half>(o[b][2 * k], a0, p0, p1);
+              mma16816<__half>(o[b][2 * k + 1], a1, p0, p1);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&raw_free[slot]);
+    }
+    n0 += pc.n;
+    // ---- the piece's partial: the warps' O, m, l joined through shared memory
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int k = 4; k < 32; k <<= 1) l[b][e] += __shfl_xor_sync(0xffffffffu, l[b][e], k);
+        if (r == 0) s_wm[warp][8 * b + 2 * j4 + e] = m[b][e], s_wl[warp][8 * b + 2 * j4 + e] = 16.f * l[b][e];
+        float z[NG];  // fp16min: row g of the mins' product is in lane 4 g + j4
+#pragma unroll
+        for (int g = 0; g < NG; ++g) z[g] = FMT == HKV_FMT_FP16MIN ? __shfl_sync(0xffffffffu, zc[b][e], 4 * g + j4) : 0.f;
+        float* dst = comb + (warp * 16 + 8 * b + 2 * j4 + e) * kRowsPitch + r;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float zz = z[16 * i / GROUP];
+          dst[16 * i] = 16.f * (o[b][i][e] + zz);
+          dst[16 * i + 8] = 16.f * (o[b][i][e + 2] + zz);
+        }
+      }
+    }
+    if (!bar_and(1, 256, ok)) break;
+    const int64_t id = (int64_t)(blockIdx.x + pc.unit) * ROWS;
+    for (int c = t; c < ROWS * 32; c += 256) {  // (row, 4 dims)
+      const int n = c >> 5, d = 4 * (c & 31);
+      float M = -1.0e30f, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) M = fmaxf(M, s_wm[w][n]);
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        const float x = fast_exp2(s_wm[w][n] - M);
+        const float4 v = *reinterpret_cast<const float4*>(comb + (w * 16 + n) * kRowsPitch + d);
+        L += x * s_wl[w][n];
+        a = make_float4(a.x + x * v.x, a.y + x * v.y, a.z + x * v.z, a.w + x * v.w);
+      }
+      if (n < rows) {
+        *reinterpret_cast<float4*>(p.part_o + (id + n) * HKV_D + d) = a;
+        if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (id + n) * 2) = make_float2(M, L);
+      }
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");  // the shared tables and areas are free again
+  }
+}
+
 // out[b][hq] from the partials of the row's pieces and of its own tokens:
 // sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i. Four warps per row, each a quarter
 // of the partials (lane = dims 4 lane .. 4 lane + 3), all (m, l) and then several
@@ -733,8 +1155,6 @@ __global__ void __launch_bounds__(128) shared_merge_kernel(const __grid_constant
   __shared__ ShGroup s_g[kShMaxGroups + 1];
   __shared__ float4 s_o[4][32];
   __shared__ float2 s_ml[4];
-  griddep_wait();
-  griddep_launch_dependents();
   if (threadIdx.x < 32) sh_schedule(p, s_g);
   __syncthreads();
   const int Hq = p.Hkv * p.G, row = blockIdx.x, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -763,7 +1183,7 @@ __global__ void __launch_bounds__(128) shared_merge_kernel(const __grid_constant
     c1 = cta(last);
   }
   // partial k: the own part (k = 0, when there is one), then the streams of the CTAs c0 .. c1
-  const int own = p.own_o ? 1 : 0, ns = sh_streams(p.N), parts = own + (c1 - c0 + 1) * ns;
+  const int own = p.own_o ? 1 : 0, ns = p.ns, parts = own + (c1 - c0 + 1) * ns;
   float M = -1.0e30f, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int k0 = w; k0 < parts; k0 += 128) {  // up to 32 partials of this warp: k0, k0 + 4, ...
