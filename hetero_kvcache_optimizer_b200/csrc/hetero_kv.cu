@@ -50,9 +50,7 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // (a chunked prefill's launches overlap their start with the previous one's
 // drain: 4.82 -> 4.68 ms for config 2's 896 chunk launches); the append kernel,
 // whose blocks would wait resident beside the decode kernel's, measured slower
-// with it (2.608 ms) and launches normally, as do the three launches of a
-// shared-prefix decode (72 KB to 222 KB of shared memory keep them from overlapping;
-// 8 samples of a 32K prompt: 59.6 us with it, 55.8 us without). HKV_PDL (bit mask: 1 decode,
+// with it (2.608 ms) and launches normally. HKV_PDL (bit mask: 1 decode,
 // 2 append, 4 quantise-pack, 8 norm + rotation and page operations; default 13)
 // overrides this for experiments.
 bool pdl_enabled(int which) {
@@ -246,7 +244,7 @@ hkv_status launch_decode_t(const hkv::DecodeParams& p, int smem, cudaStream_t st
                                     cudaFuncAttributeMaxDynamicSharedMemorySize, kDynSmemBudget);
   });
   if (attr_err != cudaSuccess) return cuda_fail(attr_err);
-  const cudaError_t e = launch_pdl(p.alone ? 0 : 1, hkv::decode_kernel<FMT, GROUP, DTy, STATS, APPEND>, dim3(p.sc.C),
+  const cudaError_t e = launch_pdl(1, hkv::decode_kernel<FMT, GROUP, DTy, STATS, APPEND>, dim3(p.sc.C),
                                    dim3(hkv::decode_threads(FMT, APPEND)), smem, st, p);
   if (e != cudaSuccess) return cuda_fail(e);
   return launch_status();
@@ -373,7 +371,7 @@ hkv_status run_decode(const void* q, int q_dtype, int64_t q_sb, int64_t q_sh, co
                       void* workspace, size_t workspace_bytes, void* out, int out_dtype, int64_t out_sb,
                       int64_t out_sh, float* out_o, float* out_ml, cudaStream_t st, float* tile_stats = nullptr,
                       int stat_tiles = 0, float* unit_ml = nullptr, const AppendArgs* app = nullptr,
-                      bool alone = false) {
+                      bool late = false) {
   hkv_status rc = check_decode_args(q, q_dtype, body, dense, B, Hq, Hkv, D);
   if (rc != HKV_OK) return rc;
   if (!(sm_scale > 0.f) || !std::isfinite(sm_scale)) return HKV_ERR_ARG;
@@ -419,7 +417,7 @@ hkv_status run_decode(const void* q, int q_dtype, int64_t q_sb, int64_t q_sh, co
   p.tile_stats = tile_stats;
   p.stat_tiles = stat_tiles;
   p.unit_ml = unit_ml;
-  p.alone = alone;
+  p.late = late;
   if (app) {
     p.k_new = app->k_new;
     p.v_new = app->v_new;
@@ -604,13 +602,15 @@ hkv_status launch_shared(const hkv::SharedParams& p, cudaStream_t st) {
   return launch_shared_n<FMT, 128>(p, st);
 }
 
-// Rows per product, CTAs and workspace of a shared-prefix decode:
-// own part's workspace | its (o, m, l) | the pieces' (o, m, l).
+// Rows per product, CTAs and workspace of a shared-prefix decode: own part's workspace
+// (its counters first) | its (o, m, l) | the pieces' (o, m, l). The prefix and the own
+// part run side by side, each on a share of the SMs in proportion to its work: one after
+// the other, each would pay its start and end (about 10 us) alone (PLACEHOLDER).
 struct SharedPlan {
-  int N, ns, C;
-  size_t own_ws, own_o, own_ml, part_o, part_ml, bytes;  // offsets
+  int N, ns, C, own_ctas;
+  size_t own_ws, own_o, own_ml, part_o, part_ml, bytes;  // sizes and offsets
 };
-hkv_status shared_plan(const hkv_int4_store* prefix, const int32_t* start, int P, const hkv_int4_store* body,
+hkv_status shared_plan(const hkv_int4_store* prefix, const int32_t* start, const int32_t* lens, int P, const hkv_int4_store* body,
                        const hkv_dense_kv* dense, int B, int Hq, int Hkv, int D, int ctas, SharedPlan* out) {
   const hkv_status rc = check_store(prefix);
   if (rc != HKV_OK) return rc;
@@ -628,27 +628,37 @@ hkv_status shared_plan(const hkv_int4_store* prefix, const int32_t* start, int P
   // largest group (its cost grows with its width); at most 16 rows run on shared_rows_kernel.
   pl.N = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
   pl.ns = pl.N == 16 ? 1 : hkv::sh_streams(pl.N);
-  pl.C = std::min(ctas > 0 ? ctas : device_sms(), 65535);
-  int64_t units = 0, steps = 0;
+  const int all = std::min(ctas > 0 ? ctas : device_sms(), 65535);
+  int64_t units = 0, steps = 0, hint_steps = 0;
   const int64_t cap = (int64_t)prefix->max_pages * (prefix->page_tokens / HKV_BLOCK_TOKENS);
   for (int g = 0; g < P; ++g) {
     const int64_t u = Hkv * (((int64_t)(start[g + 1] - start[g]) * G + pl.N - 1) / pl.N);
     units += u;
     steps += u * (cap + hkv::kShCharge);
+    const int len = lens ? lens[g] : prefix->len;
+    hint_steps += u * ((len > 0 ? std::min<int64_t>(cap, cdiv(len, HKV_BLOCK_TOKENS)) : lens ? 0 : cap) + hkv::kShCharge);
   }
-  if (steps >= (int64_t(1) << 31) || (units + pl.C) * pl.N >= (int64_t(1) << 30) || (int64_t)B * Hq >= (int64_t(1) << 28) ||
-      (int64_t)prefix->max_pages * prefix->page_tokens >= (int64_t(1) << 31))
-    return HKV_ERR_UNSUPPORTED;
-  size_t at = 0;
-  pl.own_ws = 0;
+  pl.C = all;
+  pl.own_ws = kCounterBytes;
+  pl.own_ctas = 0;
   if (body || dense) {
     Plan dp;
     const int dummy = 0;  // an address for the argument check: the queries are not read here
     hkv_status r = check_decode_args(&dummy, HKV_DT_F16, body, dense, B, Hq, Hkv, D);
-    if (r == HKV_OK) r = make_plan(B, Hq, Hkv, body, dense, ctas, &dp);
+    if (r == HKV_OK) r = make_plan(B, Hq, Hkv, body, dense, all, &dp);
     if (r != HKV_OK) return r;
-    at = (dp.ws_bytes + 255) & ~(size_t)255;
+    // nanoseconds of one SM: a tile of the prefix (measured, by the rows of its product),
+    // 128 bytes of the own part's schedule (about 36 GB/s per SM, piece starts charged in it)
+    const double mine = hint_steps * (pl.N == 16 ? 900. : pl.N == 32 ? 1200. : pl.N == 64 ? 2000. : 2400.), own = dp.sc.Btot * 3.6;
+    pl.C = std::max(1, std::min(all - 1, (int)std::lround(all * mine / (mine + own))));
+    pl.own_ctas = std::max(1, all - pl.C);
+    if ((r = make_plan(B, Hq, Hkv, body, dense, pl.own_ctas, &dp)) != HKV_OK) return r;
+    pl.own_ws = dp.ws_bytes;
   }
+  if (steps >= (int64_t(1) << 31) || (units + pl.C) * pl.N >= (int64_t(1) << 30) || (int64_t)B * Hq >= (int64_t(1) << 28) ||
+      (int64_t)prefix->max_pages * prefix->page_tokens >= (int64_t(1) << 31))
+    return HKV_ERR_UNSUPPORTED;
+  const size_t at = (pl.own_ws + 255) & ~(size_t)255;
   const bool own = body || dense;
   pl.own_o = at;
   pl.own_ml = pl.own_o + (own ? (size_t)B * Hq * HKV_D * 4 : 0);
@@ -1559,16 +1569,17 @@ hkv_status hkv_pages_compact(const hkv_int4_store* src, int32_t B, int32_t H, co
 }
 
 // --------------------------------------------------------------------------- shared prefix
-size_t hkv_decode_shared_workspace_bytes(const hkv_int4_store* prefix, const int32_t* group_start, int32_t n_groups,
+size_t hkv_decode_shared_workspace_bytes(const hkv_int4_store* prefix, const int32_t* group_start,
+                                         const int32_t* group_len, int32_t n_groups,
                                          const hkv_int4_store* body, const hkv_dense_kv* dense, int32_t B,
                                          int32_t Hq, int32_t Hkv, int32_t D, int32_t ctas) {
   SharedPlan pl;
-  return shared_plan(prefix, group_start, n_groups, body, dense, B, Hq, Hkv, D, ctas, &pl) == HKV_OK ? pl.bytes : 0;
+  return shared_plan(prefix, group_start, group_len, n_groups, body, dense, B, Hq, Hkv, D, ctas, &pl) == HKV_OK ? pl.bytes : 0;
 }
 
 hkv_status hkv_decode_shared(const void* q, int32_t q_dtype, int64_t q_stride_b, int64_t q_stride_h,
-                             const hkv_int4_store* prefix, const int32_t* group_start, int32_t n_groups,
-                             const hkv_int4_store* body, const hkv_dense_kv* dense, int32_t B, int32_t Hq,
+                             const hkv_int4_store* prefix, const int32_t* group_start,
+                             const int32_t* group_len, int32_t n_groups, const hkv_int4_store* body, const hkv_dense_kv* dense, int32_t B, int32_t Hq,
                              int32_t Hkv, int32_t D, float sm_scale, int32_t ctas, void* workspace,
                              size_t workspace_bytes, void* out, int32_t out_dtype, int64_t out_stride_b,
                              int64_t out_stride_h, hkv_stream_t stream) {
@@ -1576,7 +1587,7 @@ hkv_status hkv_decode_shared(const void* q, int32_t q_dtype, int64_t q_stride_b,
   if (out_dtype < HKV_DT_F16 || out_dtype > HKV_DT_F32) return HKV_ERR_ARG;
   if (!(sm_scale > 0.f) || !std::isfinite(sm_scale)) return HKV_ERR_ARG;
   SharedPlan pl;
-  hkv_status rc = shared_plan(prefix, group_start, n_groups, body, dense, B, Hq, Hkv, D, ctas, &pl);
+  hkv_status rc = shared_plan(prefix, group_start, group_len, n_groups, body, dense, B, Hq, Hkv, D, ctas, &pl);
   if (rc != HKV_OK) return rc;
   if (!workspace || workspace_bytes < pl.bytes || !aligned16(workspace)) return HKV_ERR_CAPACITY;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -1593,8 +1604,6 @@ hkv_status hkv_decode_shared(const void* q, int32_t q_dtype, int64_t q_stride_b,
   p.G = Hq / Hkv;
   p.C = pl.C;
   p.qscale = static_cast<float>(static_cast<double>(sm_scale) * 1.4426950408889634);
-  p.counters = reinterpret_cast<int*>(ws);
-  p.n_counters = own ? B * Hkv : 0;
   p.part_o = reinterpret_cast<float*>(ws + pl.part_o);
   p.part_ml = reinterpret_cast<float*>(ws + pl.part_ml);
   p.own_o = own ? reinterpret_cast<float*>(ws + pl.own_o) : nullptr;
@@ -1610,9 +1619,9 @@ hkv_status hkv_decode_shared(const void* q, int32_t q_dtype, int64_t q_stride_b,
   rc = prefix->format == HKV_FMT_REF ? launch_shared<HKV_FMT_REF>(p, S(stream)) : launch_shared<HKV_FMT_FP16MIN>(p, S(stream));
   if (rc != HKV_OK) return rc;
   if (own) {
-    rc = run_decode(q, q_dtype, q_stride_b, q_stride_h, body, dense, B, Hq, Hkv, D, sm_scale, ctas, ws, pl.own_o, nullptr,
+    rc = run_decode(q, q_dtype, q_stride_b, q_stride_h, body, dense, B, Hq, Hkv, D, sm_scale, pl.own_ctas, ws, pl.own_o, nullptr,
                     HKV_DT_F32, 0, 0, const_cast<float*>(p.own_o), const_cast<float*>(p.own_ml), S(stream), nullptr, 0,
-                    nullptr, nullptr, /*alone=*/true);
+                    nullptr, nullptr, /*late=*/true);
     if (rc != HKV_OK) return rc;
   }
   hkv::shared_merge_kernel<<<B * Hq, 128, 0, S(stream)>>>(p);

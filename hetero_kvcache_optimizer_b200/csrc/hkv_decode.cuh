@@ -118,7 +118,7 @@ struct DecodeParams {
   int out_dtype;
   int64_t out_sb, out_sh;
   float* out_o;    // [B][Hq][128] f32 (partial mode, when non-null)
-  int alone;       // launched without programmatic stream serialization
+  int late;        // runs beside the grid before it (whose data it does not read): it waits for that at its end
   float* out_ml;   // [B][Hq][2]
   // where the attention mass fell (optional, normalised mode): per INT4 body tile
   // k < stat_tiles of unit u, per consumer warp and head, (sum of the warp's
@@ -1195,7 +1195,7 @@ __global__ void __launch_bounds__(decode_threads(FMT, APPEND), 1)
   // trigger waits until this grid has waited for the one before it (thread 0,
   // consumer section): a grid then starts only once every grid two or more
   // launches back has completed, which is what lets it read its cache early.
-  const bool early = APPEND && p.early;
+  const bool early = APPEND && p.early, late = !APPEND && p.late;
   if (!early) griddep_launch_dependents();
   Piece first = first_piece_head(p, c, end);  // parameters only
   uint8_t* qbuf = reinterpret_cast<uint8_t*>(comb + kConsumerWarps * p.G * HKV_D + kConsumerWarps * 16);
@@ -1212,7 +1212,7 @@ __global__ void __launch_bounds__(decode_threads(FMT, APPEND), 1)
   // launches back, so it is read, and the ring filled, before the wait; every
   // role waits on its own before it reads the query or the new token (made by
   // the grid just before) and before its first global write.
-  if (!early) griddep_wait();
+  if (!early && !late) griddep_wait();
   const int2 first_st = first.valid ? seg_state<APPEND>(p, first.u, first.seg) : make_int2(0, -1);
   if (!early && warp < kConsumerWarps && p.q_async && first.valid) q_prefetch(p, first.u, qbuf);
   __syncthreads();
@@ -1636,6 +1636,7 @@ __global__ void __launch_bounds__(decode_threads(FMT, APPEND), 1)
     }
   }
   cp_async_wait_all();
+  if (late) griddep_wait();  // this grid's end then stands for both
 }
 
 // ---------------------------------------------------------------- log-sum-exp merge (cross-GPU partials)

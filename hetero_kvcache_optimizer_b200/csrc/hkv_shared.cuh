@@ -62,8 +62,6 @@ struct SharedParams {
   hkv_int4_store prefix;    // batch = groups
   int P, Hkv, G, C;         // groups, KV heads, query heads per KV head, CTAs
   float qscale;             // sm_scale * log2(e)
-  int* counters;            // own part's merge counters, zeroed here
-  int n_counters;
   float* part_o;            // [C + units][ns][N][128]
   float* part_ml;           // [C + units][ns][N][2]
   // merge
@@ -217,9 +215,12 @@ __device__ __forceinline__ bool elect_one() {
   return e != 0;
 }
 
-// Bounded wait for the phase that tile n's use of a buffer completes (the buffers
-// of `ring` tiles are used in turn; n counts the CTA's tiles).
-__device__ __forceinline__ bool sh_wait(uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity & 1u); }
+// Bounded wait for a phase. The loop is not inlined: with a copy at each of fifteen
+// places the roles' code missed the instruction cache (WAITPH).
+__device__ __noinline__ bool sh_wait_long(uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity); }
+__device__ __forceinline__ bool sh_wait(uint64_t* bar, uint32_t parity) {
+  return mbar_try_wait(bar, parity & 1u) || sh_wait_long(bar, parity & 1u);
+}
 
 // Dims of 16-byte chunk kc (8 values) of Q's and K's common order: value 2 c + e
 // is dim 32 (kc / 4) + 8 c + 2 (kc % 4) + e, the order in which nib8_to_h2 yields
@@ -404,7 +405,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "n"(kCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
-  for (int i = blockIdx.x * kThreads + t; i < p.n_counters; i += gridDim.x * kThreads) p.counters[i] = 0;
+  griddep_launch_dependents();  // the own part may start beside this grid
   if (warp == 1) sh_schedule(p, s_g);
   tc_fence_before();
   __syncthreads();
@@ -428,6 +429,9 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
       auto s_cm = s_cms[stream];
       const uint32_t tOs = tO + stream * N;
       const int j0 = NS == 2 ? (n0 ^ stream) & 1 : 0;  // the stream's first tile
+      // 16-byte chunk k of the thread's columns is at prow ^ 16 k (rows of 8 or 4 chunks, swizzled by the token)
+      const uint32_t prow = smem_u32(sP) + (col0 >> 6) * 16384 + tok * PR +
+                            (PR == 64 ? ((tok >> 1) & 3) << 4 : (((col0 & 63) >> 3) ^ (tok & 7)) << 4);
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const float2 qs2 = make_float2(p.qscale, p.qscale);
       // every group is through with the last piece's scores: its query rows make room
@@ -533,8 +537,6 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_free[buf]);
           }
-          uint8_t* prow = sP + buf * sh_p_bytes(N) + (c0 >> 6) * 16384 + tok * PR;
-          const int turn = PR == 64 ? (tok >> 1) & 3 : tok & 7;
 #pragma unroll
           for (int i = 0; i < SUB; i += 8) {
             uint32_t pk[4];
@@ -545,7 +547,8 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
               l[s0 + i + e] = z.x, l[s0 + i + e + 1] = z.y;
               pk[e >> 1] = h2u(__floats2half2_rn(y.x, y.y));
             }
-            *reinterpret_cast<uint4*>(prow + (((((c0 + i) & 63) >> 3) ^ turn) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            const uint32_t at16 = (prow + buf * sh_p_bytes(N)) ^ ((s0 + i) << 1);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at16), "r"(pk[0]), "r"(pk[1]), "r"(pk[2]), "r"(pk[3]) : "memory");
           }
         }
         if (!ok) break;
@@ -764,7 +767,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) shared_rows_kernel(const __gr
     }
     fence_barrier_init();
   }
-  for (int i = blockIdx.x * kRowsThreads + t; i < p.n_counters; i += gridDim.x * kRowsThreads) p.counters[i] = 0;
+  griddep_launch_dependents();  // the own part may start beside this grid
   if (warp == 0) sh_schedule(p, s_g);
   __syncthreads();
   const int total = s_g[p.P].step;

@@ -763,10 +763,12 @@ class SharedPrefix:
     """A prefix shared by groups of a batch's sequences: ``store`` holds one
     prefix per group (its batch is the number of groups), and the sequences
     [group_start[p], group_start[p + 1]) attend to prefix p; sequences outside
-    have none. ``group_start``: plain ints, fixed for the object's life (they
-    size the launches); the prefixes may still grow (``store.lengths``)."""
+    have none. ``group_start``: plain ints, fixed for the object's life. The
+    lengths on the device (``store.lengths``) are what counts and may change;
+    ``lengths``, plain ints, only divide the work (None: read from the device
+    here, which waits for it; ``set_lengths`` after they have changed much)."""
 
-    def __init__(self, store: Int4KVStore, group_start: Sequence[int]):
+    def __init__(self, store: Int4KVStore, group_start: Sequence[int], lengths: Optional[Sequence[int]] = None):
         starts = [int(x) for x in group_start]
         if len(starts) != store.batch + 1:
             raise ValueError(f"group_start needs {store.batch + 1} entries for {store.batch} prefixes")
@@ -775,6 +777,14 @@ class SharedPrefix:
         self.store = store
         self.group_start = starts
         self._starts = (ctypes.c_int32 * len(starts))(*starts)
+        self.set_lengths(store.lengths.tolist() if lengths is None else lengths)
+
+    def set_lengths(self, lengths: Sequence[int]) -> None:
+        """The prefixes' lengths that the launches' shares of the SMs go by."""
+        lens = [int(x) for x in lengths]
+        if len(lens) != self.store.batch:
+            raise ValueError(f"one length for each of the {self.store.batch} prefixes")
+        self._lens = (ctypes.c_int32 * len(lens))(*lens)
 
 
 def decode_shared(q: torch.Tensor, prefix: SharedPrefix, store: Optional[Int4KVStore] = None,
@@ -823,15 +833,18 @@ def decode_shared(q: torch.Tensor, prefix: SharedPrefix, store: Optional[Int4KVS
         pf = prefix.store.struct()
         st = store.struct(body_len) if store is not None else None
         ds = dense.struct(dense_len) if dense is not None else None
-        segs = (ctypes.byref(pf), prefix._starts, prefix.store.batch, ctypes.byref(st) if st is not None else None,
+        segs = (ctypes.byref(pf), prefix._starts, prefix._lens, prefix.store.batch, ctypes.byref(st) if st is not None else None,
                 ctypes.byref(ds) if ds is not None else None)
         lib = L.load()
         nbytes = lib.hkv_decode_shared_workspace_bytes(*segs, B, Hq, Hkv, D, ctas)
         if nbytes == 0:
             raise RuntimeError("hkv_decode_shared_workspace_bytes: unsupported decode configuration")
         # a captured call gets memory of its graph's own, so that graphs replayed side by side do not share it
-        ws = (torch.empty(nbytes, dtype=torch.uint8, device=q.device) if torch.cuda.is_current_stream_capturing()
-              else workspace(nbytes, q.device, kind="shared"))
+        if torch.cuda.is_current_stream_capturing():
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+            ws[:4 * B * Hkv].zero_()  # the own part's merge counters
+        else:
+            ws = workspace(nbytes, q.device, kind="shared")
         L.check(lib.hkv_decode_shared(
             q.data_ptr(), dtype_code(q.dtype), q.stride(0), q.stride(1), *segs, B, Hq, Hkv, D, float(sm_scale), ctas,
             ws.data_ptr(), ws.numel(), out.data_ptr(), dtype_code(out.dtype), out.stride(0), out.stride(1), raw_stream(q.device)),

@@ -518,17 +518,23 @@ hkv_status hkv_pages_compact(const hkv_int4_store* src, int32_t B, int32_t H, co
  * gives zeros. G = Hq/Hkv <= 8 with a body or a dense segment, else any.
  * Precision: as hkv_decode_attn for the own part; for the prefix K, V and P are
  * f16 (K and V dequantised in f16, a bf16 query rounded to it), sums and the
- * softmax statistics fp32. Three launches on `stream` (prefix, own part, merge).
- * Workspace: hkv_decode_shared_workspace_bytes, 16-byte aligned, no initial
- * contents; calls that overlap on the GPU must use different ones.
+ * softmax statistics fp32. Three launches on `stream`: prefix and own part side by
+ * side, each on a share of the `ctas` (<= 0: one per SM), then the merge. group_len
+ * (HOST array of the prefixes' lengths as far as known; NULL: prefix->len for each)
+ * and the len fields of body and dense size the shares; device lengths may exceed
+ * them. Both calls get the same arguments.
+ * Workspace: hkv_decode_shared_workspace_bytes, 16-byte aligned, its first 256 KiB
+ * zero before the first call, as for hkv_decode_attn; every completed call leaves
+ * them zero. Calls that overlap on the GPU must use different ones.
  * n_groups <= HKV_SHARED_MAX_GROUPS. */
 #define HKV_SHARED_MAX_GROUPS 512
-size_t hkv_decode_shared_workspace_bytes(const hkv_int4_store* prefix, const int32_t* group_start, int32_t n_groups,
+size_t hkv_decode_shared_workspace_bytes(const hkv_int4_store* prefix, const int32_t* group_start,
+                                         const int32_t* group_len, int32_t n_groups,
                                          const hkv_int4_store* body, const hkv_dense_kv* dense, int32_t B,
                                          int32_t Hq, int32_t Hkv, int32_t D, int32_t ctas);
 hkv_status hkv_decode_shared(const void* q, int32_t q_dtype, int64_t q_stride_b, int64_t q_stride_h,
-                             const hkv_int4_store* prefix, const int32_t* group_start, int32_t n_groups,
-                             const hkv_int4_store* body, const hkv_dense_kv* dense, int32_t B, int32_t Hq,
+                             const hkv_int4_store* prefix, const int32_t* group_start,
+                             const int32_t* group_len, int32_t n_groups, const hkv_int4_store* body, const hkv_dense_kv* dense, int32_t B, int32_t Hq,
                              int32_t Hkv, int32_t D, float sm_scale, int32_t ctas, void* workspace,
                              size_t workspace_bytes, void* out, int32_t out_dtype, int64_t out_stride_b,
                              int64_t out_stride_h, hkv_stream_t stream);
