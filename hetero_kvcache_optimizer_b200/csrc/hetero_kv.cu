@@ -649,7 +649,7 @@ hkv_status shared_plan(const hkv_int4_store* prefix, const int32_t* start, const
     if (r != HKV_OK) return r;
     // nanoseconds of one SM: a tile of the prefix (measured, by the rows of its product),
     // 128 bytes of the own part's schedule (about 36 GB/s per SM, piece starts charged in it)
-    const double mine = hint_steps * (pl.N == 16 ? 900. : pl.N == 32 ? 1200. : pl.N == 64 ? 2000. : 2400.), own = dp.sc.Btot * 3.6;
+    const double mine = hint_steps * (pl.N == 16 ? 900. : pl.N == 32 ? 1200. : pl.N == 64 ? 1750. : 1900.), own = dp.sc.Btot * 3.6;
     pl.C = std::max(1, std::min(all - 1, (int)std::lround(all * mine / (mine + own))));
     pl.own_ctas = std::max(1, all - pl.C);
     if ((r = make_plan(B, Hq, Hkv, body, dense, pl.own_ctas, &dp)) != HKV_OK) return r;

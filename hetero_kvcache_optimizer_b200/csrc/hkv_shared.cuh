@@ -295,7 +295,7 @@ __device__ __forceinline__ void sh_convert_v(const uint8_t* rb, uint8_t* sVt, in
   constexpr int NG = HKV_D / GROUP;
   const int i = t & 7, o0 = t >> 4, k2 = (t >> 3) & 1;
   const uint8_t* meta = rb + HKV_META_OFF;
-#pragma unroll
+#pragma unroll 1  // half the code: the roles share the instruction cache
   for (int rep = 0; rep < 2; ++rep) {
     const int o = o0 + 8 * rep;
     uint2 cw[4];
