@@ -15,15 +15,22 @@ and holds the CTA back: 107.4 us per layer against 95.4 us for the two launches
 (config 1); in fp16min the append has a warp of its own and the fused step is
 the faster one (2.485 against 2.569 ms per 32-layer step). All state (lengths, ring heads) lives on the device, so a whole
 multi-layer step can be captured once into a CUDA graph and replayed every token.
+
+Several sequences from one prompt: ``attach_prefix`` puts a shared INT4 prefix in
+front of every layer's cache (read once for all of its sequences), ``num_pages``
+keeps the bodies in page pools, ``fork`` continues sequences from others (samples,
+beams), and ``set_rotary`` lets a step take the queries and keys as the layer's
+projections give them (normed and rotated in one launch before the append).
 """
 from __future__ import annotations
 
-from typing import List, Optional
+from typing import List, Optional, Sequence, Union
 
 import torch
 
 from . import _lib as L
 from . import kvstore as kv
+from .memory.page_pool import PagePool
 
 
 class TieredKVDecoder:
@@ -32,7 +39,7 @@ class TieredKVDecoder:
                  fmt: str = "fp16min", group: int = 32, page_tokens: int = 256,
                  kv_dtype: torch.dtype = torch.float16, out_dtype: torch.dtype = torch.float32,
                  device="cuda", ctas: int = 0, fused_append: Optional[bool] = None,
-                 early: Optional[bool] = None):
+                 early: Optional[bool] = None, num_pages: Optional[int] = None):
         # the fused launch takes at most 8 query heads per KV head; more run as
         # the two launches (the attention split in groups of at most 8)
         fused_ok = q_heads // kv_heads <= 8
@@ -51,9 +58,14 @@ class TieredKVDecoder:
         self.dense: List[kv.DenseKV] = []
         for _ in range(num_layers):
             self.stores.append(kv.Int4KVStore(batch, kv_heads, body_capacity, fmt=fmt, group=group,
-                                              page_tokens=page_tokens, device=self.device))
+                                              page_tokens=page_tokens, num_pages=num_pages, device=self.device))
             self.dense.append(kv.DenseKV(batch, kv_heads, sink + recent, dtype=kv_dtype,
                                          device=self.device))
+        # with num_pages (pages per layer), the bodies' pages are owned by pools
+        self.pools: List[PagePool] = [PagePool(st) for st in self.stores] if num_pages is not None else []
+        self.prefixes: Optional[List[kv.SharedPrefix]] = None
+        self._rotary = None
+        self.positions: Optional[torch.Tensor] = None
         self.body_len = 0
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.host_graph: Optional[torch.cuda.CUDAGraph] = None
@@ -74,6 +86,9 @@ class TieredKVDecoder:
             d.k[:, :, self.sink:self.sink + nr] = k[:, :, S - nr:]
             d.v[:, :, self.sink:self.sink + nr] = v[:, :, S - nr:]
         nb = S - ns - nr
+        if self.pools:
+            st.set_lengths(0)
+            self.pools[layer].reserve(nb)
         if nb:
             kv.prefill(st, k[:, :, ns:ns + nb], v[:, :, ns:ns + nb])
         else:
@@ -90,6 +105,63 @@ class TieredKVDecoder:
             d.ring_head.zero_()
         self.body_len = body_len
 
+    # ------------------------------------------------------------------ several sequences from one prompt
+    def attach_prefix(self, prefixes: Optional[Sequence[kv.SharedPrefix]]) -> None:
+        """One shared prefix per layer (None: none), in front of what the layer's
+        cache holds; it stays attached until replaced. Steps then append and run
+        ``kvstore.decode_shared``."""
+        if prefixes is not None:
+            prefixes = list(prefixes)
+            if len(prefixes) != self.num_layers:
+                raise ValueError(f"attach_prefix needs {self.num_layers} prefixes, one per layer")
+            for p in prefixes:
+                if p.store.kv_heads != self.kv_heads or p.group_start[-1] > self.batch:
+                    raise ValueError("a prefix with other KV heads or more sequences than the batch")
+        self.prefixes = prefixes
+
+    def reserve(self, tokens: int) -> None:
+        """Pages for ``tokens`` more body tokens in every layer (``num_pages`` only)."""
+        if not self.pools:
+            raise RuntimeError("reserve needs a decoder with num_pages")
+        for pool in self.pools:
+            pool.reserve(tokens)
+
+    def fork(self, parents: Union[torch.Tensor, Sequence[int]]) -> None:
+        """Sequence b continues from what sequence ``parents[b]`` was, in every layer
+        and for all b at once (``num_pages`` only): body pages are shared or copied
+        (``PagePool.fork``), the sink and recent rows and their state are copied.
+        ``reserve`` before the next steps."""
+        if not self.pools:
+            raise RuntimeError("fork needs a decoder with num_pages")
+        par = self.pools[0]._per_sequence(parents, "parents")
+        if not isinstance(parents, torch.Tensor) and any(not 0 <= int(b) < self.batch for b in parents):
+            raise ValueError(f"parents must lie in [0, {self.batch})")
+        at = par.long()
+        for pool, d in zip(self.pools, self.dense):
+            for t in (d.k, d.v, d.lengths, d.ring_head):
+                t.copy_(t.index_select(0, at))
+            pool.fork(par)
+
+    def set_rotary(self, table: torch.Tensor, q_weights: Optional[Sequence[torch.Tensor]] = None,
+                   k_weights: Optional[Sequence[torch.Tensor]] = None, eps: float = 1e-6,
+                   adjacent: bool = False) -> None:
+        """Steps that are given positions take queries and keys before their norm
+        and rotation: ``kvstore.norm_rope`` with ``table`` and the layers' head-norm
+        weights (None: no norm) runs ahead of each layer's append."""
+        for w in (q_weights, k_weights):
+            if w is not None and len(w) != self.num_layers:
+                raise ValueError(f"set_rotary needs {self.num_layers} weights, one per layer")
+        self._rotary = (table, q_weights, k_weights, eps, adjacent)
+
+    def _ready(self, layer: int, q: torch.Tensor, k_new: torch.Tensor, positions: Optional[torch.Tensor]):
+        if positions is None:
+            return q, k_new
+        if self._rotary is None:
+            raise RuntimeError("positions without set_rotary")
+        table, qw, kw, eps, adjacent = self._rotary
+        return kv.norm_rope(q, k_new, positions, table, qw[layer] if qw is not None else None,
+                            kw[layer] if kw is not None else None, eps=eps, adjacent=adjacent)
+
     # ------------------------------------------------------------------ decode
     def step_layer(self, layer: int, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
                    out: Optional[torch.Tensor] = None, len_hint: Optional[int] = None,
@@ -99,6 +171,10 @@ class TieredKVDecoder:
         the fused launch may stream the cache while that one finishes."""
         st, d = self.stores[layer], self.dense[layer]
         hint = len_hint if len_hint is not None else self.body_len + 1
+        if self.prefixes is not None:
+            kv.append_kv(k_new, v_new, d, self.sink, st)
+            return kv.decode_shared(q, self.prefixes[layer], st, d, out_dtype=self.out_dtype, out=out, ctas=self.ctas,
+                                    body_len=hint, dense_len=self.sink + self.recent)
         if self.fused_append:
             return kv.decode_append(q, k_new, v_new, d, self.sink, st, out_dtype=self.out_dtype, out=out,
                                     ctas=self.ctas, body_len=hint, dense_len=self.sink + self.recent,
@@ -110,7 +186,7 @@ class TieredKVDecoder:
     @property
     def launches_per_layer(self) -> int:
         """Kernel launches of one layer's decode step."""
-        return 1 if self.fused_append else 2
+        return 4 if self.prefixes is not None else 1 if self.fused_append else 2
 
     @property
     def _early(self) -> bool:
@@ -119,13 +195,17 @@ class TieredKVDecoder:
         return self.num_layers >= 2 if self.early is None else (self.early and self.num_layers >= 2)
 
     def step(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
-             out: Optional[torch.Tensor] = None, len_hint: Optional[int] = None) -> torch.Tensor:
-        """q [L, B, Hq, 128], k_new/v_new [L, B, Hkv, 128] -> out [L, B, Hq, 128]."""
+             out: Optional[torch.Tensor] = None, len_hint: Optional[int] = None,
+             positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """q [L, B, Hq, 128], k_new/v_new [L, B, Hkv, 128] -> out [L, B, Hq, 128].
+        ``positions`` (int32 or int64 [B], after ``set_rotary``): q and k_new are
+        still to be normed and rotated."""
         if out is None:
             out = torch.empty(self.num_layers, self.batch, self.q_heads, 128, dtype=self.out_dtype,
                               device=self.device)
         for l in range(self.num_layers):
-            self.step_layer(l, q[l], k_new[l], v_new[l], out=out[l], len_hint=len_hint, early=self._early)
+            ql, kl = self._ready(l, q[l], k_new[l], positions)
+            self.step_layer(l, ql, kl, v_new[l], out=out[l], len_hint=len_hint, early=self._early)
         self.body_len += 1
         return out
 
@@ -137,10 +217,13 @@ class TieredKVDecoder:
                       ctas=self.ctas, body_len=hint, dense_len=self.sink + self.recent)
 
     # ------------------------------------------------------------------ CUDA graph
-    def capture(self, max_steps: int) -> None:
+    def capture(self, max_steps: int, positions: Optional[torch.Tensor] = None) -> None:
         """Capture one decode step over static input/output buffers. The split
         grid is sized for a body of ``body_len + max_steps`` tokens; device-side
-        lengths keep replays exact as the body grows."""
+        lengths keep replays exact as the body grows. ``positions`` (after
+        ``set_rotary``): the positions of the first step's tokens; the captured
+        step norms and rotates its queries and keys and moves ``self.positions``
+        on by one."""
         Lyr, B = self.num_layers, self.batch
         q = torch.zeros(Lyr, B, self.q_heads, 128, dtype=torch.bfloat16, device=self.device)
         kn = torch.zeros(Lyr, B, self.kv_heads, 128, dtype=self.kv_dtype, device=self.device)
@@ -148,6 +231,12 @@ class TieredKVDecoder:
         out = torch.empty(Lyr, B, self.q_heads, 128, dtype=self.out_dtype, device=self.device)
         hint = self.body_len + max_steps
         self._hint = hint
+        self.positions = None if positions is None else positions.to(device=self.device, dtype=torch.int32).clone()
+
+        def run():
+            for l in range(Lyr):
+                ql, kl = self._ready(l, q[l], kn[l], self.positions)
+                self.step_layer(l, ql, kl, vn[l], out=out[l], len_hint=hint, early=self._early)
         s = torch.cuda.Stream(device=self.device)
         s.wait_stream(torch.cuda.current_stream(self.device))
         g = torch.cuda.CUDAGraph()
@@ -155,13 +244,13 @@ class TieredKVDecoder:
         # throwaway copy of the state, then restore it
         snap = self._snapshot()
         with torch.cuda.stream(s):
-            for l in range(Lyr):
-                self.step_layer(l, q[l], kn[l], vn[l], out=out[l], len_hint=hint, early=self._early)
+            run()
         s.synchronize()
         self._restore(snap)
         with torch.cuda.graph(g, stream=s):
-            for l in range(Lyr):
-                self.step_layer(l, q[l], kn[l], vn[l], out=out[l], len_hint=hint, early=self._early)
+            run()
+            if self.positions is not None:
+                self.positions += 1
         torch.cuda.current_stream(self.device).wait_stream(s)
         self.graph = g
         self._static = (q, kn, vn, out)
@@ -180,6 +269,8 @@ class TieredKVDecoder:
         as few of them as the overlap allows (measured on the 32-layer config-1
         step: per-layer copies +138 us over the device-only step, this ~+55 us)."""
         assert self._static is not None, "capture() first"
+        if self.positions is not None:
+            raise RuntimeError("capture_host takes queries and keys that are rotated already: capture() without positions")
         q, kn, vn, out = self._static
         hq = torch.empty(q.shape, dtype=q.dtype, pin_memory=True)
         hk = torch.empty(kn.shape, dtype=kn.dtype, pin_memory=True)
