@@ -812,7 +812,8 @@ def decode_shared(q: torch.Tensor, prefix: SharedPrefix, store: Optional[Int4KVS
             raise ValueError(f"the own segments must hold {B} sequences of {Hkv} KV heads")
     if prefix.group_start[-1] > B:
         raise ValueError(f"group_start goes to {prefix.group_start[-1]}, beyond the batch of {B}")
-    if any(t.device != q.device for t in (prefix.store.pool, *((store.pool,) if store else ()), *((dense.k,) if dense else ()))):
+    if (prefix.store.pool.device != q.device or (store is not None and store.pool.device != q.device)
+            or (dense is not None and dense.k.device != q.device)):
         raise ValueError("q and the caches must be on one device")
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(D)
@@ -835,18 +836,28 @@ def decode_shared(q: torch.Tensor, prefix: SharedPrefix, store: Optional[Int4KVS
         ds = dense.struct(dense_len) if dense is not None else None
         segs = (ctypes.byref(pf), prefix._starts, prefix._lens, prefix.store.batch, ctypes.byref(st) if st is not None else None,
                 ctypes.byref(ds) if ds is not None else None)
-        lib = L.load()
-        nbytes = lib.hkv_decode_shared_workspace_bytes(*segs, B, Hq, Hkv, D, ctas)
-        if nbytes == 0:
-            raise RuntimeError("hkv_decode_shared_workspace_bytes: unsupported decode configuration")
-        # a captured call gets memory of its graph's own, so that graphs replayed side by side do not share it
+        lib, stream_h = L.load(), raw_stream(q.device)
+
+        def need() -> int:
+            n = lib.hkv_decode_shared_workspace_bytes(*segs, B, Hq, Hkv, D, ctas)
+            if n == 0:
+                raise RuntimeError("hkv_decode_shared_workspace_bytes: unsupported decode configuration")
+            return n
+
+        def run(ws: torch.Tensor) -> int:
+            return lib.hkv_decode_shared(
+                q.data_ptr(), dtype_code(q.dtype), q.stride(0), q.stride(1), *segs, B, Hq, Hkv, D, float(sm_scale), ctas,
+                ws.data_ptr(), ws.numel(), out.data_ptr(), dtype_code(out.dtype), out.stride(0), out.stride(1), stream_h)
+
         if torch.cuda.is_current_stream_capturing():
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+            # memory of the graph's own, so that graphs replayed side by side do not share it
+            ws = torch.empty(need(), dtype=torch.uint8, device=q.device)
             ws[:4 * B * Hkv].zero_()  # the own part's merge counters
+            rc = run(ws)
         else:
-            ws = workspace(nbytes, q.device, kind="shared")
-        L.check(lib.hkv_decode_shared(
-            q.data_ptr(), dtype_code(q.dtype), q.stride(0), q.stride(1), *segs, B, Hq, Hkv, D, float(sm_scale), ctas,
-            ws.data_ptr(), ws.numel(), out.data_ptr(), dtype_code(out.dtype), out.stride(0), out.stride(1), raw_stream(q.device)),
-            "hkv_decode_shared")
+            ws = _ws_cache.get((q.device.index, stream_h, "shared"))
+            rc = run(ws) if ws is not None else L.HKV_ERR_CAPACITY
+            if rc == L.HKV_ERR_CAPACITY:  # nothing was launched: the workspace is missing or too small
+                rc = run(workspace(need(), q.device, kind="shared"))
+        L.check(rc, "hkv_decode_shared")
     return out[:, :, None, :] if squeeze else out

@@ -42,17 +42,17 @@ class PagePool:
             raise ValueError(f"refs must be a contiguous int32 [{store.num_pages}] tensor on the store's device")
         self.refs = refs
         kv._require_cuda(store.pool, refs)
-        s = store.struct()
-        nbytes = L.load().hkv_pages_workspace_bytes(ctypes.byref(s), store.batch, store.kv_heads)
+        self._struct = store.struct()  # addresses and geometry, which stay for the store's life
+        self._ref = ctypes.byref(self._struct)
+        nbytes = L.load().hkv_pages_workspace_bytes(self._ref, store.batch, store.kv_heads)
         if nbytes == 0:
             raise ValueError("unsupported store geometry")
         self._ws = torch.empty(nbytes, dtype=torch.uint8, device=store.pool.device)
 
     def _call(self, name: str, *args) -> None:
         st = self.store
-        s = st.struct()
-        L.check(getattr(L.load(), name)(ctypes.byref(s), st.batch, st.kv_heads, *args, self._ws.data_ptr(),
-                                        self._ws.numel(), kv.raw_stream(self.refs.device)), name)
+        L.check(getattr(L.load(), name)(self._ref, st.batch, st.kv_heads, *args, self._ws.data_ptr(), self._ws.numel(),
+                                        kv.raw_stream(self.refs.device)), name)
 
     def _per_sequence(self, x: Union[torch.Tensor, Sequence[int]], name: str) -> torch.Tensor:
         if not isinstance(x, torch.Tensor):
@@ -101,9 +101,8 @@ class PagePool:
             raise ValueError("compact needs a pool of the same batch, heads, format and page size")
         if a.pool.device != b.pool.device:
             raise ValueError("both pools must be on one device")
-        s = b.struct()
         with kv.launch_on(self.refs.device, stream):
-            self._call("hkv_pages_compact", ctypes.byref(s), into.refs.data_ptr())
+            self._call("hkv_pages_compact", into._ref, into.refs.data_ptr())
         b.len_hint = a.len_hint
 
     def free_pages(self) -> int:
