@@ -604,8 +604,9 @@ hkv_status launch_shared(const hkv::SharedParams& p, cudaStream_t st) {
 
 // Rows per product, CTAs and workspace of a shared-prefix decode: own part's workspace
 // (its counters first) | its (o, m, l) | the pieces' (o, m, l). The prefix and the own
-// part run side by side, each on a share of the SMs in proportion to its work: one after
-// the other, each would pay its start and end (about 10 us) alone (PLACEHOLDER).
+// part run side by side, each on a share of the SMs in proportion to its work, since each
+// has a start and an end of about 10 us (one after the other: 4 samples of 1,000 tokens
+// 27.0 us, 8 samples of a 32K prompt 57.6; side by side 18.5 and 47.7).
 struct SharedPlan {
   int N, ns, C, own_ctas;
   size_t own_ws, own_o, own_ml, part_o, part_ml, bytes;  // sizes and offsets
@@ -625,7 +626,9 @@ hkv_status shared_plan(const hkv_int4_store* prefix, const int32_t* start, const
   }
   SharedPlan pl;
   // Rows of a unit that share its dequantised tiles: the narrowest product that holds the
-  // largest group (its cost grows with its width); at most 16 rows run on shared_rows_kernel.
+  // largest group. 65,536 tokens of 8 heads: 16 rows 35.3 us on shared_rows_kernel (40.1 on a
+  // 16-row shared_prefix_kernel; 32 rows there 58.2 against 44.3), 64 rows 55.3 (as 128: 74),
+  // 128 rows 74.1, 256 as two row tiles 127.8.
   pl.N = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
   pl.ns = pl.N == 16 ? 1 : hkv::sh_streams(pl.N);
   const int all = std::min(ctas > 0 ? ctas : device_sms(), 65535);
@@ -649,7 +652,7 @@ hkv_status shared_plan(const hkv_int4_store* prefix, const int32_t* start, const
     if (r != HKV_OK) return r;
     // nanoseconds of one SM: a tile of the prefix (measured, by the rows of its product),
     // 128 bytes of the own part's schedule (about 36 GB/s per SM, piece starts charged in it)
-    const double mine = hint_steps * (pl.N == 16 ? 900. : pl.N == 32 ? 1200. : pl.N == 64 ? 1750. : 1900.), own = dp.sc.Btot * 3.6;
+    const double mine = hint_steps * (pl.N == 16 ? 900. : pl.N == 32 ? 1050. : pl.N == 64 ? 1500. : 1900.), own = dp.sc.Btot * 3.6;
     pl.C = std::max(1, std::min(all - 1, (int)std::lround(all * mine / (mine + own))));
     pl.own_ctas = std::max(1, all - pl.C);
     if ((r = make_plan(B, Hq, Hkv, body, dense, pl.own_ctas, &dp)) != HKV_OK) return r;
@@ -1598,6 +1601,7 @@ hkv_status hkv_decode_shared(const void* q, int32_t q_dtype, int64_t q_stride_b,
   p.q_dtype = q_dtype;
   p.q_sb = q_stride_b;
   p.q_sh = q_stride_h;
+  p.q_pairs = reinterpret_cast<uintptr_t>(q) % 4 == 0 && q_stride_b % 2 == 0 && q_stride_h % 2 == 0;
   p.prefix = *prefix;
   p.P = n_groups;
   p.Hkv = Hkv;
@@ -1624,6 +1628,7 @@ hkv_status hkv_decode_shared(const void* q, int32_t q_dtype, int64_t q_stride_b,
                     nullptr, nullptr, /*late=*/true);
     if (rc != HKV_OK) return rc;
   }
+  // in plain stream order: a programmatic launch measured 3.5 us slower (18.1 -> 21.6 us for a small call)
   hkv::shared_merge_kernel<<<B * Hq, 128, 0, S(stream)>>>(p);
   return launch_status();
 }

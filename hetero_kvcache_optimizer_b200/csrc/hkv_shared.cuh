@@ -3,32 +3,47 @@
 //
 // A group of n sequences has one prefix; per KV head its n G query heads are the
 // columns of ONE product over the prefix's tokens, so the packed pages are read
-// and dequantised once per kShN rows instead of once per sequence:
+// and dequantised once per row tile of N = 32, 64 or 128 rows instead of once per
+// sequence (at most 16 rows: shared_rows_kernel below):
 //   S^T[token][row] = K Q^T,  P = 2^(S qscale - m),  O^T[dim][row] += V^T P
 // on tcgen05 with the tokens (then the dims) as the MMA's M = 128 and the rows as
-// its N = 16 .. 128: a decode batch has few rows, and this way they cost what they
-// are (with the rows as M, 8 rows would cost 128). The running max m and the sum
-// of P are fp32, m moves only when a score beats it by more than 2^8.
+// its N: a decode batch has few rows, and this way they cost what they are (with
+// the rows as M, 32 of them would cost 128, and the exponentials would sit in one
+// warp). The running max m and the sum of P are fp32; m moves only when a score
+// beats it by more than 2^8. K, V and P are rounded to f16, the type of their MMA:
+// K and V where they are dequantised (2^-11 relative, ref's f32 scale rounded as
+// well), P in (0, 2^8]; with key channels ten times as large as the rest that
+// leaves the output 5e-4 (fp16min) to 1.4e-3 (ref) off in the 2-norm, 3e-4 without.
 //
-// One persistent CTA per SM; every (group, KV head, row tile) unit's 128-token
+// A grid of p.C persistent CTAs; every (group, KV head, row tile) unit's 128-token
 // tiles, with a charge of kShCharge tiles per unit for a piece's start and end,
 // are cut into equal ranges, one per CTA (so a CTA has a few "pieces", runs of
-// tiles of one unit). Each piece leaves an un-normalised partial (O, m, l) at
-// index cta + unit (unique: each next piece raises one of the two), and
+// tiles of one unit). Each piece leaves un-normalised partials (O, m, l) at index
+// cta + unit (unique: each next piece raises one of the two), and
 // shared_merge_kernel joins a row's partials with the one of its own tokens.
 //
-// Roles (tile n of the CTA, in order, lives in the buffers n & 1):
-//   producer  one bulk copy per packed 128-token block into a ring of raw slots
+// Roles (tile n of the CTA uses the buffers n mod their number):
+//   softmax   thread = token, 16 or 32 of the tile's rows: S^T from TMEM, P as f16
+//             rows [token][row] (N-major B of O^T)
 //   K warps   thread = token: dequantised f16 K straight into TMEM (A of S^T, so
-//             K never crosses shared memory again)
+//             K does not cross shared memory again)
 //   V warps   dequantised V^T into shared memory (128-byte swizzle, A of O^T)
-//   two MMA warps  one issues S^T, up to two tiles ahead, the other O^T: one thread for
-//             both held S^T(n + 2) back until P(n) was written
-//   softmax   thread = token: kShCols columns each of S^T from TMEM, P as f16
-//             rows [token][row] (N-major B of O^T, 128-byte swizzle)
+//   producer  one bulk copy per packed 128-token block into a ring of raw slots
+//   two MMA warps  one issues S^T, up to two tiles ahead, the other O^T: one thread
+//             for both held S^T(n + 2) back until P(n) was written
 // Every wait is bounded (HKV_WAIT_NS); on expiry the device error word is set, the
 // CTA's roles leave, and copies and products in flight are waited for before TMEM
 // is freed.
+//
+// Measured (65,536 tokens, 8 KV heads, fp16min g32, all SMs, prefix and merge alone):
+// 32 rows 44.3 us, 64 rows 55.3, 128 rows 74.1, 256 rows 127.8 (538 TFLOP/s), of which
+// about 10 us are start and end. The steady state is 1.25 / 1.65 / 2.3 us per tile and
+// SM, bound by none of its resources alone: at 32 rows 4,700 warp instructions (1,180
+// issue slots of 2,350 cycles, K and V's unpacking 2,180 of them), 880 wavefronts of
+// loads and stores beside about 550 of the MMAs' and copies' in shared memory, 530
+// cycles of tcgen05; at 128 rows 9,500 instructions, 1,024 cycles of exponentials,
+// 1,080 of tcgen05. Steps that counted: K through TMEM, one elected thread for the
+// MMAs (57 -> 10 cycles to issue one), one polling warp a role, half-size V code.
 #pragma once
 #include "hkv_prefill.cuh"
 
@@ -44,8 +59,10 @@ constexpr int kShRawBytes = 21504;  // the largest block (ref, group 32)
 constexpr int sh_streams(int n) { return n <= 64 ? 2 : 1; }
 constexpr int sh_col_groups(int n) { return n <= 32 ? 1 : n <= 64 ? 2 : 4; }  // softmax groups that share a tile's rows
 constexpr int sh_softmax_groups(int n) { return sh_streams(n) * sh_col_groups(n); }
-constexpr int sh_halves(int n) { return n <= 32 ? 2 : 1; }  // sets of four K and of four V warps
-constexpr int sh_threads(int n) { return 32 * (4 * sh_softmax_groups(n) + 8 * sh_halves(n) + 3); }
+// Sets of four V warps, a tile each in turn (65,536 tokens, 8 heads: 44.2 us for 32 rows, one set
+// 47.0; 55.6 us for 64 rows, two sets 58.3: their registers are missed by the softmax).
+constexpr int sh_v_sets(int n) { return n <= 32 ? 2 : 1; }
+constexpr int sh_threads(int n) { return 32 * (4 * (sh_softmax_groups(n) + 1 + sh_v_sets(n)) + 3); }
 constexpr int sh_slots(int n) { return n <= 32 ? 4 : n <= 64 ? 3 : 2; }
 constexpr int sh_v_bufs(int n) { return n <= 64 ? 3 : 2; }
 constexpr int sh_p_row(int n) { return n <= 32 ? 64 : 128; }  // bytes of a token's row of P, swizzled as wide
@@ -59,6 +76,7 @@ struct SharedParams {
   const void* q;
   int q_dtype;
   int64_t q_sb, q_sh;
+  int q_pairs;              // pairs of query values are 4-byte aligned
   hkv_int4_store prefix;    // batch = groups
   int P, Hkv, G, C;         // groups, KV heads, query heads per KV head, CTAs
   float qscale;             // sm_scale * log2(e)
@@ -75,10 +93,8 @@ struct SharedParams {
 };
 
 // The schedule of a launch, from the device lengths: steps before group p.
-__device__ __forceinline__ int sh_tiles(const SharedParams& p, int g) {
-  const int cap = p.prefix.max_pages * (p.prefix.page_tokens / HKV_BLOCK_TOKENS);
-  const int len = max(0, p.prefix.lengths ? p.prefix.lengths[g] : p.prefix.len);
-  return min(cap, (len + HKV_BLOCK_TOKENS - 1) / HKV_BLOCK_TOKENS);
+__device__ __forceinline__ int sh_len(const SharedParams& p, int g) {
+  return min(p.prefix.max_pages * p.prefix.page_tokens, max(0, p.prefix.lengths ? p.prefix.lengths[g] : p.prefix.len));
 }
 __device__ __forceinline__ int sh_row_tiles(const SharedParams& p, int g) {
   return ((p.start[g + 1] - p.start[g]) * p.G + p.N - 1) / p.N;
@@ -87,6 +103,7 @@ __device__ __forceinline__ int sh_units(const SharedParams& p, int g) { return p
 
 struct ShGroup {
   int step, unit;  // steps and units before the group
+  int len;         // its prefix's length
 };
 // Fills s_g[0 .. P] (one warp); s_g[P].step is the launch's step count.
 __device__ __forceinline__ void sh_schedule(const SharedParams& p, ShGroup* s_g) {
@@ -94,9 +111,10 @@ __device__ __forceinline__ void sh_schedule(const SharedParams& p, ShGroup* s_g)
   int step = 0, unit = 0;
   for (int g0 = 0; g0 <= p.P; g0 += 32) {
     const int g = g0 + lane;
-    int st = 0, un = 0;
+    int st = 0, un = 0, len = 0;
     if (g < p.P) {
-      const int tiles = sh_tiles(p, g);
+      len = sh_len(p, g);
+      const int tiles = (len + HKV_BLOCK_TOKENS - 1) / HKV_BLOCK_TOKENS;
       un = sh_units(p, g);
       st = tiles > 0 ? un * (tiles + kShCharge) : 0;
     }
@@ -106,7 +124,7 @@ __device__ __forceinline__ void sh_schedule(const SharedParams& p, ShGroup* s_g)
       const int a = __shfl_up_sync(0xffffffffu, si, k), b = __shfl_up_sync(0xffffffffu, ui, k);
       if (lane >= k) si += a, ui += b;
     }
-    if (g <= p.P) s_g[g] = ShGroup{step + si - st, unit + ui - un};
+    if (g <= p.P) s_g[g] = ShGroup{step + si - st, unit + ui - un, len};
     step += __shfl_sync(0xffffffffu, si, 31);
     unit += __shfl_sync(0xffffffffu, ui, 31);
   }
@@ -215,11 +233,18 @@ __device__ __forceinline__ bool elect_one() {
   return e != 0;
 }
 
-// Bounded wait for a phase. The loop is not inlined: with a copy at each of fifteen
-// places the roles' code missed the instruction cache (WAITPH).
+// Bounded wait for a phase. The loop is out of line: with a copy at each of fifteen
+// places the roles' code missed the instruction cache (64 rows: 64.6 -> 56.5 us).
 __device__ __noinline__ bool sh_wait_long(uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity); }
 __device__ __forceinline__ bool sh_wait(uint64_t* bar, uint32_t parity) {
   return mbar_try_wait(bar, parity & 1u) || sh_wait_long(bar, parity & 1u);
+}
+
+// Query values i and i + 1 as two f16 (bf16 rounded to them).
+__device__ __forceinline__ uint32_t sh_q2(const SharedParams& p, int64_t i) {
+  if (!p.q_pairs) return h2u(__floats2half2_rn(load_any(p.q, p.q_dtype, i), load_any(p.q, p.q_dtype, i + 1)));
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p.q) + i);
+  return p.q_dtype == HKV_DT_F16 ? w : h2u(__float22half2_rn(__bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w))));
 }
 
 // Dims of 16-byte chunk kc (8 values) of Q's and K's common order: value 2 c + e
@@ -358,9 +383,9 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
   constexpr int NS = sh_streams(N), CG = sh_col_groups(N);
   constexpr int SG = NS * CG;                // softmax groups of 128 threads
   constexpr int COLS = N / CG;               // columns of a softmax thread
-  constexpr int SUB = 16;                    // taken at a time
+  constexpr int SUB = 16;  // taken at a time
   constexpr int VB = sh_v_bufs(N), PR = sh_p_row(N);
-  constexpr int KH = sh_halves(N);           // sets of four K and of four V warps (a tile each in turn)
+  constexpr int VS = sh_v_sets(N);
   constexpr int R = sh_slots(N);
   constexpr int kThreads = sh_threads(N);
   constexpr uint32_t kBlock = block_bytes(FMT, GROUP);
@@ -436,7 +461,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
       const float2 qs2 = make_float2(p.qscale, p.qscale);
       // every group is through with the last piece's scores: its query rows make room
       // for this one's, in K's dim order (a group that gave up says so here)
-      if (!bar_and(9, 128 * SG, ok)) break;
+      if (!bar_and(8, 128 * SG, ok)) break;
       for (int c = t; c < N * 16; c += 128 * SG) {
         const int n = c >> 4, kc = c & 15;
         uint32_t o[4] = {0u, 0u, 0u, 0u};
@@ -444,10 +469,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
           const int r = pc.rt * N + n, sq = r / p.G;
           const int64_t base = (int64_t)(p.start[pc.g] + sq) * p.q_sb + (int64_t)(pc.h * p.G + r - sq * p.G) * p.q_sh;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int64_t i = base + sh_dim(kc, e);
-            o[e] = h2u(__floats2half2_rn(load_any(p.q, p.q_dtype, i), load_any(p.q, p.q_dtype, i + 1)));
-          }
+          for (int e = 0; e < 4; ++e) o[e] = sh_q2(p, base + sh_dim(kc, e));
         }
         *reinterpret_cast<uint4*>(sQ + (kc >> 3) * (N * 128) + n * 128 + (((kc & 7) ^ (n & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
       }
@@ -593,11 +615,10 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
             *reinterpret_cast<float2*>(p.part_ml + (id + c) * 2) = make_float2(s_m[c], (s_cm[0][c] + s_cm[1][c]) + (s_cm[2][c] + s_cm[3][c]));
         }
       }
-    } else if (warp < 4 * SG + 4 * KH) {
+    } else if (warp < 4 * (SG + 1)) {
       // ---------------- K: thread = token = TMEM lane ----------------
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-      const int set = (warp - 4 * SG) >> 2;  // takes the tiles of its parity (KH == 2)
-      for (int j = KH == 2 ? (n0 ^ set) & 1 : 0; j < pc.n; j += KH) {
+      for (int j = 0; j < pc.n; ++j) {
         const uint32_t n = n0 + j, buf = n & 1, slot = n % R;
         bool good = true;
         if ((warp & 3) == 0) {
@@ -605,7 +626,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
           if (n >= 2) good = sh_wait(&s_full[buf], (n >> 1) - 1) && good;  // S(n - 2) has read K[buf]
           __syncwarp();
         }
-        ok = bar_and(5 + set, 128, good);
+        ok = bar_and(5, 128, good);
         if (!ok) break;
         tc_fence_after();
         sh_convert_k<FMT, GROUP>(raw + slot * kShRawBytes, tmem + 64 * buf + lanes, t & 127, (t & 127) < s_valid[n & 15]);
@@ -616,10 +637,10 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
           mbar_arrive(&raw_free[slot]);
         }
       }
-    } else if (warp < 4 * SG + 8 * KH) {
+    } else if (warp < 4 * (SG + 1 + VS)) {
       // ---------------- V ----------------
-      const int set = (warp - 4 * SG - 4 * KH) >> 2, vt = t & 127;
-      for (int j = KH == 2 ? (n0 ^ set) & 1 : 0; j < pc.n; j += KH) {
+      const int set = (warp - 4 * (SG + 1)) >> 2, vt = t & 127;
+      for (int j = VS == 2 ? (n0 ^ set) & 1 : 0; j < pc.n; j += VS) {
         const uint32_t n = n0 + j, vb = n % VB, slot = n % R;
         bool good = true;
         if ((warp & 3) == 0) {
@@ -627,7 +648,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
           if (n >= VB) good = sh_wait(&v_free[vb], n / VB - 1) && good;  // O(n - VB) has read Vt[vb]
           __syncwarp();
         }
-        ok = bar_and(7 + set, 128, good);
+        ok = bar_and(6 + set, 128, good);
         if (!ok) break;
         sh_convert_v<FMT, GROUP>(raw + slot * kShRawBytes, sV + vb * kPfTileBytes, vt, s_valid[n & 15]);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -637,10 +658,10 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
           mbar_arrive(&raw_free[slot]);
         }
       }
-    } else if (warp == 4 * SG + 8 * KH) {
+    } else if (warp == 4 * (SG + 1 + VS)) {
       // ---------------- producer ----------------
       const int u = pc.g * p.Hkv + pc.h;
-      const int len = max(0, p.prefix.lengths ? p.prefix.lengths[pc.g] : p.prefix.len);
+      const int len = s_g[pc.g].len;
       int64_t ids = -1;
       for (int j = 0; j < pc.n; ++j) {
         const uint32_t n = n0 + j, slot = n % R;
@@ -668,7 +689,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
       }
       if (!ok)  // copies in flight land before the CTA ends
         for (uint32_t n = issued > R ? issued - R : 0; n < issued; ++n) sh_wait(&raw_full[n % R], n / R);
-    } else if (warp == 4 * SG + 8 * KH + 1) {
+    } else if (warp == 4 * (SG + 1 + VS) + 1) {
       // ---------------- S^T(n) = K(n) Q^T, up to two tiles ahead of the softmax ----------------
       if (elect_one()) {
         const uint32_t q0 = smem_u32(sQ);
@@ -783,7 +804,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) shared_rows_kernel(const __gr
     while (ok) {
       const ShPiece pc = sh_next(p, s_g, at, end);
       if (pc.n == 0) break;
-      const int u = pc.g * p.Hkv + pc.h, len = max(0, p.prefix.lengths ? p.prefix.lengths[pc.g] : p.prefix.len);
+      const int u = pc.g * p.Hkv + pc.h, len = s_g[pc.g].len;
       int64_t ids = -1;
       int i = 0;
       for (int j = (n0 ^ par) & 1; j < pc.n; j += 2, ++i) {
@@ -831,21 +852,21 @@ __global__ void __launch_bounds__(kRowsThreads, 1) shared_rows_kernel(const __gr
     // (+ {8, 9}) / 16, + {16, 17}, (+ {24, 25}) / 16; sums of 32 dims beside them
     {
       const int c = warp, b = c >> 2, w = c & 3, n = 8 * b + r;
-      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      uint32_t v[4] = {0u, 0u, 0u, 0u};
       if (n < rows) {
         const int row = pc.rt * ROWS + n, sq = row / p.G;
         const int64_t base = (int64_t)(p.start[pc.g] + sq) * p.q_sb + (int64_t)(pc.h * p.G + row - sq * p.G) * p.q_sh + 32 * w + 2 * j4;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = load_any(p.q, p.q_dtype, base + 8 * (e >> 1) + (e & 1));
+        for (int e = 0; e < 4; ++e) v[e] = sh_q2(p, base + 8 * e);
       }
       float ps = 0.f, pb = 0.f;
       uint32_t f[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float d = e & 1 ? 0.0625f : 1.f, up = e & 1 ? 16.f : 1.f;
-        const __half a = __float2half_rn(to_f32(__float2half_rn(v[2 * e])) * d), q2 = __float2half_rn(to_f32(__float2half_rn(v[2 * e + 1])) * d);
-        f[e] = (uint32_t)__half_as_ushort(a) | ((uint32_t)__half_as_ushort(q2) << 16);
-        const float sum = __half2float(a) + __half2float(q2);
+        const float up = e & 1 ? 16.f : 1.f;
+        f[e] = e & 1 ? hmul2(v[e], 0x2C002C00u) : v[e];  // / 16
+        const float2 v2 = __half22float2(u2h(f[e]));
+        const float sum = v2.x + v2.y;
         pb += sum;
         ps += up * sum;
       }
