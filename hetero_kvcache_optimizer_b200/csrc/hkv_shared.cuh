@@ -23,7 +23,7 @@
 // shared_merge_kernel joins a row's partials with the one of its own tokens.
 //
 // Roles (tile n of the CTA uses the buffers n mod their number):
-//   softmax   thread = token, 16 or 32 of the tile's rows: S^T from TMEM, P as f16
+//   softmax   thread = token, 32 of the tile's rows, 16 at a time: S^T from TMEM, P as f16
 //             rows [token][row] (N-major B of O^T)
 //   K warps   thread = token: dequantised f16 K straight into TMEM (A of S^T, so
 //             K does not cross shared memory again)
@@ -188,30 +188,22 @@ __device__ __forceinline__ void sh_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
       "r"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
-template <int N>
-__device__ __forceinline__ void sh_ld(uint32_t addr, float (&v)[N]) {  // N columns of this thread's lane
-  static_assert(N == 16 || N == 32, "");
-  if constexpr (N == 32) {
-    tm_ld32(addr, v);
-  } else {
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(addr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+__device__ __forceinline__ void sh_ld(uint32_t addr, float (&v)[16]) {  // 16 columns of this thread's lane
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-  }
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
-template <int N>
-__device__ __forceinline__ void sh_st(uint32_t addr, const float (&v)[N]) {
-  uint32_t r[N];
+__device__ __forceinline__ void sh_st(uint32_t addr, const float (&v)[16]) {
+  uint32_t r[16];
 #pragma unroll
-  for (int i = 0; i < N; ++i) r[i] = __float_as_uint(v[i]);
-  if constexpr (N == 32) tm_st32u(addr, r);
-  else tm_st16u(addr, r);
+  for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(v[i]);
+  tm_st16u(addr, r);
 }
 __device__ __forceinline__ bool bar_or(int id, int n, bool v) {
   uint32_t r;
@@ -501,7 +493,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
           const uint32_t ts = tS + buf * N + c0 + lanes;
           float x[SUB];  // S qscale - m
           auto scores = [&]() {
-            sh_ld<SUB>(ts, x);
+            sh_ld(ts, x);
 #pragma unroll
             for (int i = 0; i < SUB; i += 4) {
               const float4 m = *reinterpret_cast<const float4*>(&s_m[c0 + i]);
@@ -515,7 +507,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
 #pragma unroll
           for (int i = 1; i + 1 < SUB; i += 2) mx = fmax3(mx, x[i], x[i + 1]);
           if (bar_or(1 + sg, 128, see && mx > kPfLazy)) {  // a column's max moves
-            sh_ld<SUB>(ts, x);
+            sh_ld(ts, x);
             float mine = -INFINITY;  // the warp's max of column c0 + lane
 #pragma unroll
             for (int i = 0; i < SUB; ++i) {
@@ -540,10 +532,10 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
             if (!ok) break;
             if (j > j0) {
               tc_fence_after();
-              sh_ld<SUB>(tOs + c0 + lanes, x);
+              sh_ld(tOs + c0 + lanes, x);
 #pragma unroll
               for (int i = 0; i < SUB; ++i) x[i] *= s_f[c0 + i];
-              sh_st<SUB>(tOs + c0 + lanes, x);
+              sh_st(tOs + c0 + lanes, x);
               tm_wait_st();
             }
 #pragma unroll
@@ -591,13 +583,13 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
 #pragma unroll
           for (int s0 = 0; s0 < COLS; s0 += SUB) {
             float o[SUB];
-            sh_ld<SUB>(tOs + col0 + s0 + lanes, o);
+            sh_ld(tOs + col0 + s0 + lanes, o);
 #pragma unroll
             for (int i = 0; i < SUB; ++i)
               if (any && col0 + s0 + i < rows) p.part_o[(id + col0 + s0 + i) * HKV_D + tok] = o[i];
             // sums over the warp's tokens: lane ends with column lane % SUB
 #pragma unroll
-            for (int i = 0; i < SUB; ++i) o[i] = l[s0 + i] + (SUB == 16 ? __shfl_xor_sync(0xffffffffu, l[s0 + i], 16) : 0.f);
+            for (int i = 0; i < SUB; ++i) o[i] = l[s0 + i] + __shfl_xor_sync(0xffffffffu, l[s0 + i], 16);
 #pragma unroll
             for (int k = SUB / 2; k >= 1; k >>= 1) {
               const bool up = lane & k;

@@ -64,6 +64,7 @@ class TieredKVDecoder:
         # with num_pages (pages per layer), the bodies' pages are owned by pools
         self.pools: List[PagePool] = [PagePool(st) for st in self.stores] if num_pages is not None else []
         self.prefixes: Optional[List[kv.SharedPrefix]] = None
+        self._nobody: Optional[torch.Tensor] = None
         self._rotary = None
         self.positions: Optional[torch.Tensor] = None
         self.body_len = 0
@@ -86,8 +87,8 @@ class TieredKVDecoder:
             d.k[:, :, self.sink:self.sink + nr] = k[:, :, S - nr:]
             d.v[:, :, self.sink:self.sink + nr] = v[:, :, S - nr:]
         nb = S - ns - nr
-        if self.pools:
-            st.set_lengths(0)
+        if self.pools:  # pages that others share as well must not be written
+            self._empty_pool(layer)
             self.pools[layer].reserve(nb)
         if nb:
             kv.prefill(st, k[:, :, ns:ns + nb], v[:, :, ns:ns + nb])
@@ -98,18 +99,27 @@ class TieredKVDecoder:
         self.body_len = nb
 
     def set_state(self, body_len: int) -> None:
-        """Declare that every layer holds ``body_len`` INT4 tokens and a full sink + ring."""
-        for st, d in zip(self.stores, self.dense):
+        """Declare that every layer holds ``body_len`` INT4 tokens and a full sink + ring
+        (with ``num_pages``, on pages of each sequence's own)."""
+        for l, (st, d) in enumerate(zip(self.stores, self.dense)):
+            if self.pools:
+                self._empty_pool(l)
+                self.pools[l].reserve(body_len)
             st.set_lengths(body_len)
             d.set_lengths(self.sink + self.recent)
             d.ring_head.zero_()
         self.body_len = body_len
 
     # ------------------------------------------------------------------ several sequences from one prompt
+    def _empty_pool(self, layer: int) -> None:
+        if self._nobody is None:
+            self._nobody = torch.full((self.batch,), -1, dtype=torch.int32, device=self.device)
+        self.pools[layer].fork(self._nobody)
+
     def attach_prefix(self, prefixes: Optional[Sequence[kv.SharedPrefix]]) -> None:
         """One shared prefix per layer (None: none), in front of what the layer's
         cache holds; it stays attached until replaced. Steps then append and run
-        ``kvstore.decode_shared``."""
+        ``kvstore.decode_shared``. A captured step is dropped: ``capture`` again."""
         if prefixes is not None:
             prefixes = list(prefixes)
             if len(prefixes) != self.num_layers:
@@ -118,6 +128,7 @@ class TieredKVDecoder:
                 if p.store.kv_heads != self.kv_heads or p.group_start[-1] > self.batch:
                     raise ValueError("a prefix with other KV heads or more sequences than the batch")
         self.prefixes = prefixes
+        self.graph = self.host_graph = self._host = None
 
     def reserve(self, tokens: int) -> None:
         """Pages for ``tokens`` more body tokens in every layer (``num_pages`` only)."""
@@ -129,17 +140,20 @@ class TieredKVDecoder:
     def fork(self, parents: Union[torch.Tensor, Sequence[int]]) -> None:
         """Sequence b continues from what sequence ``parents[b]`` was, in every layer
         and for all b at once (``num_pages`` only): body pages are shared or copied
-        (``PagePool.fork``), the sink and recent rows and their state are copied.
-        ``reserve`` before the next steps."""
+        (``PagePool.fork``), the sink and recent rows and their state are copied; -1
+        empties a sequence. ``reserve`` before the next steps."""
         if not self.pools:
             raise RuntimeError("fork needs a decoder with num_pages")
         par = self.pools[0]._per_sequence(parents, "parents")
-        if not isinstance(parents, torch.Tensor) and any(not 0 <= int(b) < self.batch for b in parents):
-            raise ValueError(f"parents must lie in [0, {self.batch})")
-        at = par.long()
+        if not isinstance(parents, torch.Tensor) and any(not -1 <= int(b) < self.batch for b in parents):
+            raise ValueError(f"parents must be -1 or lie in [0, {self.batch})")
+        at = par.long().clamp(0, self.batch - 1)  # values on the device are not known here
+        gone = par != at
         for pool, d in zip(self.pools, self.dense):
             for t in (d.k, d.v, d.lengths, d.ring_head):
                 t.copy_(t.index_select(0, at))
+            d.lengths.masked_fill_(gone, 0)
+            d.ring_head.masked_fill_(gone, 0)
             pool.fork(par)
 
     def set_rotary(self, table: torch.Tensor, q_weights: Optional[Sequence[torch.Tensor]] = None,
@@ -194,6 +208,10 @@ class TieredKVDecoder:
         # before a layer's is always another layer's (which never writes its cache)
         return self.num_layers >= 2 if self.early is None else (self.early and self.num_layers >= 2)
 
+    def _early_layer(self, layer: int) -> bool:
+        # a call on layer 0's pool may be the launch just before a step
+        return self._early and not (layer == 0 and self.pools)
+
     def step(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
              out: Optional[torch.Tensor] = None, len_hint: Optional[int] = None,
              positions: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -205,7 +223,7 @@ class TieredKVDecoder:
                               device=self.device)
         for l in range(self.num_layers):
             ql, kl = self._ready(l, q[l], k_new[l], positions)
-            self.step_layer(l, ql, kl, v_new[l], out=out[l], len_hint=len_hint, early=self._early)
+            self.step_layer(l, ql, kl, v_new[l], out=out[l], len_hint=len_hint, early=self._early_layer(l))
         self.body_len += 1
         return out
 
@@ -213,6 +231,10 @@ class TieredKVDecoder:
         """Attention of every layer without appending (cache unchanged)."""
         hint = len_hint if len_hint is not None else self.body_len
         for l in range(self.num_layers):
+            if self.prefixes is not None:
+                kv.decode_shared(q[l], self.prefixes[l], self.stores[l], self.dense[l], out_dtype=self.out_dtype, out=out[l],
+                                 ctas=self.ctas, body_len=hint, dense_len=self.sink + self.recent)
+                continue
             kv.decode(q[l], self.stores[l], self.dense[l], out_dtype=self.out_dtype, out=out[l],
                       ctas=self.ctas, body_len=hint, dense_len=self.sink + self.recent)
 
@@ -236,7 +258,7 @@ class TieredKVDecoder:
         def run():
             for l in range(Lyr):
                 ql, kl = self._ready(l, q[l], kn[l], self.positions)
-                self.step_layer(l, ql, kl, vn[l], out=out[l], len_hint=hint, early=self._early)
+                self.step_layer(l, ql, kl, vn[l], out=out[l], len_hint=hint, early=self._early_layer(l))
         s = torch.cuda.Stream(device=self.device)
         s.wait_stream(torch.cuda.current_stream(self.device))
         g = torch.cuda.CUDAGraph()
@@ -292,7 +314,7 @@ class TieredKVDecoder:
         snap = self._snapshot()
         with torch.cuda.stream(s):
             for l in range(Lyr):
-                self.step_layer(l, q[l], kn[l], vn[l], out=out[l], len_hint=hint, early=self._early)
+                self.step_layer(l, q[l], kn[l], vn[l], out=out[l], len_hint=hint, early=self._early_layer(l))
         s.synchronize()
         self._restore(snap)
         g = torch.cuda.CUDAGraph()
@@ -310,7 +332,7 @@ class TieredKVDecoder:
                 for i, (a, _) in enumerate(in_chunks):
                     if l == a:  # the first layer that reads input copy i
                         s.wait_event(ev_in[i])
-                self.step_layer(l, q[l], kn[l], vn[l], out=out[l], len_hint=hint, early=self._early)
+                self.step_layer(l, q[l], kn[l], vn[l], out=out[l], len_hint=hint, early=self._early_layer(l))
                 a, b = chunks[ci]
                 if l == b - 1:
                     ev_out[ci].record(s)
@@ -349,6 +371,8 @@ class TieredKVDecoder:
         return self._static
 
     def replay(self) -> None:
+        if self.graph is None:
+            raise RuntimeError("replay needs a captured step (capture; attach_prefix drops it)")
         self.graph.replay()
         self.body_len += 1
 
@@ -380,6 +404,7 @@ class TieredKVDecoder:
         return self.num_layers * (self.layer_attn_bytes(nb + 1) + self.layer_append_bytes())
 
     def layer_attn_bytes(self, body_tokens: int) -> int:
+        """Without a shared prefix's bytes (its lengths are on the device)."""
         ng = 128 // self.group
         meta = 4 * ng + (ng if self.fmt == "ref" else 0)
         per_tok_body = 2 * (64 + meta)

@@ -66,7 +66,9 @@ class PagePool:
         (sampling several continuations, reordering the beams of a search); -1
         empties it. Full pages are shared; a partly filled last page goes to the
         lowest b with that parent and is copied for the others. An int32 tensor
-        on the device is used as it is."""
+        on the device is used as it is. Afterwards only tokens behind the lengths
+        may be written: a sequence that is to be cut back into shared pages or
+        filled anew is emptied (-1, ``free``) first."""
         with kv.launch_on(self.refs.device, stream):
             par = self._per_sequence(parents, "parents")
             self._call("hkv_pages_fork", self.refs.data_ptr(), par.data_ptr())

@@ -158,4 +158,70 @@ def test_refusals():
     with pytest.raises(ValueError):
         run.dec.set_rotary(run.table, run.qw[:1])
     with pytest.raises(ValueError):
-        run.dec.fork([0, 0, 0, 0, 0, -1])
+        run.dec.fork([0, 0, 0, 0, 0, -2])
+
+
+def test_parents_on_the_device_and_emptied_sequences():
+    from hetero_kvcache_optimizer_b200 import _lib
+    _lib.device_error(clear=True)
+    run = Run("fp16min", seed=7)
+    run.dec.reserve(200)
+    pos = torch.arange(run.B, dtype=torch.int64, device="cuda")
+    for _ in range(20):
+        q, k, v = run.inputs()
+        run.dec.step(q, k, v, positions=pos)
+    for parents in (torch.tensor([4, -1, 4, 0, -1, 0], device="cuda"), [-1, 2, 2, 3, 3, -1]):
+        run.dec.fork(parents)
+        run.dec.reserve(200)
+        gone = [b for b in range(run.B) if int(parents[b]) < 0]
+        for st, d in zip(run.dec.stores, run.dec.dense):
+            assert all(st.lengths[b] == 0 and d.lengths[b] == 0 for b in gone)
+        for _ in range(11):
+            q, k, v = run.inputs()
+            out = run.dec.step(q, k, v, positions=pos)
+        run.check(out, q, pos)
+    assert _lib.device_error() == 0
+
+
+def test_prefill_after_a_fork_writes_no_shared_page():
+    from hetero_kvcache_optimizer_b200 import _lib
+    _lib.device_error(clear=True)
+    run = Run("ref", seed=8)
+    n = 2 + 6 + 300
+    pos = torch.full((run.B,), 3, dtype=torch.int32, device="cuda")
+    for again in range(2):
+        for l in range(run.L):
+            run.dec.prefill_layer(l, run.randn(run.B, run.H, n, 128).to(BF16), run.randn(run.B, run.H, n, 128).to(BF16))
+        for st in run.dec.stores:
+            t = st.page_table[st.page_table >= 0]
+            assert t.numel() == run.B * run.H * 3 and t.unique().numel() == t.numel()
+        run.dec.reserve(20)
+        q, k, v = run.inputs()
+        run.check(run.dec.step(q, k, v, positions=pos), q, pos)
+        run.dec.fork([0, 0, 0, 1, 1, 1])
+    run.dec.set_state(200)
+    for st in run.dec.stores:
+        t = st.page_table[st.page_table >= 0]
+        assert t.numel() == run.B * run.H * 2 and t.unique().numel() == t.numel()
+    assert _lib.device_error() == 0
+
+
+def test_attention_alone_sees_the_prefix_and_a_stale_graph_is_dropped():
+    from hetero_kvcache_optimizer_b200 import _lib
+    _lib.device_error(clear=True)
+    run = Run("fp16min", prefix=False, seed=9)
+    run.dec.reserve(64)
+    pos = torch.zeros(run.B, dtype=torch.int32, device="cuda")
+    for _ in range(12):
+        q, k, v = run.inputs()
+        run.dec.step(q, k, v, positions=pos)
+    run.dec.capture(4, positions=pos)
+    run.dec.attach_prefix(run.prefix)
+    with pytest.raises(RuntimeError):
+        run.dec.replay()
+    q = run.inputs()[0]
+    out = torch.empty(run.L, run.B, run.H * run.G, 128, device="cuda")
+    ready = torch.stack([run.kv.norm_rope(q[l], None, pos, run.table, run.qw[l])[0] for l in range(run.L)])
+    run.dec.decode_only(ready, out)
+    run.check(out, q, pos)
+    assert _lib.device_error() == 0
