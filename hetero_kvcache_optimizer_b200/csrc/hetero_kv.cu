@@ -674,29 +674,23 @@ hkv_status shared_plan(const hkv_int4_store* prefix, const int32_t* start, const
 }
 
 // --------------------------------------------------------------------------- norm + rotation
-template <typename T, int MODE, int kHeads, bool LOOP>
-cudaError_t launch_norm_rope(hkv::NormRopeParams& p, int per_warp, cudaStream_t st) {
-  p.per_warp = per_warp;
-  for (int i = 0; i < 2; ++i) p.chunks[i] = cdiv(p.H[i], per_warp);
+template <typename T, int MODE, int kHeads>
+cudaError_t launch_norm_rope(hkv::NormRopeParams& p, cudaStream_t st) {
+  for (int i = 0; i < 2; ++i) p.chunks[i] = cdiv(p.H[i], kHeads);
   p.items = (uint32_t)((int64_t)p.B * p.T * (p.chunks[0] + p.chunks[1]));
   const int grid = cdiv(p.items, hkv::kNrThreads / 32);
-  return launch_pdl(8, hkv::norm_rope_kernel<T, MODE, kHeads, LOOP>, dim3((unsigned)grid), dim3(hkv::kNrThreads), 0, st, p);
+  return launch_pdl(8, hkv::norm_rope_kernel<T, MODE, kHeads>, dim3((unsigned)grid), dim3(hkv::kNrThreads), 0, st, p);
 }
 
 template <typename T>
 cudaError_t launch_norm_rope_t(hkv::NormRopeParams& p, int mode, cudaStream_t st) {
   // Two heads a warp while that leaves warps to spare (320 rows: 2.9 us against 3.6 with
-  // eight); all of a token's heads where that still makes four times the resident warps
-  // (the table row and the weights are loaded once: 32,768 tokens of 40 heads 145 us
-  // against 154, but 4,096 tokens of 32 heads 22.8 us against 22.1); else eight.
-  const int64_t tokens = (int64_t)p.B * p.T, warps = (int64_t)device_sms() * 24;
-  const int most = std::max(p.H[0], p.H[1]);
-  const bool few = tokens * (p.H[0] + p.H[1]) <= (int64_t)device_sms() * 64, all = most > 8 && tokens * 2 >= 4 * warps;
-#define HKV_NR(MODE)                                           \
-  (few ? launch_norm_rope<T, MODE, 2, false>(p, 2, st)         \
-       : all ? launch_norm_rope<T, MODE, 8, true>(p, most, st) \
-             : launch_norm_rope<T, MODE, 8, false>(p, 8, st))
-  return mode == hkv::kNrLane ? HKV_NR(hkv::kNrLane) : mode == hkv::kNrAdjacent ? HKV_NR(hkv::kNrAdjacent) : HKV_NR(hkv::kNrAny);
+  // eight), else eight (all heads of a token in one warp, their loads ahead of their work,
+  // saves the table's re-reads and costs resident warps: 124.7 us against 124.2 for
+  // 32,768 tokens of 40 heads).
+  const bool few = (int64_t)p.B * p.T * (p.H[0] + p.H[1]) <= (int64_t)device_sms() * 64;
+#define HKV_NR(MODE) (few ? launch_norm_rope<T, MODE, 2>(p, st) : launch_norm_rope<T, MODE, 8>(p, st))
+  return mode == hkv::kNrWhole ? HKV_NR(hkv::kNrWhole) : mode == hkv::kNrLane ? HKV_NR(hkv::kNrLane) : mode == hkv::kNrAdjacent ? HKV_NR(hkv::kNrAdjacent) : HKV_NR(hkv::kNrAny);
 #undef HKV_NR
 }
 }  // namespace
@@ -1430,7 +1424,7 @@ hkv_status hkv_norm_rope(const hkv_rows* q, const hkv_rows* k, const hkv_rows* q
   p.B = B;
   p.T = T;
   p.table_vec = table && aligned16(table) && table_stride % 4 == 0 && rot % 8 == 0;
-  const int mode = adjacent ? hkv::kNrAdjacent : rot % 16 == 0 ? hkv::kNrLane : hkv::kNrAny;
+  const int mode = adjacent ? hkv::kNrAdjacent : rot == HKV_D ? hkv::kNrWhole : rot % 16 == 0 ? hkv::kNrLane : hkv::kNrAny;
   const cudaError_t e = dtype == HKV_DT_F16 ? launch_norm_rope_t<__half>(p, mode, S(stream))
                                             : launch_norm_rope_t<__nv_bfloat16>(p, mode, S(stream));
   if (e != cudaSuccess) return cuda_fail(e);

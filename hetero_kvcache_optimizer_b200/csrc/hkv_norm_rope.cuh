@@ -11,12 +11,15 @@
 // of its heads). A half-warp holds a row (16 lanes x 8 values: one 16-byte load
 // and store a lane), and a warp takes kHeads heads of ONE token, two rows at a
 // time: cos and sin stay in registers for all of them, and all loads of the
-// warp's rows are in flight before the first is used. A pair's other half is 8 k
-// dims away when rot % 16 == 0, so it sits in the same register of another lane
-// (one shuffle); other sizes read it from the row again (L1).
-// Measured: 32,768 tokens of 32 + 8 heads 145 us = 4.7 TB/s (a kernel that only copies
-// the same rows: 107 us), 4,096 tokens of 28 + 4 heads 22.1 us, 8 tokens of 32 + 8
-// heads 2.9 us (a launch).
+// warp's rows are in flight before the first is used. With rot = 128 a lane holds
+// both halves of four pairs instead (two 8-byte loads: no exchange, one unpacking,
+// 145 -> 124 us below); with another rot % 16 == 0 a pair's other half is 8 k dims
+// away and sits in the same register of another lane (one shuffle); other sizes read
+// it from the row again (L1).
+// Measured: 32,768 tokens of 32 + 8 heads 124 us = 5.5 TB/s (a kernel that only copies
+// the same rows: 107 us), 4,096 tokens of 28 + 4 heads 16.7 us, 8 tokens of 32 + 8
+// heads 2.5 us (a launch). Issue slots are the second bound: about 60 instructions a
+// row and warp.
 // The next launch is let in after this one's wait, so that it never runs beside
 // a grid two launches back.
 #pragma once
@@ -42,14 +45,14 @@ struct NormRopeParams {
   float eps;
   int B, T;
   uint32_t items;          // warps' pieces of work
-  int per_warp;            // heads of one token a warp takes
   int chunks[2];           // warps per token of q and of k
 };
 
 constexpr int kNrThreads = 256;
 
 // Half-split pairs whose halves are whole lanes apart | pairs of neighbours | any other half-split
-enum { kNrLane = 0, kNrAdjacent = 1, kNrAny = 2 };
+// | half-split pairs over the whole head (rot = 128): a lane holds both halves of four pairs
+enum { kNrLane = 0, kNrAdjacent = 1, kNrAny = 2, kNrWhole = 3 };
 
 template <typename T>
 __device__ __forceinline__ void nr_unpack(const uint4& r, float (&v)[8]) {
@@ -75,31 +78,44 @@ __device__ __forceinline__ uint4 nr_load(const T* p, bool vec) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Four values from `p` and four from `p + 64`.
+template <typename T>
+__device__ __forceinline__ uint4 nr_load2(const T* p, bool vec) {
+  uint2 a, b;
+  if (vec) {
+    a = *reinterpret_cast<const uint2*>(p);
+    b = *reinterpret_cast<const uint2*>(p + 64);
+  } else {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+    a = make_uint2((uint32_t)h[0] | ((uint32_t)h[1] << 16), (uint32_t)h[2] | ((uint32_t)h[3] << 16));
+    b = make_uint2((uint32_t)h[64] | ((uint32_t)h[65] << 16), (uint32_t)h[66] | ((uint32_t)h[67] << 16));
+  }
+  return make_uint4(a.x, a.y, b.x, b.y);
+}
+
 __device__ __forceinline__ void nr_ld4(const float* p, float* v) {
   const float4 x = __ldg(reinterpret_cast<const float4*>(p));
   v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
 }
 
-// One warp: heads h0 .. h1 - 1 of side SIDE (0 q, 1 k) of token (b, t): at most kHeads
-// of them, or with LOOP kHeads at a time, the next ones' loads out before these are
-// worked on. With rn the row's factor, out = rn (x (w c) + x' (w' s)), x' and w' the
+// One warp: heads h0 .. h1 - 1 (at most kHeads) of side SIDE (0 q, 1 k) of token (b, t). With rn the row's factor, out = rn (x (w c) + x' (w' s)), x' and w' the
 // pair's other half: the products with the weights are made once for all heads, and
 // x' is exchanged as it was loaded (16 bits), beside the sum of squares.
-template <typename T, int MODE, int kHeads, bool LOOP, int SIDE>
+template <typename T, int MODE, int kHeads, int SIDE>
 __device__ __forceinline__ void nr_rows(const NormRopeParams& p, int b, int t, int h0, int h1, int lane) {
   const int l = lane & 15, hi = lane >> 4;
   const int64_t pi = (int64_t)b * p.ps_b + (int64_t)t * p.ps_t;
   const int64_t pos = !p.pos ? 0 : p.pos64 ? static_cast<const int64_t*>(p.pos)[pi] : (int64_t) static_cast<const int32_t*>(p.pos)[pi];
-  const T* x = static_cast<const T*>(p.x[SIDE]) + b * p.xs[SIDE][0] + t * p.xs[SIDE][2] + (int64_t)(h0 + hi) * p.xs[SIDE][1] + 8 * l;
+  constexpr bool kWhole = MODE == kNrWhole;
+  constexpr int kPer = kWhole ? 4 : 8;  // neighbouring values of a lane
+  const T* x = static_cast<const T*>(p.x[SIDE]) + b * p.xs[SIDE][0] + t * p.xs[SIDE][2] + (int64_t)(h0 + hi) * p.xs[SIDE][1] + kPer * l;
   const int64_t xstep = 2 * p.xs[SIDE][1];
   const bool vec = p.vec[SIDE];
-  uint4 raw[kHeads / 2], nraw[LOOP ? kHeads / 2 : 1];
+  uint4 raw[kHeads / 2];
   const T* xn = x;
-  auto fetch = [&](int h, uint4* v) {
 #pragma unroll
-    for (int i = 0; i < kHeads / 2; ++i, xn += xstep) v[i] = h + 2 * i + hi < h1 ? nr_load(xn, vec) : make_uint4(0, 0, 0, 0);
-  };
-  fetch(h0, LOOP ? nraw : raw);
+  for (int i = 0; i < kHeads / 2; ++i, xn += xstep)
+    raw[i] = h0 + 2 * i + hi < h1 ? (kWhole ? nr_load2(xn, vec) : nr_load(xn, vec)) : make_uint4(0, 0, 0, 0);
   if (pos < 0) return;  // a padding row: not written
   if (pos >= p.max_pos) {
     if (lane == 0) hkv_flag_error(HKV_DEVERR_BAD_POSITION);
@@ -113,16 +129,36 @@ __device__ __forceinline__ void nr_rows(const NormRopeParams& p, int b, int t, i
   for (int e = 0; e < 8; ++e) w[e] = cs[e] = 1.f, sn[e] = 0.f;
   if (wp) {
     if (p.w_dtype[SIDE] == DT<T>::id && (reinterpret_cast<uintptr_t>(wp) & 15) == 0) {
-      nr_unpack<T>(__ldg(reinterpret_cast<const uint4*>(wp) + l), w);
+      if constexpr (kWhole) {
+        const uint2 a = __ldg(reinterpret_cast<const uint2*>(wp) + l), c = __ldg(reinterpret_cast<const uint2*>(wp) + 16 + l);
+        nr_unpack<T>(make_uint4(a.x, a.y, c.x, c.y), w);
+      } else {
+        nr_unpack<T>(__ldg(reinterpret_cast<const uint4*>(wp) + l), w);
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = load_any(wp, p.w_dtype[SIDE], 8 * l + e);
+      for (int e = 0; e < 8; ++e) w[e] = load_any(wp, p.w_dtype[SIDE], kWhole ? 4 * l + (e & 3) + 16 * (e & 4) : 8 * l + e);
     }
   }
   const int k = r >> 3;  // kNrLane: lanes between the halves of a pair
   const int from = (lane & 16) | (l < k ? l + k : l < 2 * k ? l - k : l);
   const bool turned = MODE == kNrAdjacent ? 4 * l < r : 8 * l < 2 * r;  // some of the lane's values
-  if constexpr (MODE == kNrAdjacent) {
+  if constexpr (kWhole) {
+    if (p.table_vec) {
+      nr_ld4(row + 4 * l, cs);
+      nr_ld4(row + 64 + 4 * l, sn);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) cs[e] = __ldg(row + 4 * l + e), sn[e] = __ldg(row + 64 + 4 * l + e);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      cs[e + 4] = cs[e] * w[e + 4];
+      sn[e + 4] = sn[e] * w[e];
+      cs[e] *= w[e];
+      sn[e] *= -w[e + 4];
+    }
+  } else if constexpr (MODE == kNrAdjacent) {
     if (p.table_vec) {  // r is a multiple of 4: the lane's four pairs turn together or not at all
       if (turned) {
         nr_ld4(row + 4 * l, cs);
@@ -165,90 +201,98 @@ __device__ __forceinline__ void nr_rows(const NormRopeParams& p, int b, int t, i
       cs[e] *= w[e];
     }
   }
-  T* yi = static_cast<T*>(p.y[SIDE]) + b * p.ys[SIDE][0] + t * p.ys[SIDE][2] + (int64_t)(h0 + hi) * p.ys[SIDE][1] + 8 * l;
+  T* yi = static_cast<T*>(p.y[SIDE]) + b * p.ys[SIDE][0] + t * p.ys[SIDE][2] + (int64_t)(h0 + hi) * p.ys[SIDE][1] + kPer * l;
   const int64_t ystep = 2 * p.ys[SIDE][1];
   const T* xi = x - 8 * l;
-#pragma unroll 1
-  for (int h = h0;; h += kHeads) {
-    if constexpr (LOOP) {
 #pragma unroll
-      for (int i = 0; i < kHeads / 2; ++i) raw[i] = nraw[i];
-      if (h + kHeads < h1) fetch(h + kHeads, nraw);
+  for (int i = 0; i < kHeads / 2; ++i, yi += ystep, xi += xstep) {
+    const bool on = h0 + 2 * i + hi < h1;
+    float v[8], o[8];
+    nr_unpack<T>(raw[i], v);
+    float rn = 1.f;
+    if (wp) {
+      float2 s2 = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) s2 = __ffma2_rn(make_float2(v[e], v[e + 1]), make_float2(v[e], v[e + 1]), s2);
+      float s = s2.x + s2.y;
+#pragma unroll
+      for (int q = 1; q < 16; q <<= 1) s += __shfl_xor_sync(0xffffffffu, s, q);
+      rn = rsqrtf(s * (1.f / HKV_D) + p.eps);
     }
-#pragma unroll
-    for (int i = 0; i < kHeads / 2; ++i, yi += ystep, xi += xstep) {
-      const bool on = h + 2 * i + hi < h1;
-      float v[8], o[8];
-      nr_unpack<T>(raw[i], v);
-      float rn = 1.f;
-      if (wp) {
-        float2 s2 = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) s2 = __ffma2_rn(make_float2(v[e], v[e + 1]), make_float2(v[e], v[e + 1]), s2);
-        float s = s2.x + s2.y;
-#pragma unroll
-        for (int q = 1; q < 16; q <<= 1) s += __shfl_xor_sync(0xffffffffu, s, q);
-        rn = rsqrtf(s * (1.f / HKV_D) + p.eps);
-      }
-      if constexpr (MODE == kNrAdjacent) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float a = v[2 * e] * w[2 * e], c = v[2 * e + 1] * w[2 * e + 1];
-          const bool on_pair = 4 * l + e < r;  // the rest passes through, infinities included
-          o[2 * e] = on_pair ? a * cs[e] - c * sn[e] : a;
-          o[2 * e + 1] = on_pair ? c * cs[e] + a * sn[e] : c;
-        }
-      } else if constexpr (MODE == kNrLane) {
-        uint4 po;  // the pairs' other halves; nothing (not an infinity) where a lane passes through
-        po.x = __shfl_sync(0xffffffffu, raw[i].x, from);
-        po.y = __shfl_sync(0xffffffffu, raw[i].y, from);
-        po.z = __shfl_sync(0xffffffffu, raw[i].z, from);
-        po.w = __shfl_sync(0xffffffffu, raw[i].w, from);
-        if (!turned) po = make_uint4(0, 0, 0, 0);
-        nr_unpack<T>(po, o);
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const float2 z = __fmul2_rn(make_float2(o[e], o[e + 1]), make_float2(sn[e], sn[e + 1]));
-          const float2 u = __ffma2_rn(make_float2(v[e], v[e + 1]), make_float2(cs[e], cs[e + 1]), z);
-          o[e] = u.x, o[e + 1] = u.y;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int d = 8 * l + e;
-          o[e] = v[e] * cs[e];
-          if (on && d < 2 * r) o[e] = fmaf(to_f32(xi[d < r ? d + r : d - r]), sn[e], o[e]);
-        }
-        __syncwarp();  // in place: the row's values are all read before the first is written
-      }
+    if constexpr (kWhole) {
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
-        const float2 u = __fmul2_rn(make_float2(o[e], o[e + 1]), make_float2(rn, rn));
+        const float2 z = __fmul2_rn(make_float2(v[e ^ 4], v[(e + 1) ^ 4]), make_float2(sn[e], sn[e + 1]));
+        const float2 u = __ffma2_rn(make_float2(v[e], v[e + 1]), make_float2(cs[e], cs[e + 1]), z);
         o[e] = u.x, o[e + 1] = u.y;
       }
-      if (!on) continue;
+    } else if constexpr (MODE == kNrAdjacent) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float a = v[2 * e] * w[2 * e], c = v[2 * e + 1] * w[2 * e + 1];
+        const bool on_pair = 4 * l + e < r;  // the rest passes through, infinities included
+        o[2 * e] = on_pair ? a * cs[e] - c * sn[e] : a;
+        o[2 * e + 1] = on_pair ? c * cs[e] + a * sn[e] : c;
+      }
+    } else if constexpr (MODE == kNrLane) {
+      uint4 po;  // the pairs' other halves; nothing (not an infinity) where a lane passes through
+      po.x = __shfl_sync(0xffffffffu, raw[i].x, from);
+      po.y = __shfl_sync(0xffffffffu, raw[i].y, from);
+      po.z = __shfl_sync(0xffffffffu, raw[i].z, from);
+      po.w = __shfl_sync(0xffffffffu, raw[i].w, from);
+      if (!turned) po = make_uint4(0, 0, 0, 0);
+      nr_unpack<T>(po, o);
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float2 z = __fmul2_rn(make_float2(o[e], o[e + 1]), make_float2(sn[e], sn[e + 1]));
+        const float2 u = __ffma2_rn(make_float2(v[e], v[e + 1]), make_float2(cs[e], cs[e + 1]), z);
+        o[e] = u.x, o[e + 1] = u.y;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int d = 8 * l + e;
+        o[e] = v[e] * cs[e];
+        if (on && d < 2 * r) o[e] = fmaf(to_f32(xi[d < r ? d + r : d - r]), sn[e], o[e]);
+      }
+      __syncwarp();  // in place: the row's values are all read before the first is written
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float2 u = __fmul2_rn(make_float2(o[e], o[e + 1]), make_float2(rn, rn));
+      o[e] = u.x, o[e + 1] = u.y;
+    }
+    if (!on) continue;
+    if constexpr (kWhole) {
       if (vec) {
-        *reinterpret_cast<uint4*>(yi) = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]), pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));
+        *reinterpret_cast<uint2*>(yi) = make_uint2(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]));
+        *reinterpret_cast<uint2*>(yi + 64) = make_uint2(pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) yi[e] = from_f32<T>(o[e]);
+        for (int e = 0; e < 8; ++e) yi[(e & 3) + 16 * (e & 4)] = from_f32<T>(o[e]);
       }
+    } else if (vec) {
+      *reinterpret_cast<uint4*>(yi) = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]), pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) yi[e] = from_f32<T>(o[e]);
     }
-    if (!LOOP || h + kHeads >= h1) break;
   }
 }
 
-template <typename T, int MODE, int kHeads, bool LOOP>
-__global__ void __launch_bounds__(kNrThreads, MODE == kNrAny ? 2 : LOOP ? 3 : 4) norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
+// Five CTAs an SM where 48 registers do (whole heads: 16.7 against 18.1 us for a chunk with
+// four, 124 against 133 for a prompt).
+template <typename T, int MODE, int kHeads>
+__global__ void __launch_bounds__(kNrThreads, MODE == kNrAny ? 2 : MODE == kNrWhole ? 5 : 4) norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
   const uint32_t item = blockIdx.x * (kNrThreads / 32) + (threadIdx.x >> 5);
   griddep_wait();
   griddep_launch_dependents();
   if (item >= p.items) return;
   const uint32_t per = p.chunks[0] + p.chunks[1], tok = item / per;
   const int c = (int)(item - tok * per), b = (int)(tok / (uint32_t)p.T), t = (int)(tok - (uint32_t)b * p.T), lane = threadIdx.x & 31;
-  const int h0 = (c < p.chunks[0] ? c : c - p.chunks[0]) * p.per_warp;
-  if (c < p.chunks[0]) nr_rows<T, MODE, kHeads, LOOP, 0>(p, b, t, h0, min(p.H[0], h0 + p.per_warp), lane);
-  else nr_rows<T, MODE, kHeads, LOOP, 1>(p, b, t, h0, min(p.H[1], h0 + p.per_warp), lane);
+  const int h0 = (c < p.chunks[0] ? c : c - p.chunks[0]) * kHeads;
+  if (c < p.chunks[0]) nr_rows<T, MODE, kHeads, 0>(p, b, t, h0, min(p.H[0], h0 + kHeads), lane);
+  else nr_rows<T, MODE, kHeads, 1>(p, b, t, h0, min(p.H[1], h0 + kHeads), lane);
 }
 
 }  // namespace hkv

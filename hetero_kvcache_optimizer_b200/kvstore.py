@@ -701,8 +701,9 @@ def norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: O
     dt = dtype_code(dtype)
     if dt == L.DT_F32:
         raise TypeError("norm_rope takes float16 or bfloat16")
+    index = x0.get_device()
     for t in (q, k, positions, table, q_weight, k_weight, q_out, k_out):
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:
             _require_cuda(t)
             raise ValueError("all tensors must be on one device")
     _require_cuda(x0)
@@ -747,9 +748,9 @@ def norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: O
         tptr, pptr = table.data_ptr(), positions.data_ptr()
     with launch_on(device, stream):
         if q is not None and q_out is None:
-            q_out = torch.empty(q.shape, dtype=dtype, device=device)
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         if k is not None and k_out is None:
-            k_out = torch.empty(k.shape, dtype=dtype, device=device)
+            k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
         if B and T:
             L.check(L.load().hkv_norm_rope(
                 _rows(q), _rows(k), _rows(q_out), _rows(k_out), dt, B, T, HEAD_DIM,
@@ -821,7 +822,7 @@ def decode_shared(q: torch.Tensor, prefix: SharedPrefix, store: Optional[Int4KVS
         raise ValueError("out must be [B, Hq, 128] on q's device with a contiguous head dimension")
     with launch_on(q.device, stream):
         if out is None:
-            out = torch.empty(B, Hq, D, dtype=out_dtype, device=q.device)
+            out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
         G = Hq // Hkv
         if G > 8 and Hq % Hkv == 0 and (store is not None or dense is not None):
             gs = max(d for d in range(1, 9) if G % d == 0)  # as in ``decode``
