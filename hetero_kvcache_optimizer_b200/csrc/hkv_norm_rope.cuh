@@ -18,8 +18,7 @@
 // it from the row again (L1).
 // Measured: 32,768 tokens of 32 + 8 heads 124 us = 5.5 TB/s (a kernel that only copies
 // the same rows: 107 us), 4,096 tokens of 28 + 4 heads 16.7 us, 8 tokens of 32 + 8
-// heads 2.5 us (a launch). Issue slots are the second bound: about 60 instructions a
-// row and warp.
+// heads 2.5 us (a launch). 61 warp instructions a row keep 60 % of the issue slots busy.
 // The next launch is let in after this one's wait, so that it never runs beside
 // a grid two launches back.
 #pragma once
