@@ -86,6 +86,22 @@ def test_many_rows_take_the_wide_split(kv):
         check(ko, expected(k, pos, table, w, 1e-6, adjacent))
 
 
+@pytest.mark.parametrize("T", [5, 1501])
+@pytest.mark.parametrize("rot,adjacent", [(128, False), (96, False), (64, False), (44, False), (64, True)])
+def test_tables_and_weights_that_are_slices(kv, rot, adjacent, T):
+    q, k = inputs(3, 2, 9, T, F16), inputs(4, 2, 8, T, F16)
+    wide = torch.zeros(T, rot + 9, device="cuda")
+    w3 = 1 + 0.3 * torch.randn(3 * 128 + 1, device="cuda")
+    pos = torch.arange(T, device="cuda").expand(2, -1)
+    for off in (0, 1, 4):  # table rows of odd strides, from odd addresses
+        table = wide[:, off:off + rot]
+        table.copy_(kv.rope_table(T, rot))
+        for w in (w3[:128], w3[1:129].to(BF16), w3.to(F16)[1:129]):
+            qo, ko = kv.norm_rope(q, k, pos, table, w, w, adjacent=adjacent)
+            check(qo, expected(q, pos, table, w, 1e-6, adjacent))
+            check(ko, expected(k, pos, table, w, 1e-6, adjacent))
+
+
 @pytest.mark.parametrize("rot,adjacent", [(128, False), (20, False), (128, True)])
 def test_strided_in_place_and_unaligned(kv, rot, adjacent):
     B, T, Hq, Hkv = 2, 37, 6, 2
