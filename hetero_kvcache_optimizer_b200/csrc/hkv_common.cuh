@@ -102,6 +102,9 @@ __device__ __forceinline__ bool mbar_try_wait_sleep(uint64_t* bar, uint32_t pari
 // completed and its memory operations are visible, so it goes before the first
 // global access; griddep_launch_dependents lets the next grid in the stream
 // start its own prologue early (that grid then waits for this one the same way).
+// A grid launched with the attribute lets the next one in after its own wait, never
+// before: the next then runs beside this one alone, every grid further back having
+// completed. The fused decode step's early reads (HKV_APPEND_EARLY) rest on that.
 // Both are no-ops for a normal launch.
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void griddep_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

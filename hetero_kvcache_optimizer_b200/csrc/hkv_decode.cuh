@@ -1190,13 +1190,12 @@ __global__ void __launch_bounds__(decode_threads(FMT, APPEND), 1)
   float* comb = reinterpret_cast<float*>(ring + nsl * kSlot);  // [8][G][128] + [8][8][2]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  // The next grid in the stream may start its prologue now (it waits for this one
-  // before touching global memory, as this one does below). In early mode the
-  // trigger waits until this grid has waited for the one before it (thread 0,
-  // consumer section): a grid then starts only once every grid two or more
-  // launches back has completed, which is what lets it read its cache early.
+  // The next grid in the stream is let in only after this grid has waited for the
+  // one before it (below; in early mode by thread 0, consumer section): a grid
+  // then starts only once every grid two or more launches back has completed,
+  // which is what lets an early grid read its cache before its own wait, whatever
+  // the grid before it is. A late grid lets the next one in by its end.
   const bool early = APPEND && p.early, late = !APPEND && p.late;
-  if (!early) griddep_launch_dependents();
   Piece first = first_piece_head(p, c, end);  // parameters only
   uint8_t* qbuf = reinterpret_cast<uint8_t*>(comb + kConsumerWarps * p.G * HKV_D + kConsumerWarps * 16);
   if (warp == kConsumerWarps - 1 && lane < nsl) {  // a warp whose first work waits anyway
@@ -1212,7 +1211,10 @@ __global__ void __launch_bounds__(decode_threads(FMT, APPEND), 1)
   // launches back, so it is read, and the ring filled, before the wait; every
   // role waits on its own before it reads the query or the new token (made by
   // the grid just before) and before its first global write.
-  if (!early && !late) griddep_wait();
+  if (!early && !late) {
+    griddep_wait();
+    griddep_launch_dependents();
+  }
   const int2 first_st = first.valid ? seg_state<APPEND>(p, first.u, first.seg) : make_int2(0, -1);
   if (!early && warp < kConsumerWarps && p.q_async && first.valid) q_prefetch(p, first.u, qbuf);
   __syncthreads();

@@ -267,7 +267,13 @@ hkv_status hkv_decode_attn(const void* q, int32_t q_dtype, int64_t q_stride_b,
  * multi-layer step, each layer's cache touched once per step. The launch then
  * reads its cache and streams the first tiles while that kernel finishes
  * (programmatic dependent launch), and only the query, the new token and its
- * own writes wait for it. Without the guarantee pass 0. */
+ * own writes wait for it. Kernels further back have completed by then: every
+ * kernel of this library lets the next one start only after it has itself waited
+ * for the one before it, and a kernel launched without the programmatic attribute
+ * starts after all before it. A caller's own kernel that is launched with that
+ * attribute and lets its dependents in before its own wait breaks this: it counts
+ * together with the kernels before it as "just before this call". Without the
+ * guarantee pass 0. */
 #define HKV_APPEND_EARLY 1
 hkv_status hkv_decode_append(const void* q, int32_t q_dtype, int64_t q_stride_b, int64_t q_stride_h,
                              const void* k_new, const void* v_new, int64_t new_stride_b, int64_t new_stride_h,

@@ -1,0 +1,48 @@
+"""TieredKVDecoder over page pools: steps, forks and reserves back to back."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+def decoder(layers, **kw):
+    from hetero_kvcache_optimizer_b200.decode_engine import TieredKVDecoder
+    return TieredKVDecoder(layers, 3, 8, 2, sink=2, recent=6, body_capacity=1024, fmt="fp16min", page_tokens=128,
+                           kv_dtype=BF16, num_pages=40, **kw)
+
+
+@pytest.mark.parametrize("layers", [2, 3])
+@pytest.mark.parametrize("ctas", [2, 0])
+def test_early_layers_see_what_the_pool_calls_and_the_last_step_wrote(layers, ctas):
+    """Fused steps without positions (no launch between the layers), with pool calls just
+    before them and few CTAs (room for the next grid beside a running one), give the same
+    bits as steps that wait for everything before them."""
+    from hetero_kvcache_optimizer_b200 import _lib
+    _lib.device_error(clear=True)
+    runs = []
+    for early in (None, False):
+        gen = torch.Generator(device="cuda").manual_seed(5)
+        dec = decoder(layers, ctas=ctas, early=early)
+        for l in range(layers):
+            k, v = (torch.randn(3, 2, 8 + 300, 128, generator=gen, device="cuda").to(BF16) for _ in range(2))
+            dec.prefill_layer(l, k, v)
+        dec.reserve(128)
+        outs = []
+        for step in range(24):
+            q = torch.randn(layers, 3, 8, 128, generator=gen, device="cuda").to(BF16)
+            k, v = (torch.randn(layers, 3, 2, 128, generator=gen, device="cuda").to(BF16) for _ in range(2))
+            if step % 6 == 3:
+                dec.fork([[0, 0, 2], [1, 1, 0], [2, 0, 1], [0, 1, 2]][step // 6])
+                dec.reserve(128)
+            elif step % 6 == 5:
+                dec.pools[layers - 1].reserve(128)
+            outs.append(dec.step(q, k, v))
+        torch.cuda.synchronize()
+        runs.append((outs, [(s.lengths.clone(), s.page_table.clone(), d.k.clone(), d.ring_head.clone())
+                            for s, d in zip(dec.stores, dec.dense)]))
+    for a, b in zip(runs[0][0], runs[1][0]):
+        assert torch.equal(a, b)
+    for a, b in zip(runs[0][1], runs[1][1]):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert _lib.device_error() == 0
