@@ -49,7 +49,7 @@ struct PagesParams {
   int32_t* vecs;             // [wants] 16-byte vectors to copy
   int32_t* list;             // [copies][3]: source page, destination page, vectors
   int32_t* count;            // [1]: entries of list
-  int32_t* first;            // compact: [src_num_pages] first entry naming the page
+  int32_t* first;            // compact: [src_num_pages] first entry naming the page and whether any is in use (pg_see)
   int wants;                 // length of want
 };
 
@@ -241,11 +241,25 @@ __global__ void __launch_bounds__(kPgThreads) pages_fork_apply_kernel(const __gr
 // many first entries it has, then adds up those before it.
 constexpr int kPgSpan = kPgPages * kPgGive;
 
+// What the table says of a page, in one word that entries join in any order: the
+// lowest entry e that names it as kPgEntry - e (0: none; e < 2^30), and kPgUsed if any
+// that names it lies within its sequence's length.
+constexpr int kPgEntry = (1 << 30) - 1, kPgUsed = 1 << 30;
+__device__ __forceinline__ void pg_see(int* seen, int mine) {
+  for (int w = 0;;) {  // nobody yet, as a rule
+    const int both = max(w & kPgEntry, mine & kPgEntry) | ((w | mine) & kPgUsed);
+    if (both == w) return;
+    const int old = atomicCAS(seen, w, both);
+    if (old == w) return;
+    w = old;
+  }
+}
+
 __global__ void __launch_bounds__(kPgThreads) pages_compact_clear_kernel(const __grid_constant__ PagesParams p) {
   griddep_wait();
   griddep_launch_dependents();
   for (int i = blockIdx.x * kPgThreads + threadIdx.x; i < max(p.src_num_pages, p.num_pages); i += gridDim.x * kPgThreads) {
-    if (i < p.src_num_pages) p.first[i] = 0x7fffffff;
+    if (i < p.src_num_pages) p.first[i] = 0;
     if (i < p.num_pages) p.refs[i] = 0;
   }
 }
@@ -256,19 +270,27 @@ __global__ void __launch_bounds__(kPgThreads) pages_compact_map_kernel(const __g
   const int n = p.B * p.H * p.src_max_pages;
   for (int e = blockIdx.x * kPgThreads + threadIdx.x; e < n; e += gridDim.x * kPgThreads) {
     const int page = p.src_table[e];
-    if (pg_ok(page, p.src_num_pages)) atomicMin(p.first + page, e);
-    else if (page >= 0) hkv_flag_error(HKV_DEVERR_BAD_PAGE);
+    if (pg_ok(page, p.src_num_pages)) {
+      const int u = e / p.src_max_pages, i = e - u * p.src_max_pages;
+      pg_see(p.first + page, (kPgEntry - e) | ((int64_t)i * p.page_tokens < p.src_lengths[u / p.H] ? kPgUsed : 0));
+    } else if (page >= 0) {
+      hkv_flag_error(HKV_DEVERR_BAD_PAGE);
+    }
   }
 }
 
-// Which of the thread's kPgPages entries from e1 on name a page first.
+// Which of the thread's kPgPages entries from e1 on name a page first (and, in the
+// bits from kPgPages on, which of those pages any sequence uses).
 __device__ __forceinline__ unsigned pg_firsts(const PagesParams& p, int e1, int n, int (&page)[kPgPages]) {
   unsigned mask = 0;
 #pragma unroll
   for (int j = 0; j < kPgPages; ++j) page[j] = e1 + j < n ? p.src_table[e1 + j] : -1;
 #pragma unroll
   for (int j = 0; j < kPgPages; ++j)
-    if (pg_ok(page[j], p.src_num_pages) && p.first[page[j]] == e1 + j) mask |= 1u << j;
+    if (pg_ok(page[j], p.src_num_pages)) {
+      const int w = p.first[page[j]];
+      if ((w & kPgEntry) == kPgEntry - (e1 + j)) mask |= (w & kPgUsed ? (1u << kPgPages) + 1u : 1u) << j;
+    }
   return mask;
 }
 
@@ -278,12 +300,13 @@ __global__ void __launch_bounds__(kPgGive) pages_compact_count_kernel(const __gr
   __shared__ int s_warp[32];
   int page[kPgPages], total;
   const unsigned mask = pg_firsts(p, blockIdx.x * kPgSpan + kPgPages * threadIdx.x, p.B * p.H * p.src_max_pages, page);
-  pg_scan(__popc(mask), total, s_warp);
+  pg_scan(__popc(mask & ((1u << kPgPages) - 1)), total, s_warp);
   if (threadIdx.x == 0) p.from[blockIdx.x] = total;
 }
 
 // list[3 r]: the page of rank r, want[e]: the rank at its first entry e. Pages behind
-// the sequence's length keep their place but are not copied (list[3 r + 2] = 0).
+// the length of every sequence that names them keep their place but are not copied
+// (list[3 r + 2] = 0).
 __global__ void __launch_bounds__(kPgGive) pages_compact_give_kernel(const __grid_constant__ PagesParams p) {
   griddep_wait();
   griddep_launch_dependents();
@@ -295,15 +318,14 @@ __global__ void __launch_bounds__(kPgGive) pages_compact_give_kernel(const __gri
   before = total;
   int page[kPgPages];
   const unsigned mask = pg_firsts(p, e1, n, page);
-  int r = before + pg_scan(__popc(mask), total, s_warp);
+  int r = before + pg_scan(__popc(mask & ((1u << kPgPages) - 1)), total, s_warp);
 #pragma unroll
   for (int j = 0; j < kPgPages; ++j)
     if (mask >> j & 1) {
-      const int e = e1 + j, u = e / p.src_max_pages, i = e - u * p.src_max_pages;
-      p.want[e] = r;
+      p.want[e1 + j] = r;
       p.list[3 * r] = page[j];
       p.list[3 * r + 1] = r;
-      p.list[3 * r + 2] = (int64_t)i * p.page_tokens < p.src_lengths[u / p.H] ? p.page_tokens / HKV_BLOCK_TOKENS * (p.block_bytes >> 4) : 0;
+      p.list[3 * r + 2] = mask >> (kPgPages + j) & 1 ? p.page_tokens / HKV_BLOCK_TOKENS * (p.block_bytes >> 4) : 0;
       ++r;
     }
   if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
@@ -323,7 +345,7 @@ __global__ void __launch_bounds__(kPgThreads) pages_compact_apply_kernel(const _
     if (i < p.src_max_pages) {
       const int page = p.src_table[(int64_t)u * p.src_max_pages + i];
       if (pg_ok(page, p.src_num_pages)) {
-        id = p.want[p.first[page]];
+        id = p.want[kPgEntry - (p.first[page] & kPgEntry)];
         if (id < p.num_pages) atomicAdd(p.refs + id, 1);
         else id = -1;
       }

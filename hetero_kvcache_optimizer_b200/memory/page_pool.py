@@ -92,12 +92,12 @@ class PagePool:
         self.fork([-1 if b in gone else b for b in range(self.store.batch)], stream=stream)
 
     def compact(self, into: "PagePool", stream=None) -> None:
-        """Copies every page in use into another pool (same format, page size,
-        batch and heads), in the order of the table: a sequence's pages become
-        consecutive, so that a move to the host is a few long copies, and a
-        smaller pool can take a thinned-out one. ``into`` is rewritten whole
-        (table, lengths, counts); shared pages stay shared; this pool is left as
-        it is."""
+        """Copies every page in use (within the length of any sequence that names
+        it) into another pool (same format, page size, batch and heads), in the
+        order of the table: a sequence's pages become consecutive, so that a move
+        to the host is a few long copies, and a smaller pool can take a
+        thinned-out one. ``into`` is rewritten whole (table, lengths, counts);
+        shared pages stay shared; this pool is left as it is."""
         a, b = self.store, into.store
         if (a.batch, a.kv_heads, a.fmt, a.group, a.page_tokens) != (b.batch, b.kv_heads, b.fmt, b.group, b.page_tokens):
             raise ValueError("compact needs a pool of the same batch, heads, format and page size")

@@ -506,8 +506,8 @@ hkv_status hkv_pages_reserve(const hkv_int4_store* store, int32_t B, int32_t H, 
 /* Copies the store's pages into another pool of the same format, page size and
  * units: in order of their first entry in the table they become pages 0, 1, ...
  * of `into`, whose page_table, lengths and into_refs are rewritten whole; shared
- * pages stay shared. The bytes of pages that lie behind the length are not
- * copied, nor is the rest of into's pool written. into->max_pages >=
+ * pages stay shared. The bytes of pages that lie behind the length of every
+ * sequence that names them are not copied, nor is the rest of into's pool written. into->max_pages >=
  * src->max_pages; src is left as it is; the pools must not overlap. */
 hkv_status hkv_pages_compact(const hkv_int4_store* src, int32_t B, int32_t H, const hkv_int4_store* into,
                              int32_t* into_refs, void* workspace, size_t workspace_bytes, hkv_stream_t stream);

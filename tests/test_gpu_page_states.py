@@ -1,0 +1,70 @@
+"""PagePool calls on states that a long life of forks alone does not reach: sequences cut
+back while others still use the pages, tables and lengths that the caller built, full rows.
+Ids, counts and bytes are equal to what the text of each call says."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+P = 128
+
+
+@pytest.fixture(scope="module")
+def kv():
+    from hetero_kvcache_optimizer_b200 import kvstore
+    return kvstore
+
+
+@pytest.fixture(scope="module")
+def PagePool():
+    from hetero_kvcache_optimizer_b200.memory.page_pool import PagePool
+    return PagePool
+
+
+@pytest.fixture(scope="module")
+def L():
+    from hetero_kvcache_optimizer_b200 import _lib
+    _lib.device_error(clear=True)
+    return _lib
+
+
+def pool_of(kv, PagePool, table, lengths, H, pages, fill=None, fmt="ref", group=128):
+    """A pool over a table [B * H][max_pages] and lengths of the caller's own."""
+    nbytes = kv.page_bytes(fmt, group, P)
+    data = (torch.full((pages, nbytes), fill, dtype=torch.uint8, device="cuda") if fill is not None
+            else torch.randint(0, 256, (pages, nbytes), dtype=torch.uint8, device="cuda", generator=torch.Generator(device="cuda").manual_seed(pages)))
+    return PagePool(kv.Int4KVStore.wrap(data, torch.tensor(table, dtype=torch.int32, device="cuda"),
+                                        torch.tensor(lengths, dtype=torch.int32, device="cuda"), H, fmt=fmt, group=group, page_tokens=P))
+
+
+@pytest.mark.parametrize("lengths", [(0, 300, 150), (129, 384, 1), (128, 127, 384), (384, 0, 0), (0, 0, 0), (1, 0, 129)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_compact_copies_a_page_that_any_sequence_uses(kv, PagePool, L, lengths, wide):
+    """Three sequences of two heads that share pages and stand at different lengths; with
+    `wide` rows the table takes several CTAs to rank and sharers lie in different ones."""
+    H, maxp = 2, 6 if not wide else 3000
+    rows = np.full((6, maxp), -1, np.int64)
+    rows[:, :3] = [[4, 9, 2], [7, 0, 12], [4, 9, 2], [7, 0, 13], [4, 3, 2], [7, 11, 13]]
+    src = pool_of(kv, PagePool, rows.tolist(), lengths, H, 16)
+    into = pool_of(kv, PagePool, np.full((6, maxp), -1).tolist(), [5, 5, 5], H, 16, fill=9)
+    before = src.store.pool.cpu().numpy().copy()
+    src.compact(into)
+    assert L.device_error() == 0
+    rank, used = {}, set()
+    for u in range(6):
+        for i in range(3):
+            rank.setdefault(rows[u, i], len(rank))
+            if i * P < lengths[u // H]:
+                used.add(rows[u, i])
+    want = np.full_like(before, 9)
+    for page in used:
+        want[rank[page]] = before[page]
+    table = np.full((6, maxp), -1)
+    table[:, :3] = np.vectorize(rank.get)(rows[:, :3])
+    assert np.array_equal(into.store.page_table.cpu().numpy(), table)
+    assert np.array_equal(into.store.pool.cpu().numpy(), want)
+    assert np.array_equal(src.store.pool.cpu().numpy(), before)
+    assert into.store.lengths.tolist() == list(lengths)
+    refs = np.zeros(16, np.int64)
+    np.add.at(refs, table[table >= 0], 1)
+    assert into.refs.tolist() == refs.tolist()
