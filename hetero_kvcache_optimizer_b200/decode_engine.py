@@ -24,6 +24,7 @@ projections give them (normed and rotated in one launch before the append).
 """
 from __future__ import annotations
 
+import bisect
 from typing import List, Optional, Sequence, Union
 
 import torch
@@ -64,6 +65,8 @@ class TieredKVDecoder:
         # with num_pages (pages per layer), the bodies' pages are owned by pools
         self.pools: List[PagePool] = [PagePool(st) for st in self.stores] if num_pages is not None else []
         self.prefixes: Optional[List[kv.SharedPrefix]] = None
+        self._groups: List[tuple] = []  # per sequence, the group of its slot in each layer's prefix
+        self._behind: List[tuple] = []  # ... and the one that its own tokens were computed behind
         self._nobody: Optional[torch.Tensor] = None
         self._rotary = None
         self.positions: Optional[torch.Tensor] = None
@@ -87,6 +90,7 @@ class TieredKVDecoder:
             d.k[:, :, self.sink:self.sink + nr] = k[:, :, S - nr:]
             d.v[:, :, self.sink:self.sink + nr] = v[:, :, S - nr:]
         nb = S - ns - nr
+        self._behind = list(self._groups)
         if self.pools:  # pages that others share as well must not be written
             self._empty_pool(layer)
             self.pools[layer].reserve(nb)
@@ -101,6 +105,7 @@ class TieredKVDecoder:
     def set_state(self, body_len: int) -> None:
         """Declare that every layer holds ``body_len`` INT4 tokens and a full sink + ring
         (with ``num_pages``, on pages of each sequence's own)."""
+        self._behind = list(self._groups)
         for l, (st, d) in enumerate(zip(self.stores, self.dense)):
             if self.pools:
                 self._empty_pool(l)
@@ -119,7 +124,9 @@ class TieredKVDecoder:
     def attach_prefix(self, prefixes: Optional[Sequence[kv.SharedPrefix]]) -> None:
         """One shared prefix per layer (None: none), in front of what the layer's
         cache holds; it stays attached until replaced. Steps then append and run
-        ``kvstore.decode_shared``. A captured step is dropped: ``capture`` again."""
+        ``kvstore.decode_shared``. A sequence's group is that of its slot in the
+        batch: what the caches hold now is taken to belong behind it. A captured
+        step is dropped: ``capture`` again."""
         if prefixes is not None:
             prefixes = list(prefixes)
             if len(prefixes) != self.num_layers:
@@ -128,7 +135,18 @@ class TieredKVDecoder:
                 if p.store.kv_heads != self.kv_heads or p.group_start[-1] > self.batch:
                     raise ValueError("a prefix with other KV heads or more sequences than the batch")
         self.prefixes = prefixes
+        self._groups = ([tuple(bisect.bisect_right(p.group_start, b) if b < p.group_start[-1] else 0 for p in prefixes)
+                         for b in range(self.batch)] if prefixes is not None else [])
+        self._behind = list(self._groups)
         self.graph = self.host_graph = self._host = None
+
+    def _check_context(self) -> None:
+        """A fork moves a sequence's own tokens, not its slot's prefix: attention over
+        both would be over a context that no prompt had."""
+        if self.prefixes is not None and self._behind != self._groups:
+            mixed = [b for b in range(self.batch) if self._behind[b] != self._groups[b]]
+            raise RuntimeError(f"sequences {mixed} were forked from another prefix group: their tokens do not follow their "
+                               "slot's prefix (fork within groups, fill them anew, or attach_prefix with other groups)")
 
     def reserve(self, tokens: int) -> None:
         """Pages for ``tokens`` more body tokens in every layer (``num_pages`` only)."""
@@ -141,12 +159,21 @@ class TieredKVDecoder:
         """Sequence b continues from what sequence ``parents[b]`` was, in every layer
         and for all b at once (``num_pages`` only): body pages are shared or copied
         (``PagePool.fork``), the sink and recent rows and their state are copied; -1
-        empties a sequence. ``reserve`` before the next steps."""
+        empties a sequence. ``reserve`` before the next steps.
+
+        With a prefix attached, a parent lies in the sequence's own group (the prefix
+        is the slot's): parents given on the host from another group leave sequences
+        that the next step refuses, until they are filled anew, forked back or given
+        another prefix; parents on the device are not known here and are the caller's
+        to keep within the groups."""
         if not self.pools:
             raise RuntimeError("fork needs a decoder with num_pages")
         par = self.pools[0]._per_sequence(parents, "parents")
         if not isinstance(parents, torch.Tensor) and any(not -1 <= int(b) < self.batch for b in parents):
             raise ValueError(f"parents must be -1 or lie in [0, {self.batch})")
+        if self._groups and not (isinstance(parents, torch.Tensor) and parents.is_cuda):
+            old = self._behind
+            self._behind = [old[a] if 0 <= a < self.batch else self._groups[b] for b, a in enumerate(int(x) for x in parents)]
         at = par.long().clamp(0, self.batch - 1)  # values on the device are not known here
         gone = par != at
         for pool, d in zip(self.pools, self.dense):
@@ -186,6 +213,7 @@ class TieredKVDecoder:
         st, d = self.stores[layer], self.dense[layer]
         hint = len_hint if len_hint is not None else self.body_len + 1
         if self.prefixes is not None:
+            self._check_context()
             kv.append_kv(k_new, v_new, d, self.sink, st)
             return kv.decode_shared(q, self.prefixes[layer], st, d, out_dtype=self.out_dtype, out=out, ctas=self.ctas,
                                     body_len=hint, dense_len=self.sink + self.recent)
@@ -230,6 +258,7 @@ class TieredKVDecoder:
     def decode_only(self, q: torch.Tensor, out: torch.Tensor, len_hint: Optional[int] = None) -> None:
         """Attention of every layer without appending (cache unchanged)."""
         hint = len_hint if len_hint is not None else self.body_len
+        self._check_context()
         for l in range(self.num_layers):
             if self.prefixes is not None:
                 kv.decode_shared(q[l], self.prefixes[l], self.stores[l], self.dense[l], out_dtype=self.out_dtype, out=out[l],
@@ -373,6 +402,7 @@ class TieredKVDecoder:
     def replay(self) -> None:
         if self.graph is None:
             raise RuntimeError("replay needs a captured step (capture; attach_prefix drops it)")
+        self._check_context()
         self.graph.replay()
         self.body_len += 1
 
@@ -385,6 +415,7 @@ class TieredKVDecoder:
         copies everything in, replays the step and copies everything out."""
         if self._host is not None and all(a.data_ptr() == b.data_ptr() for a, b in
                                           zip((q_host, k_host, v_host, out_host), self._host)):
+            self._check_context()
             self.host_graph.replay()
             self.body_len += 1
             return
