@@ -158,8 +158,9 @@ class TieredKVDecoder:
     def fork(self, parents: Union[torch.Tensor, Sequence[int]]) -> None:
         """Sequence b continues from what sequence ``parents[b]`` was, in every layer
         and for all b at once (``num_pages`` only): body pages are shared or copied
-        (``PagePool.fork``), the sink and recent rows and their state are copied; -1
-        empties a sequence. ``reserve`` before the next steps.
+        (``PagePool.fork``), the sink and recent rows and their state are copied, and
+        ``positions`` of a captured step; -1 empties a sequence (its position is 0).
+        ``reserve`` before the next steps.
 
         With a prefix attached, a parent lies in the sequence's own group (the prefix
         is the slot's): parents given on the host from another group leave sequences
@@ -176,6 +177,8 @@ class TieredKVDecoder:
             self._behind = [old[a] if 0 <= a < self.batch else self._groups[b] for b, a in enumerate(int(x) for x in parents)]
         at = par.long().clamp(0, self.batch - 1)  # values on the device are not known here
         gone = par != at
+        if self.positions is not None:  # of the captured step's next tokens
+            self.positions.copy_(self.positions.index_select(0, at).masked_fill_(gone, 0))
         for pool, d in zip(self.pools, self.dense):
             for t in (d.k, d.v, d.lengths, d.ring_head):
                 t.copy_(t.index_select(0, at))

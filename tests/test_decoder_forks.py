@@ -107,3 +107,13 @@ def test_layers_may_be_cut_into_different_groups(dec):
     step(dec)
     dec.fork([0, 1, 2, 0, 4, 5])
     refused(dec)
+
+
+def test_positions_of_a_captured_step_follow_the_fork(dec):
+    dec.positions = torch.tensor([7, 20, 300, 4, 50, 6], dtype=torch.int32)
+    address = dec.positions.data_ptr()
+    dec.fork([2, 0, -1, 5, 5, 3])
+    assert dec.positions.tolist() == [300, 7, 0, 6, 6, 4]
+    dec.fork(torch.tensor([1, 1, 1, -1, 0, 9], dtype=torch.int32))
+    assert dec.positions.tolist() == [7, 7, 7, 0, 300, 0]
+    assert dec.positions.data_ptr() == address  # the graph's own buffer

@@ -46,3 +46,42 @@ def test_early_layers_see_what_the_pool_calls_and_the_last_step_wrote(layers, ct
     for a, b in zip(runs[0][1], runs[1][1]):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
     assert _lib.device_error() == 0
+
+
+def test_a_captured_step_goes_on_from_its_parents_positions():
+    """Sequences at different positions, forked between replays: the same caches and
+    outputs as eager steps that are given the parents' positions."""
+    from hetero_kvcache_optimizer_b200 import _lib, kvstore as kv
+    _lib.device_error(clear=True)
+    runs = []
+    for captured in (True, False):
+        gen = torch.Generator(device="cuda").manual_seed(6)
+        dec = decoder(2)
+        table = kv.rope_table(1024, 128)
+        dec.set_rotary(table)
+        pos = torch.tensor([5, 300, 77], dtype=torch.int32, device="cuda")
+        dec.reserve(128)
+        if captured:
+            dec.capture(20, positions=pos)
+        outs = []
+        for step in range(9):
+            q = torch.randn(2, 3, 8, 128, generator=gen, device="cuda").to(BF16)
+            k, v = (torch.randn(2, 3, 2, 128, generator=gen, device="cuda").to(BF16) for _ in range(2))
+            if step in (3, 6):
+                parents = [1, 0, 1] if step == 3 else [2, -1, 0]
+                dec.fork(parents)
+                pos = torch.where(torch.tensor(parents, device="cuda") < 0, 0, pos[torch.tensor(parents, device="cuda").clamp(min=0)])
+                dec.reserve(128)
+            if captured:
+                for buf, x in zip(dec.static_buffers, (q, k, v)):
+                    buf.copy_(x)
+                dec.replay()
+                outs.append(dec.static_buffers[3].clone())
+            else:
+                outs.append(dec.step(q, k, v, positions=pos, len_hint=20))
+            pos = pos + 1
+            if captured:
+                assert dec.positions.tolist() == pos.tolist()
+        runs.append(outs + [d.k.clone() for d in dec.dense])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+    assert _lib.device_error() == 0
