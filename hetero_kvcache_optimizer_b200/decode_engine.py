@@ -191,11 +191,15 @@ class TieredKVDecoder:
                    adjacent: bool = False) -> None:
         """Steps that are given positions take queries and keys before their norm
         and rotation: ``kvstore.norm_rope`` with ``table`` and the layers' head-norm
-        weights (None: no norm) runs ahead of each layer's append."""
+        weights (None: no norm) runs ahead of each layer's append. A step captured
+        with positions holds the addresses of the table and weights before and is
+        dropped: ``capture`` again."""
         for w in (q_weights, k_weights):
             if w is not None and len(w) != self.num_layers:
                 raise ValueError(f"set_rotary needs {self.num_layers} weights, one per layer")
         self._rotary = (table, q_weights, k_weights, eps, adjacent)
+        if self.positions is not None:
+            self.graph = self.positions = None
 
     def _ready(self, layer: int, q: torch.Tensor, k_new: torch.Tensor, positions: Optional[torch.Tensor]):
         if positions is None:
@@ -404,7 +408,7 @@ class TieredKVDecoder:
 
     def replay(self) -> None:
         if self.graph is None:
-            raise RuntimeError("replay needs a captured step (capture; attach_prefix drops it)")
+            raise RuntimeError("replay needs a captured step (capture; attach_prefix and set_rotary drop it)")
         self._check_context()
         self.graph.replay()
         self.body_len += 1

@@ -117,3 +117,17 @@ def test_positions_of_a_captured_step_follow_the_fork(dec):
     dec.fork(torch.tensor([1, 1, 1, -1, 0, 9], dtype=torch.int32))
     assert dec.positions.tolist() == [7, 7, 7, 0, 300, 0]
     assert dec.positions.data_ptr() == address  # the graph's own buffer
+
+
+def test_another_rotation_drops_the_step_captured_with_the_old_one(dec):
+    class Graph:
+        def replay(self):
+            pass
+    dec.graph, dec.positions = Graph(), None  # captured without positions: holds no table
+    dec.set_rotary(torch.zeros(8, 128))
+    dec.replay()
+    dec.positions = torch.zeros(6, dtype=torch.int32)
+    dec.set_rotary(torch.zeros(16, 128))
+    with pytest.raises(RuntimeError, match="captured"):
+        dec.replay()
+    assert dec.positions is None
