@@ -804,8 +804,6 @@ def decode_shared(q: torch.Tensor, prefix: SharedPrefix, store: Optional[Int4KVS
     squeeze = q.dim() == 4
     if squeeze:
         q = q[:, :, 0]
-    if q.stride(2) != 1:
-        q = q.contiguous()
     B, Hq, D = q.shape
     Hkv = prefix.store.kv_heads
     for seg in (store, dense):
@@ -821,6 +819,8 @@ def decode_shared(q: torch.Tensor, prefix: SharedPrefix, store: Optional[Int4KVS
     if out is not None and (out.shape != q.shape or out.stride(2) != 1 or out.device != q.device):
         raise ValueError("out must be [B, Hq, 128] on q's device with a contiguous head dimension")
     with launch_on(q.device, stream):
+        if q.stride(2) != 1:  # behind whatever the stream still does to q
+            q = q.contiguous()
         if out is None:
             out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
         G = Hq // Hkv
