@@ -1513,7 +1513,7 @@ hkv_status hkv_pages_reserve(const hkv_int4_store* store, int32_t B, int32_t H, 
   if (!refs || tokens < 0) return HKV_ERR_ARG;
   if (!workspace || !aligned16(workspace) || workspace_bytes < 4 * pages_words(store, B, H)) return HKV_ERR_CAPACITY;
   if (tokens == 0) return HKV_OK;
-  // more than a row holds is wanted: the entries behind the row's end are flagged
+  // a row that is too short for its sequence's tokens is flagged on the device
   const int64_t per = std::min<int64_t>(cdiv(tokens, store->page_tokens) + 1, store->max_pages);
   if ((int64_t)tokens > (int64_t)store->max_pages * store->page_tokens) return HKV_ERR_CAPACITY;
   hkv::PagesParams p;

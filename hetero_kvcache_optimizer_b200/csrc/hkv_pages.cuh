@@ -140,13 +140,9 @@ __global__ void __launch_bounds__(kPgThreads) pages_reserve_map_kernel(const __g
     const int64_t extra = min((int64_t)p.extra, max((int64_t)0, p.extra_of ? (int64_t)p.extra_of[b] : (int64_t)p.extra));
     const int i = len / p.page_tokens + j;
     const int64_t end = ((int64_t)len + extra + p.page_tokens - 1) / p.page_tokens;  // pages held afterwards
-    bool wants = i < end;
-    if (wants && i >= p.max_pages) {
-      hkv_flag_error(HKV_DEVERR_CAPACITY);
-      wants = false;
-    }
+    if (j == 0 && end > p.max_pages) hkv_flag_error(HKV_DEVERR_CAPACITY);  // the row is too short for the last ones
     const int64_t at = (int64_t)u * p.max_pages + i;
-    p.want[k] = wants && p.table[at] < 0 ? (int)at : -1;
+    p.want[k] = i < min(end, (int64_t)p.max_pages) && p.table[at] < 0 ? (int)at : -1;
     p.from[k] = -1;
     p.vecs[k] = 0;
   }

@@ -68,3 +68,24 @@ def test_compact_copies_a_page_that_any_sequence_uses(kv, PagePool, L, lengths, 
     refs = np.zeros(16, np.int64)
     np.add.at(refs, table[table >= 0], 1)
     assert into.refs.tolist() == refs.tolist()
+
+
+@pytest.mark.parametrize("held,tokens,short", [(10, 502, False), (10, 503, True), (10, 512, True), (0, 512, False), (1, 512, True),
+                                               (128, 384, False), (128, 385, True), (512, 1, True), (511, 1, False), (600, 1, True)])
+@pytest.mark.parametrize("lowered", [False, True])
+def test_reserve_beyond_a_rows_end_is_flagged(kv, PagePool, L, held, tokens, short, lowered):
+    """Rows of 4 pages: the entries that exist get pages, and what does not fit sets
+    DEVERR_CAPACITY, however far behind the row's end it lies."""
+    n = min(4, -(-held // P))
+    table = [list(range(n)) + [-1] * (4 - n), [-1] * 4]
+    pool = pool_of(kv, PagePool, table, [held, 0], 1, 12)
+    if lowered:
+        pool.reserve(512, torch.tensor([tokens, 0]))
+    else:
+        pool.reserve(tokens)
+    assert L.device_error() == (L.DEVERR_CAPACITY if short else 0)
+    full = min(4, -(-(held + tokens) // P))
+    got = pool.store.page_table.tolist()
+    assert got[0] == list(range(full)) + [-1] * (4 - full)
+    assert (sum(x >= 0 for x in got[1]) == (0 if lowered else -(-tokens // P)))
+    assert pool.refs.tolist() == [int(i < sum(x >= 0 for r in got for x in r)) for i in range(12)]
