@@ -111,6 +111,7 @@ SIGNATURES = {
                                                  c_i32]),
     "hkv_decode_shared": (c_i32, [c_vp, c_i32, c_i64, c_i64, P_store, P_i32, P_i32, c_i32, P_store, P_dense, c_i32, c_i32,
                                   c_i32, c_i32, c_f32, c_i32, c_vp, c_sz, c_vp, c_i32, c_i64, c_i64, c_vp]),
+    "hkv_put_i32": (c_i32, [P_i32, c_i32, c_vp, c_vp]),
     "hkv_pages_workspace_bytes": (c_sz, [P_store, c_i32, c_i32]),
     "hkv_pages_fork": (c_i32, [P_store, c_i32, c_i32, c_vp, c_vp, c_vp, c_sz, c_vp]),
     "hkv_pages_reserve": (c_i32, [P_store, c_i32, c_i32, c_vp, c_i32, c_vp, c_vp, c_sz, c_vp]),

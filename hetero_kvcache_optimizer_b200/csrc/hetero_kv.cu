@@ -1486,6 +1486,20 @@ size_t hkv_pages_workspace_bytes(const hkv_int4_store* store, int32_t B, int32_t
   return check_paged(store, B, H) == HKV_OK ? 4 * pages_words(store, B, H) : 0;
 }
 
+hkv_status hkv_put_i32(const int32_t* values, int32_t n, int32_t* dst, hkv_stream_t stream) {
+  if (n < 0 || (n > 0 && (!values || !dst || (reinterpret_cast<uintptr_t>(dst) & 3)))) return HKV_ERR_ARG;
+  hkv::PutParams p;
+  for (int32_t i = 0; i < n; i += p.n) {
+    p.n = std::min(n - i, hkv::kPgPut);
+    p.dst = dst + i;
+    std::memcpy(p.v, values + i, sizeof(int32_t) * p.n);
+    hkv::put_i32_kernel<<<1, hkv::kPgThreads, 0, S(stream)>>>(p);
+    const hkv_status rc = launch_status();
+    if (rc != HKV_OK) return rc;
+  }
+  return HKV_OK;
+}
+
 hkv_status hkv_pages_fork(const hkv_int4_store* store, int32_t B, int32_t H, int32_t* refs, const int32_t* parents,
                           void* workspace, size_t workspace_bytes, hkv_stream_t stream) {
   hkv_status rc = check_paged(store, B, H);

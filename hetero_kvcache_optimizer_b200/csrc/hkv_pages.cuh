@@ -78,6 +78,19 @@ __device__ __forceinline__ int pg_scan(int v, int& total, int* s_warp) {
   return __shfl_sync(0xffffffffu, sum - x, w) + incl - v;
 }
 
+// ---------------------------------------------------------------- values from the host
+// They travel as kernel parameters: a copy from pageable memory would wait for the
+// stream, and could not be captured. Launch bound, 2.5 us.
+constexpr int kPgPut = 960;
+struct PutParams {
+  int32_t* dst;
+  int n;
+  int32_t v[kPgPut];
+};
+__global__ void __launch_bounds__(kPgThreads) put_i32_kernel(const __grid_constant__ PutParams p) {
+  for (int i = threadIdx.x; i < p.n; i += kPgThreads) p.dst[i] = p.v[i];
+}
+
 // ---------------------------------------------------------------- fork
 // Sequence b becomes sequence parents[b] as it was (all at once). The lowest b
 // with a given parent keeps the parent's row; the others share its full pages

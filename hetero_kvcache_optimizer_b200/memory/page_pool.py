@@ -3,9 +3,10 @@
 A page table alone says where a sequence's tokens lie; ``PagePool`` adds how many
 table entries name each page (``refs``), so that sequences can share pages (the
 samples of one prompt, the beams of a search), get new ones as they grow and
-give them back. No call reads anything back or waits for the device, so all of
-them can be captured in a CUDA graph beside the decode step; the same state
-always gives the same page ids (the lowest free ones, in table order).
+give them back. No call but ``free_pages`` reads anything back or waits for the
+device (lists from the host travel in a launch's parameters), so all of them can
+be captured in a CUDA graph beside the decode step; the same state always gives
+the same page ids (the lowest free ones, in table order).
 
 The reference keeps one cache per sequence and drops whole entries
 (src/memory/dram_storage.py:20-255, src/memory/manager.py:1231-1299); it has no
@@ -55,18 +56,27 @@ class PagePool:
                                         kv.raw_stream(self.refs.device)), name)
 
     def _per_sequence(self, x: Union[torch.Tensor, Sequence[int]], name: str) -> torch.Tensor:
-        if not isinstance(x, torch.Tensor):
-            x = torch.tensor(list(x), dtype=torch.int32)
-        if x.shape != (self.store.batch,) or x.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"{name} must be {self.store.batch} integers, one per sequence")
-        return x.to(device=self.store.pool.device, dtype=torch.int32).contiguous()
+        B = self.store.batch
+        if isinstance(x, torch.Tensor):
+            if x.shape != (B,) or x.dtype not in (torch.int32, torch.int64):
+                raise ValueError(f"{name} must be {B} integers, one per sequence")
+            if x.is_cuda:
+                return x.to(device=self.refs.device, dtype=torch.int32).contiguous()
+        values = [int(v) for v in (x.tolist() if isinstance(x, torch.Tensor) else x)]
+        if len(values) != B or any(not -2**31 <= v < 2**31 for v in values):
+            raise ValueError(f"{name} must be {B} integers, one per sequence")
+        with kv.launch_on(self.refs.device):
+            out = torch.empty(B, dtype=torch.int32, device=self.refs.device)
+            L.check(L.load().hkv_put_i32((ctypes.c_int32 * B)(*values), B, out.data_ptr(), kv.raw_stream(out.device)), "hkv_put_i32")
+        return out
 
     def fork(self, parents: Union[torch.Tensor, Sequence[int]], stream=None) -> None:
         """Sequence b becomes what sequence ``parents[b]`` was, for all b at once
         (sampling several continuations, reordering the beams of a search); -1
         empties it. Full pages are shared; a partly filled last page goes to the
         lowest b with that parent and is copied for the others. An int32 tensor
-        on the device is used as it is. Afterwards only tokens behind the lengths
+        on the device is used as it is (a captured fork reads it at each replay;
+        a list is kept as it was). Afterwards only tokens behind the lengths
         may be written: a sequence that is to be cut back into shared pages or
         filled anew is emptied (-1, ``free``) first."""
         with kv.launch_on(self.refs.device, stream):

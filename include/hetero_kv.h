@@ -489,6 +489,12 @@ hkv_status hkv_norm_rope(const hkv_rows* q, const hkv_rows* k, const hkv_rows* q
  * No counterpart in the reference (one cache per sequence, chunks never shared). */
 size_t hkv_pages_workspace_bytes(const hkv_int4_store* store, int32_t B, int32_t H);
 
+/* dst[i] = values[i] for i < n, with the values (a HOST array, read before the call
+ * returns) in the launches' own parameters: parents or token counts that the host
+ * has made reach the device in stream order, without a wait, and a captured call
+ * keeps them. */
+hkv_status hkv_put_i32(const int32_t* values, int32_t n, int32_t* dst, hkv_stream_t stream);
+
 /* Sequence b becomes what sequence parents[b] (device int32 [B]) was before the
  * call, for all b at once; -1 empties it. The lowest b with a given parent takes
  * over the parent's whole row of pages; the others share its full pages and get

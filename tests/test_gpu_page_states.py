@@ -89,3 +89,56 @@ def test_reserve_beyond_a_rows_end_is_flagged(kv, PagePool, L, held, tokens, sho
     assert got[0] == list(range(full)) + [-1] * (4 - full)
     assert (sum(x >= 0 for x in got[1]) == (0 if lowered else -(-tokens // P)))
     assert pool.refs.tolist() == [int(i < sum(x >= 0 for r in got for x in r)) for i in range(12)]
+
+
+def test_lists_from_the_host_do_not_wait_and_are_captured(kv, PagePool, L):
+    """free, fork and reserve with plain lists (and tensors on the host): queued behind a
+    busy stream without waiting for it, captured with their values, the same state after."""
+    table = [[0, 1, -1, -1], [2, 3, 4, -1], [5, -1, -1, -1]]
+
+    def calls(pool):
+        pool.fork([1, 0, 0])
+        pool.reserve(200, torch.tensor([1, 200, 100]))
+        pool.free([2])
+        pool.fork(torch.tensor([0, 1, 1]))
+    plain, queued, graphed = (pool_of(kv, PagePool, table, [250, 300, 7], 1, 24) for _ in range(3))
+    calls(plain)
+    torch.cuda.synchronize()
+    done = torch.cuda.Event()
+    torch.cuda._sleep(400_000_000)  # about 0.2 s
+    calls(queued)
+    done.record()
+    assert not done.query()
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        calls(graphed)
+    torch.cuda.synchronize()
+    assert graphed.store.lengths.tolist() == [250, 300, 7]
+    torch.empty(1 << 20, device="cuda").fill_(1)  # whatever memory the calls' temporaries had
+    g.replay()
+    torch.cuda.synchronize()
+    for pool in (queued, graphed):
+        for a, b in ((pool.refs, plain.refs), (pool.store.page_table, plain.store.page_table), (pool.store.lengths, plain.store.lengths),
+                     (pool.store.pool, plain.store.pool)):
+            assert torch.equal(a, b)
+    assert L.device_error() == 0
+
+
+@pytest.mark.parametrize("n", [1, 255, 960, 961, 4000])
+def test_many_values_from_the_host(L, n):
+    import ctypes
+    dst = torch.full((n + 1,), 7, dtype=torch.int32, device="cuda")
+    values = [(i * 2654435761) % 2**32 - 2**31 for i in range(n)]
+    host = (ctypes.c_int32 * n)(*values)
+    L.check(L.load().hkv_put_i32(host, n, dst.data_ptr(), torch.cuda.current_stream().cuda_stream), "hkv_put_i32")
+    ctypes.memset(host, 0, 4 * n)  # read before the call returned
+    assert dst.tolist() == values + [7]
+
+
+def test_lists_of_another_length_or_range_are_refused(kv, PagePool):
+    pool = pool_of(kv, PagePool, [[0], [1]], [5, 5], 1, 4)
+    for bad in ([0], [0, 1, 2], [0, 2**31], [-2**31 - 1, 0], torch.tensor([0, 2**40])):
+        with pytest.raises(ValueError):
+            pool.fork(bad)
+        with pytest.raises(ValueError):
+            pool.reserve(1, bad)
