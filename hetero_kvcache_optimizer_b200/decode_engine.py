@@ -278,10 +278,12 @@ class TieredKVDecoder:
     def capture(self, max_steps: int, positions: Optional[torch.Tensor] = None) -> None:
         """Capture one decode step over static input/output buffers. The split
         grid is sized for a body of ``body_len + max_steps`` tokens; device-side
-        lengths keep replays exact as the body grows. ``positions`` (after
+        lengths keep replays exact as the body grows. Steps captured before
+        (``capture_host``'s too) are dropped. ``positions`` (after
         ``set_rotary``): the positions of the first step's tokens; the captured
         step norms and rotates its queries and keys and moves ``self.positions``
         on by one."""
+        self.graph = self.host_graph = self._host = None  # they hold the buffers that are replaced here
         Lyr, B = self.num_layers, self.batch
         q = torch.zeros(Lyr, B, self.q_heads, 128, dtype=torch.bfloat16, device=self.device)
         kn = torch.zeros(Lyr, B, self.kv_heads, 128, dtype=self.kv_dtype, device=self.device)

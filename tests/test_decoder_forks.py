@@ -131,3 +131,13 @@ def test_another_rotation_drops_the_step_captured_with_the_old_one(dec):
     with pytest.raises(RuntimeError, match="captured"):
         dec.replay()
     assert dec.positions is None
+
+
+def test_a_new_capture_drops_the_steps_over_the_buffers_it_replaces(dec, monkeypatch):
+    def stream(*a, **k):
+        raise Reached
+    monkeypatch.setattr(torch.cuda, "Stream", stream)
+    dec.graph = dec.host_graph = dec._host = object()
+    with pytest.raises(Reached):
+        dec.capture(4)
+    assert dec.graph is None and dec.host_graph is None and dec.host_buffers is None

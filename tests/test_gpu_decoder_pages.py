@@ -85,3 +85,30 @@ def test_a_captured_step_goes_on_from_its_parents_positions():
         runs.append(outs + [d.k.clone() for d in dec.dense])
     assert all(torch.equal(a, b) for a, b in zip(*runs))
     assert _lib.device_error() == 0
+
+
+def test_host_steps_after_a_second_capture():
+    """The host buffers of the first capture still serve as plain inputs; their graph is gone."""
+    runs = []
+    for again in (False, True):
+        gen = torch.Generator(device="cuda").manual_seed(8)
+        dec = decoder(2)
+        for l in range(2):
+            dec.prefill_layer(l, *(torch.randn(3, 2, 8 + 200, 128, generator=gen, device="cuda").to(BF16) for _ in range(2)))
+        dec.reserve(128)
+        dec.capture(8)
+        dec.capture_host()
+        bufs = dec.host_buffers
+        if again:
+            dec.capture(8)
+            assert dec.host_buffers is None
+        outs = []
+        for _ in range(3):
+            for b, n in zip(bufs, (8, 2, 2)):
+                b.copy_(torch.randn(2, 3, n, 128, generator=gen, device="cuda"))
+            torch.cuda.synchronize()
+            dec.step_host(*bufs)
+            torch.cuda.synchronize()
+            outs.append(bufs[3].clone())
+        runs.append(outs)
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
