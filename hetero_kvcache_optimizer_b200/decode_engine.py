@@ -282,7 +282,7 @@ class TieredKVDecoder:
         (``capture_host``'s too) are dropped. ``positions`` (after
         ``set_rotary``): the positions of the first step's tokens; the captured
         step norms and rotates its queries and keys and moves ``self.positions``
-        on by one."""
+        on by one (negative ones, sequences that pad the batch, stay)."""
         self.graph = self.host_graph = self._host = None  # they hold the buffers that are replaced here
         Lyr, B = self.num_layers, self.batch
         q = torch.zeros(Lyr, B, self.q_heads, 128, dtype=torch.bfloat16, device=self.device)
@@ -310,7 +310,7 @@ class TieredKVDecoder:
         with torch.cuda.graph(g, stream=s):
             run()
             if self.positions is not None:
-                self.positions += 1
+                self.positions += self.positions >= 0  # a sequence that pads the batch stays one
         torch.cuda.current_stream(self.device).wait_stream(s)
         self.graph = g
         self._static = (q, kn, vn, out)

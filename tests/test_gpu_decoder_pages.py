@@ -112,3 +112,36 @@ def test_host_steps_after_a_second_capture():
             outs.append(bufs[3].clone())
         runs.append(outs)
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_a_padded_batch_stays_padded_in_a_captured_step():
+    """A sequence of negative position pads the batch at every replay; the others go on
+    as eager steps with the same positions do."""
+    from hetero_kvcache_optimizer_b200 import _lib, kvstore as kv
+    _lib.device_error(clear=True)
+    runs = []
+    for captured in (True, False):
+        gen = torch.Generator(device="cuda").manual_seed(9)
+        dec = decoder(2)
+        dec.set_rotary(kv.rope_table(64, 128))
+        dec.reserve(128)
+        pos = torch.tensor([5, -3, 40], dtype=torch.int32, device="cuda")
+        if captured:
+            dec.capture(12, positions=pos)
+        outs = []
+        for step in range(12):
+            q = torch.randn(2, 3, 8, 128, generator=gen, device="cuda").to(BF16)
+            k, v = (torch.randn(2, 3, 2, 128, generator=gen, device="cuda").to(BF16) for _ in range(2))
+            if captured:
+                for buf, x in zip(dec.static_buffers, (q, k, v)):
+                    buf.copy_(x)
+                dec.replay()
+                outs.append(dec.static_buffers[3][:, [0, 2]])
+            else:
+                outs.append(dec.step(q, k, v, positions=pos, len_hint=12)[:, [0, 2]])
+            pos = torch.where(pos < 0, pos, pos + 1)
+            if captured:
+                assert dec.positions.tolist() == pos.tolist()
+        runs.append(outs)
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+    assert _lib.device_error() == 0
