@@ -61,6 +61,8 @@ class PagePool:
             if x.shape != (B,) or x.dtype not in (torch.int32, torch.int64):
                 raise ValueError(f"{name} must be {B} integers, one per sequence")
             if x.is_cuda:
+                if x.dtype == torch.int64:  # out of range stays out of range
+                    x = x.clamp(-2**31, 2**31 - 1)
                 return x.to(device=self.refs.device, dtype=torch.int32).contiguous()
         values = [int(v) for v in (x.tolist() if isinstance(x, torch.Tensor) else x)]
         if len(values) != B or any(not -2**31 <= v < 2**31 for v in values):

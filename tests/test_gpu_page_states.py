@@ -142,3 +142,16 @@ def test_lists_of_another_length_or_range_are_refused(kv, PagePool):
             pool.fork(bad)
         with pytest.raises(ValueError):
             pool.reserve(1, bad)
+
+
+def test_wide_integers_on_the_device_are_not_cut_down(kv, PagePool, L):
+    """Parents beyond 32 bits are outside the batch like any other, and counts beyond them
+    lower nothing."""
+    pool = pool_of(kv, PagePool, [[0, -1, -1], [1, -1, -1], [2, -1, -1]], [100, 90, 80], 1, 12)
+    pool.reserve(200, torch.tensor([2**32, -2**32, 2**33 + 5], device="cuda"))
+    assert L.device_error() == 0
+    assert pool.store.page_table.tolist() == [[0, 3, 4], [1, -1, -1], [2, 5, 6]]
+    pool.fork(torch.tensor([2**32, 1, -2**32 + 2], device="cuda"))
+    assert L.device_error() == L.DEVERR_BAD_PAGE
+    assert pool.store.lengths.tolist() == [0, 90, 0]
+    assert pool.store.page_table.tolist() == [[-1] * 3, [1, -1, -1], [-1] * 3]
