@@ -11,9 +11,9 @@
 // the rows as M, 32 of them would cost 128, and the exponentials would sit in one
 // warp). The running max m and the sum of P are fp32; m moves only when a score
 // beats it by more than 2^8. K, V and P are rounded to f16, the type of their MMA:
-// K and V where they are dequantised (2^-11 relative, ref's f32 scale rounded as
-// well), P in (0, 2^8]; with key channels ten times as large as the rest that
-// leaves the output 5e-4 (fp16min) to 1.7e-3 (ref) off in the 2-norm, 3e-4 without.
+// K and V where they are dequantised (2^-11 relative; ref's f32 scale enters K as the
+// sum of two f16 and V rounded), P in (0, 2^8]; with key channels ten times as large
+// as the rest that leaves the output 5e-4 (fp16min) to 1e-3 (ref) off in the 2-norm.
 //
 // A grid of p.C persistent CTAs; every (group, KV head, row tile) unit's 128-token
 // tiles, with a charge of kShCharge tiles per unit for a piece's start and end,
@@ -275,15 +275,16 @@ __device__ __forceinline__ void sh_convert_k(const uint8_t* rb, uint32_t tmem, i
 #pragma unroll
     for (int w2 = 0; w2 < 2; ++w2) {  // dims 32 w .. + 31
       const int w = 2 * half + w2, g = w * 32 / GROUP;
-      __half2 s2, m2;
+      __half2 s2, m2;  // ref: the f32 scale as the sum of two f16
       uint32_t zlo = 0, zhi = 0;
       if constexpr (FMT == HKV_FMT_FP16MIN) {
         s2 = __half2half2(ks[g]);
         m2 = __half2half2(km[g]);
       } else {
         const uint32_t z = meta[1024 * NG + t * NG + g];
-        s2 = __float2half2_rn(reinterpret_cast<const float*>(meta)[t * NG + g]);
-        m2 = __float2half2_rn(0.f);
+        const float s = reinterpret_cast<const float*>(meta)[t * NG + g];
+        s2 = __float2half2_rn(s);
+        m2 = __float2half2_rn(s - __low2float(s2));
         zlo = h2u(__float2half2_rn(1024.f + (float)z));
         zhi = h2u(__float2half2_rn(-64.f - (float)z));
       }
@@ -294,7 +295,8 @@ __device__ __forceinline__ void sh_convert_k(const uint8_t* rb, uint32_t tmem, i
         if constexpr (FMT == HKV_FMT_FP16MIN) nib8_to_h2(v[j][w], h);
         else nib8_to_h2_z(v[j][w], zlo, zhi, h);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[16 * w2 + 4 * j + c] = h2u(__hfma2(u2h(h[c]), s2, m2));
+        for (int c = 0; c < 4; ++c)
+          o[16 * w2 + 4 * j + c] = h2u(__hfma2(u2h(h[c]), s2, FMT == HKV_FMT_FP16MIN ? m2 : __hmul2(u2h(h[c]), m2)));
       }
     }
     tm_st32u(tmem + 32 * half, o);
@@ -748,10 +750,15 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
 //     instruction per pair; the accumulator starts at -1024 sum q, exact as the
 //     products are; the group's scale multiplies in fp32 afterwards; fp16min's mins
 //     are one more product, against sum q_d in f16 high and low parts;
-//   O^T += (n V^T) (s_g P)^T: the codes as exact integers, their scale in P's operand
-//     (rounded to f16 with it), fp16min's mins one more product into an accumulator
-//     of its own. The ref format's zero points enter as z sum q_d and as n - z.
-// So nothing of K is rounded, and no operand crosses shared memory twice. Two groups
+//   O^T += (n V^T) (s_g P)^T: the codes as exact integers, their scale in P's operand:
+//     fp16min's times P in f16 (2^-11 each), its mins one more product with the same P
+//     into an accumulator of its own; ref's f32 scale times P in fp32, as two f16 and
+//     two products (shared 4: 17.9 us with the scale rounded to f16, 17.5 so). The ref
+//     format's zero points enter as z sum q_d and as n - z.
+// So nothing of K is rounded, and no operand crosses shared memory twice. Against 64
+// bits, outliers of ten times the rest among the key channels, 1,000 tokens: fp16min
+// 1.1e-4 to 1.7e-4 of the output in the 2-norm, ref 2e-5 (group 32) to 1e-4 (128; the
+// sums of 1024 + n in fp32); with ref's scale rounded 2.3e-4 to 2.6e-4. Two groups
 // of four consumer warps take every second tile, 32 tokens a warp.
 constexpr int kRowsThreads = 320;  // 8 consumer warps, 2 producers
 constexpr int kRowsSlots = 6;
@@ -1034,7 +1041,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1) shared_rows_kernel(const __gr
               zc[b][e] *= a, zc[b][e + 2] *= a;
             }
         }
-        uint32_t pt[2][NB][2];  // P / 16 (below f16's largest) in f16, transposed: row r, tokens 2 j4, 2 j4 + 1 (+ 8)
+        // x becomes P / 16 (its f16 stays below the largest); fp16min: in f16, transposed:
+        // row r, tokens 2 j4, 2 j4 + 1 (+ 8)
+        uint32_t pt[2][NB][2];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
           const float m0 = m[b][0] + 4.f, m1 = m[b][1] + 4.f;
@@ -1045,15 +1054,18 @@ __global__ void __launch_bounds__(kRowsThreads, 1) shared_rows_kernel(const __gr
             xx[2] = fast_exp2(xx[2] - m0), xx[3] = fast_exp2(xx[3] - m1);
             l[b][0] += xx[0] + xx[2];
             l[b][1] += xx[1] + xx[3];
-            pt[s2][b][0] = movmatrix_t(pack2<__half>(xx[0], xx[1]));
-            pt[s2][b][1] = movmatrix_t(pack2<__half>(xx[2], xx[3]));
+            if constexpr (FMT == HKV_FMT_FP16MIN) {
+              pt[s2][b][0] = movmatrix_t(pack2<__half>(xx[0], xx[1]));
+              pt[s2][b][1] = movmatrix_t(pack2<__half>(xx[2], xx[3]));
+            }
           }
         }
         // ---- O^T += V^T P^T
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) {
           const int q0 = (t0 + 16 * s2) / 2, left = nv - 16 * s2;  // the subtile's first pair; its tokens in use
-          uint32_t vs[2][NG], vz[2][NG];  // pairs j4 and 4 + j4: scales; ref: zero points
+          uint32_t vs[2][NG], vz[2][NG];  // pairs j4 and 4 + j4: fp16min's scales; ref's zero points
+          float vf[2][NG];                // ref: scales of tokens r and r + 8
           uint32_t zmin[2] = {0u, 0u};
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
@@ -1062,15 +1074,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1) shared_rows_kernel(const __gr
               ld_row_u<NG>(reinterpret_cast<const uint32_t*>(meta + 512 * NG), q, vs[e]);
               zmin[e] = r < NG ? reinterpret_cast<const uint32_t*>(meta + 768 * NG)[q * NG + r] : 0u;
             } else {
-              float fa[NG], fb[NG];
-              ld_row<NG>(reinterpret_cast<const float*>(meta + 512 * NG), 2 * q, fa);
-              ld_row<NG>(reinterpret_cast<const float*>(meta + 512 * NG), 2 * q + 1, fb);
+              ld_row<NG>(reinterpret_cast<const float*>(meta + 512 * NG), 2 * q0 + 8 * e + r, vf[e]);
               const uint8_t* zp = meta + 1152 * NG + 2 * q * NG;
 #pragma unroll
-              for (int g = 0; g < NG; ++g) {
-                vs[e][g] = pack2<__half>(fa[g], fb[g]);
-                vz[e][g] = (uint32_t)zp[g] | ((uint32_t)zp[NG + g] << 16);
-              }
+              for (int g = 0; g < NG; ++g) vz[e][g] = (uint32_t)zp[g] | ((uint32_t)zp[NG + g] << 16);
             }
           }
           if (left < 16) {  // unused tokens' metadata may be any bits: P = 0 has to meet 0
@@ -1080,7 +1087,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1) shared_rows_kernel(const __gr
               const uint32_t keep = (tk < left ? 0x0000FFFFu : 0u) | (tk + 1 < left ? 0xFFFF0000u : 0u);
               zmin[e] &= keep;
 #pragma unroll
-              for (int g = 0; g < NG; ++g) vs[e][g] &= keep;
+              for (int g = 0; g < NG; ++g) {
+                if constexpr (FMT == HKV_FMT_FP16MIN) vs[e][g] &= keep;
+                else vf[e][g] = 8 * e + r < left ? vf[e][g] : 0.f;
+              }
             }
           }
           if constexpr (FMT == HKV_FMT_FP16MIN) {
@@ -1094,9 +1104,28 @@ __global__ void __launch_bounds__(kRowsThreads, 1) shared_rows_kernel(const __gr
             const uint4 c4 = *reinterpret_cast<const uint4*>(blk + HKV_V_CODES_OFF + v_chunk_off(q0 + 4 * e + j4, r));
             vw[e][0] = c4.x, vw[e][1] = c4.y, vw[e][2] = c4.z, vw[e][3] = c4.w;
           }
+          // the codes' other operand, P times the group's scale: fp16min's f16 scale times P as
+          // it meets the mins; ref's f32 scale as two f16, the second what the first leaves
+          uint32_t ph[NB][2], pl[NB][2];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int g = k / WPG;
+            if (k % WPG == 0) {
+#pragma unroll
+              for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  if constexpr (FMT == HKV_FMT_FP16MIN) {
+                    ph[b][e] = hmul2(pt[s2][b][e], vs[e][g]);
+                  } else {
+                    const float2 y = __fmul2_rn(make_float2(x[s2][b][2 * e], x[s2][b][2 * e + 1]), make_float2(vf[e][g], vf[e][g]));
+                    const uint32_t hi = pack2<__half>(y.x, y.y);
+                    const float2 z = __half22float2(u2h(hi));
+                    ph[b][e] = movmatrix_t(hi);
+                    pl[b][e] = movmatrix_t(pack2<__half>(y.x - z.x, y.y - z.y));
+                  }
+                }
+            }
             uint32_t ha[4], hb[4];
             if constexpr (FMT == HKV_FMT_REF) {  // 1024 + z and -64 - z in f16 are one addition to the bits
               nib8_to_h2_z(vw[0][k], 0x64006400u + vz[0][g], 0xD400D400u + 16u * vz[0][g], ha);
@@ -1108,9 +1137,12 @@ __global__ void __launch_bounds__(kRowsThreads, 1) shared_rows_kernel(const __gr
             const uint32_t a0[4] = {ha[0], ha[1], hb[0], hb[1]}, a1[4] = {ha[2], ha[3], hb[2], hb[3]};
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-              const uint32_t p0 = hmul2(pt[s2][b][0], vs[0][g]), p1 = hmul2(pt[s2][b][1], vs[1][g]);
-              mma16816<__half>(o[b][2 * k], a0, p0, p1);
-              mma16816<__half>(o[b][2 * k + 1], a1, p0, p1);
+              mma16816<__half>(o[b][2 * k], a0, ph[b][0], ph[b][1]);
+              mma16816<__half>(o[b][2 * k + 1], a1, ph[b][0], ph[b][1]);
+              if constexpr (FMT == HKV_FMT_REF) {
+                mma16816<__half>(o[b][2 * k], a0, pl[b][0], pl[b][1]);
+                mma16816<__half>(o[b][2 * k + 1], a1, pl[b][0], pl[b][1]);
+              }
             }
           }
         }
