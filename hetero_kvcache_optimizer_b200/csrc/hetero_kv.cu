@@ -612,7 +612,7 @@ struct SharedPlan {
   size_t own_ws, own_o, own_ml, part_o, part_ml, bytes;  // sizes and offsets
 };
 hkv_status shared_plan(const hkv_int4_store* prefix, const int32_t* start, const int32_t* lens, int P, const hkv_int4_store* body,
-                       const hkv_dense_kv* dense, int B, int Hq, int Hkv, int D, int ctas, SharedPlan* out) {
+                       const hkv_dense_kv* dense, int B, int Hq, int Hkv, int D, int ctas, bool exact, SharedPlan* out) {
   const hkv_status rc = check_store(prefix);
   if (rc != HKV_OK) return rc;
   if (!start || P <= 0 || B <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv) return HKV_ERR_ARG;
@@ -628,8 +628,13 @@ hkv_status shared_plan(const hkv_int4_store* prefix, const int32_t* start, const
   // Rows of a unit that share its dequantised tiles: the narrowest product that holds the
   // largest group. 65,536 tokens of 8 heads: 16 rows 35.3 us on shared_rows_kernel (40.1 on a
   // 16-row shared_prefix_kernel; 32 rows there 58.2 against 44.3), 64 rows 55.3 (as 128: 74),
-  // 128 rows 74.1, 256 as two row tiles 127.8.
-  pl.N = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  // 128 rows 74.1, 256 as two row tiles 127.8. Wide products round K, V and P to f16: their
+  // result is 4e-4 to 1.2e-3 off in the 2-norm, which a bf16 output's own 1.7e-3 covers (1.8e-3
+  // to 1.9e-3 in all) and an f16 one's 2.1e-4 does not. f16 and f32 outputs (`exact`) therefore
+  // take row tiles of 16 on shared_rows_kernel (2e-5 to 1.9e-4) at every width: 31,680 tokens of
+  // 8 heads, bf16 against f32 outputs, 32 rows 36-39 and 45 us, 64 rows 48 and 76, 128 rows 60
+  // and 136; 256 rows over 65,536 tokens 172 and 495.
+  pl.N = rows <= 16 || exact ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
   pl.ns = pl.N == 16 ? 1 : hkv::sh_streams(pl.N);
   const int all = std::min(ctas > 0 ? ctas : device_sms(), 65535);
   int64_t units = 0, steps = 0, hint_steps = 0;
@@ -1585,8 +1590,11 @@ size_t hkv_decode_shared_workspace_bytes(const hkv_int4_store* prefix, const int
                                          const int32_t* group_len, int32_t n_groups,
                                          const hkv_int4_store* body, const hkv_dense_kv* dense, int32_t B,
                                          int32_t Hq, int32_t Hkv, int32_t D, int32_t ctas) {
-  SharedPlan pl;
-  return shared_plan(prefix, group_start, group_len, n_groups, body, dense, B, Hq, Hkv, D, ctas, &pl) == HKV_OK ? pl.bytes : 0;
+  SharedPlan pl, pe;
+  if (shared_plan(prefix, group_start, group_len, n_groups, body, dense, B, Hq, Hkv, D, ctas, false, &pl) != HKV_OK ||
+      shared_plan(prefix, group_start, group_len, n_groups, body, dense, B, Hq, Hkv, D, ctas, true, &pe) != HKV_OK)
+    return 0;
+  return std::max(pl.bytes, pe.bytes);
 }
 
 hkv_status hkv_decode_shared(const void* q, int32_t q_dtype, int64_t q_stride_b, int64_t q_stride_h,
@@ -1599,7 +1607,7 @@ hkv_status hkv_decode_shared(const void* q, int32_t q_dtype, int64_t q_stride_b,
   if (out_dtype < HKV_DT_F16 || out_dtype > HKV_DT_F32) return HKV_ERR_ARG;
   if (!(sm_scale > 0.f) || !std::isfinite(sm_scale)) return HKV_ERR_ARG;
   SharedPlan pl;
-  hkv_status rc = shared_plan(prefix, group_start, group_len, n_groups, body, dense, B, Hq, Hkv, D, ctas, &pl);
+  hkv_status rc = shared_plan(prefix, group_start, group_len, n_groups, body, dense, B, Hq, Hkv, D, ctas, out_dtype != HKV_DT_BF16, &pl);
   if (rc != HKV_OK) return rc;
   if (!workspace || workspace_bytes < pl.bytes || !aligned16(workspace)) return HKV_ERR_CAPACITY;
   uint8_t* ws = static_cast<uint8_t*>(workspace);

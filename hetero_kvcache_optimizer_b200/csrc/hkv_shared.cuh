@@ -4,7 +4,7 @@
 // A group of n sequences has one prefix; per KV head its n G query heads are the
 // columns of ONE product over the prefix's tokens, so the packed pages are read
 // and dequantised once per row tile of N = 32, 64 or 128 rows instead of once per
-// sequence (at most 16 rows: shared_rows_kernel below):
+// sequence (at most 16 rows, and outputs finer than bf16: shared_rows_kernel below):
 //   S^T[token][row] = K Q^T,  P = 2^(S qscale - m),  O^T[dim][row] += V^T P
 // on tcgen05 with the tokens (then the dims) as the MMA's M = 128 and the rows as
 // its N: a decode batch has few rows, and this way they cost what they are (with
@@ -13,7 +13,8 @@
 // beats it by more than 2^8. K, V and P are rounded to f16, the type of their MMA:
 // K and V where they are dequantised (2^-11 relative; ref's f32 scale enters K as the
 // sum of two f16 and V rounded), P in (0, 2^8]; with key channels ten times as large
-// as the rest that leaves the output 5e-4 (fp16min) to 1e-3 (ref) off in the 2-norm.
+// as the rest that leaves the output 5e-4 (fp16min) to 1.2e-3 (ref) off in the 2-norm,
+// below the 1.7e-3 of a bf16 output's own rounding; other outputs do not come here.
 //
 // A grid of p.C persistent CTAs; every (group, KV head, row tile) unit's 128-token
 // tiles, with a charge of kShCharge tiles per unit for a piece's start and end,
@@ -741,8 +742,8 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
   }
 }
 
-// ---------------------------------------------------------------- few rows
-// The same partials for at most 16 rows on mma.sync (m16n8k16), tokens as M, two
+// ---------------------------------------------------------------- 16 rows a time, unrounded codes
+// The same partials for row tiles of at most 16 rows on mma.sync (m16n8k16), tokens as M, two
 // column blocks of 8 rows. Few rows are bound by unpacking the codes, and here they
 // meet the tensor cores almost as they are stored:
 //   S = sum_g s_g (sum_{d in g} (1024 + n_d) q_d - 1024 sum q_d) + sum_g min_g sum q_d:
@@ -753,7 +754,7 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
 //   O^T += (n V^T) (s_g P)^T: the codes as exact integers, their scale in P's operand:
 //     fp16min's times P in f16 (2^-11 each), its mins one more product with the same P
 //     into an accumulator of its own; ref's f32 scale times P in fp32, as two f16 and
-//     two products (shared 4: 17.9 us with the scale rounded to f16, 17.5 so). The ref
+//     two products (4 samples of 1,000 tokens, G 7: 17.8 us with it rounded, 17.5 so). The ref
 //     format's zero points enter as z sum q_d and as n - z.
 // So nothing of K is rounded, and no operand crosses shared memory twice. Against 64
 // bits, outliers of ten times the rest among the key channels, 1,000 tokens: fp16min

@@ -124,7 +124,8 @@ class TieredKVDecoder:
     def attach_prefix(self, prefixes: Optional[Sequence[kv.SharedPrefix]]) -> None:
         """One shared prefix per layer (None: none), in front of what the layer's
         cache holds; it stays attached until replaced. Steps then append and run
-        ``kvstore.decode_shared``. A sequence's group is that of its slot in the
+        ``kvstore.decode_shared`` (large groups: fastest with ``out_dtype`` bfloat16).
+        A sequence's group is that of its slot in the
         batch: what the caches hold now is taken to belong behind it. A captured
         step is dropped: ``capture`` again."""
         if prefixes is not None:

@@ -797,7 +797,10 @@ def decode_shared(q: torch.Tensor, prefix: SharedPrefix, store: Optional[Int4KVS
     128]) over [prefix of the sequence's group ; its INT4 body ; its dense
     segment], each prefix read once per KV head for its whole group. ``store``
     and ``dense`` as in ``decode``, or None. Returns [B, Hq, 128] in
-    ``out_dtype``; a row that sees no token is zero."""
+    ``out_dtype``; a row that sees no token is zero. bfloat16 outputs are the
+    fastest for more than 16 rows (sequences x Hq / Hkv) a group: their own
+    rounding covers that of f16 keys, values and probabilities, which the other
+    types' form avoids (as ``decode`` does)."""
     _require_cuda(q)
     if q.dim() not in (3, 4) or (q.dim() == 4 and q.shape[2] != 1):
         raise ValueError("q must be [B, Hq, 128] or [B, Hq, 1, 128]")
