@@ -689,11 +689,13 @@ cudaError_t launch_norm_rope(hkv::NormRopeParams& p, cudaStream_t st) {
 
 template <typename T>
 cudaError_t launch_norm_rope_t(hkv::NormRopeParams& p, int mode, cudaStream_t st) {
-  // Two heads a warp while that leaves warps to spare (320 rows: 2.9 us against 3.6 with
-  // eight), else eight (all heads of a token in one warp, their loads ahead of their work,
-  // saves the table's re-reads and costs resident warps: 124.7 us against 124.2 for
-  // 32,768 tokens of 40 heads).
-  const bool few = (int64_t)p.B * p.T * (p.H[0] + p.H[1]) <= (int64_t)device_sms() * 64;
+  // Two heads a warp while that leaves warps to spare (320 rows 2.35 us, 2.88 with eight;
+  // 7,080 rows 2.86 and 3.02), else eight (7,584 rows of 28 + 4 heads 3.19 us, 3.55 with two;
+  // 9,480 rows of 32 + 8 heads 3.37 and 3.73; 163,840 rows 20.4 and 32.2). Head counts of q
+  // or k that are no multiple of eight leave places empty (28 + 4 heads: 8 of 40). All heads
+  // of a token in one warp, their loads ahead of their work, save the table's re-reads and
+  // cost resident warps: 124.7 us against 124.2 for 32,768 tokens of 40 heads.
+  const bool few = (int64_t)p.B * p.T * (p.H[0] + p.H[1]) <= (int64_t)device_sms() * 48;
 #define HKV_NR(MODE) (few ? launch_norm_rope<T, MODE, 2>(p, st) : launch_norm_rope<T, MODE, 8>(p, st))
   return mode == hkv::kNrWhole ? HKV_NR(hkv::kNrWhole) : mode == hkv::kNrLane ? HKV_NR(hkv::kNrLane) : mode == hkv::kNrAdjacent ? HKV_NR(hkv::kNrAdjacent) : HKV_NR(hkv::kNrAny);
 #undef HKV_NR

@@ -18,7 +18,10 @@
 // it from the row again (L1).
 // Measured: 32,768 tokens of 32 + 8 heads 124 us = 5.5 TB/s (a kernel that only copies
 // the same rows: 107 us), 4,096 tokens of 28 + 4 heads 16.7 us, 8 tokens of 32 + 8
-// heads 2.5 us (a launch). 61 warp instructions a row keep 60 % of the issue slots busy.
+// heads 2.4 us (a launch). 61 warp instructions a row keep 60 % of the issue slots busy (76
+// with 28 + 4 heads, which leave 8 of 40 places empty). The other rotations of the 32,768
+// tokens: 64 of 128 dims by halves 150 us, 96 of 128 155, neighbours 137 (64) and 139 (128);
+// 50 of 128 by halves, read twice, 446.
 // The next launch is let in after this one's wait, so that it never runs beside
 // a grid two launches back.
 #pragma once
@@ -279,8 +282,9 @@ __device__ __forceinline__ void nr_rows(const NormRopeParams& p, int b, int t, i
   }
 }
 
-// Five CTAs an SM where 48 registers do (whole heads: 16.7 against 18.1 us for a chunk with
-// four, 124 against 133 for a prompt).
+// Five CTAs an SM for whole heads, although 48 registers spill a little with eight heads a
+// warp (96 bytes of stores, 24 of loads a thread): 16.7 against 18.1 us for a chunk with four
+// CTAs, 124 against 133 for a prompt.
 template <typename T, int MODE, int kHeads>
 __global__ void __launch_bounds__(kNrThreads, MODE == kNrAny ? 2 : MODE == kNrWhole ? 5 : 4) norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
   const uint32_t item = blockIdx.x * (kNrThreads / 32) + (threadIdx.x >> 5);

@@ -15,7 +15,7 @@
 // of 40 KB (1.32 GB moved): 220 us = 6.0 TB/s, 210 of them copying, with up to 64
 // CTAs queued per SM (245 us with 8 per SM that loop: their ends do not line up),
 // the same with 8 loads a thread. 4 samples of a short prompt: 7.8 us, 64 of eight
-// long ones (18 MB copied): 12.9 us, both launch latency.
+// long ones (12.6 MB copied): 12.9 us, both launch latency.
 #pragma once
 #include "hkv_common.cuh"
 

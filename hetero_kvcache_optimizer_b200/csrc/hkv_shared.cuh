@@ -39,12 +39,12 @@
 // Measured (65,536 tokens, 8 KV heads, fp16min g32, all SMs, prefix and merge alone):
 // 32 rows 44.3 us, 64 rows 55.3, 128 rows 74.1, 256 rows 127.8 (538 TFLOP/s), of which
 // about 10 us are start and end. The steady state is 1.25 / 1.65 / 2.3 us per tile and
-// SM, bound by none of its resources alone: at 32 rows 4,700 warp instructions (1,180
-// issue slots of 2,350 cycles, K and V's unpacking 2,180 of them), 880 wavefronts of
-// loads and stores beside about 550 of the MMAs' and copies' in shared memory, 530
-// cycles of tcgen05; at 128 rows 9,500 instructions, 1,024 cycles of exponentials,
-// 1,080 of tcgen05. Steps that counted: K through TMEM, one elected thread for the
-// MMAs (57 -> 10 cycles to issue one), one polling warp a role, half-size V code.
+// SM, bound by none of its resources alone: at 32 rows 5,190 warp instructions a tile
+// (the whole launch's over its tiles; about 2,180 unpack K and V), 56 % of the issue
+// slots, 11 % of the tensor pipe and 16 % of shared memory's wavefronts busy (ref, group
+// 32: 7,000 instructions, 54, 8 and 25 %); at 128 rows 8,180, 61, 30 and 32 %. Steps that counted: K through TMEM, one
+// elected thread for the MMAs (57 -> 10 cycles to issue one), one polling warp a role,
+// half-size V code.
 #pragma once
 #include "hkv_prefill.cuh"
 
@@ -761,6 +761,10 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
 // 1.1e-4 to 1.7e-4 of the output in the 2-norm, ref 2e-5 (group 32) to 1e-4 (128; the
 // sums of 1024 + n in fp32); with ref's scale rounded 2.3e-4 to 2.6e-4. Two groups
 // of four consumer warps take every second tile, 32 tokens a warp.
+// Bound by issue and latency of 8 consumer warps an SM (168 registers): 31,680 tokens of
+// 8 heads, 32 rows as two row tiles, fp16min 37 us alone, 3,160 warp instructions a tile,
+// 40 % of the issue slots, 29 % of the tensor pipe (mma.sync), 23 % of shared memory's
+// wavefronts busy; ref (group 32) 47 us, 4,780, 48, 31 and 27 %.
 constexpr int kRowsThreads = 320;  // 8 consumer warps, 2 producers
 constexpr int kRowsSlots = 6;
 constexpr int kRowsPitch = HKV_D + 4;

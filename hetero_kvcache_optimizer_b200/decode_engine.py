@@ -235,7 +235,8 @@ class TieredKVDecoder:
 
     @property
     def launches_per_layer(self) -> int:
-        """Kernel launches of one layer's decode step."""
+        """Kernel launches of one layer's decode step, with at most 8 query heads per
+        KV head; ``norm_rope``'s (steps with positions) comes on top."""
         return 4 if self.prefixes is not None else 1 if self.fused_append else 2
 
     @property
