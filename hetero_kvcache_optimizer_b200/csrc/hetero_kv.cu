@@ -629,11 +629,11 @@ hkv_status shared_plan(const hkv_int4_store* prefix, const int32_t* start, const
   // largest group. 65,536 tokens of 8 heads: 16 rows 35.3 us on shared_rows_kernel (40.1 on a
   // 16-row shared_prefix_kernel; 32 rows there 58.2 against 44.3), 64 rows 55.3 (as 128: 74),
   // 128 rows 74.1, 256 as two row tiles 127.8. Wide products round K, V and P to f16: their
-  // result is 4e-4 to 1.2e-3 off in the 2-norm, which a bf16 output's own 1.7e-3 covers (1.8e-3
-  // to 1.9e-3 in all) and an f16 one's 2.1e-4 does not. f16 and f32 outputs (`exact`) therefore
+  // result is 4e-4 to 1.4e-3 off in the 2-norm, which a bf16 output's own 1.7e-3 covers (1.8e-3
+  // to 2.1e-3 in all) and an f16 one's 2.1e-4 does not. f16 and f32 outputs (`exact`) therefore
   // take row tiles of 16 on shared_rows_kernel (2e-5 to 1.9e-4) at every width: 31,680 tokens of
-  // 8 heads, bf16 against f32 outputs, 32 rows 36-39 and 45 us, 64 rows 48 and 76, 128 rows 60
-  // and 136; 256 rows over 65,536 tokens 172 and 495.
+  // 8 heads, bf16 against f32 outputs, 32 rows 39-40 and 43-45 us, 64 rows 48 and 68-73, 128
+  // rows 60 and 118-128; 256 rows over 65,536 tokens 169 and 406-449 (fp16min g32, ref g64).
   pl.N = rows <= 16 || exact ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
   pl.ns = pl.N == 16 ? 1 : hkv::sh_streams(pl.N);
   const int all = std::min(ctas > 0 ? ctas : device_sms(), 65535);
@@ -656,8 +656,10 @@ hkv_status shared_plan(const hkv_int4_store* prefix, const int32_t* start, const
     if (r == HKV_OK) r = make_plan(B, Hq, Hkv, body, dense, all, &dp);
     if (r != HKV_OK) return r;
     // nanoseconds of one SM: a tile of the prefix (measured, by the rows of its product),
-    // 128 bytes of the own part's schedule (about 36 GB/s per SM, piece starts charged in it)
-    const double mine = hint_steps * (pl.N == 16 ? 900. : pl.N == 32 ? 1050. : pl.N == 64 ? 1500. : 1900.), own = dp.sc.Btot * 3.6;
+    // 128 bytes of the own part's schedule (about 36 GB/s per SM, piece starts charged in it).
+    // 16 rows: 700 against 900 (1,100) for 16 samples of a 32K prompt, f16: 87 and 90 (102) us;
+    // 4 samples: 37.5 and 39.8 (41.5); 19 samples of three prompts 74 and 79 (84)
+    const double mine = hint_steps * (pl.N == 16 ? 700. : pl.N == 32 ? 1050. : pl.N == 64 ? 1500. : 1900.), own = dp.sc.Btot * 3.6;
     pl.C = std::max(1, std::min(all - 1, (int)std::lround(all * mine / (mine + own))));
     pl.own_ctas = std::max(1, all - pl.C);
     if ((r = make_plan(B, Hq, Hkv, body, dense, pl.own_ctas, &dp)) != HKV_OK) return r;

@@ -13,7 +13,7 @@
 // beats it by more than 2^8. K, V and P are rounded to f16, the type of their MMA:
 // K and V where they are dequantised (2^-11 relative; ref's f32 scale enters K as the
 // sum of two f16 and V rounded), P in (0, 2^8]; with key channels ten times as large
-// as the rest that leaves the output 5e-4 (fp16min) to 1.2e-3 (ref) off in the 2-norm,
+// as the rest that leaves the output 4e-4 to 1.4e-3 off in the 2-norm,
 // below the 1.7e-3 of a bf16 output's own rounding; other outputs do not come here.
 //
 // A grid of p.C persistent CTAs; every (group, KV head, row tile) unit's 128-token
