@@ -200,7 +200,7 @@ class TieredKVDecoder:
                 raise ValueError(f"set_rotary needs {self.num_layers} weights, one per layer")
         self._rotary = (table, q_weights, k_weights, eps, adjacent)
         if self.positions is not None:
-            self.graph = self.positions = None
+            self.graph = None
 
     def _ready(self, layer: int, q: torch.Tensor, k_new: torch.Tensor, positions: Optional[torch.Tensor]):
         if positions is None:

@@ -130,7 +130,9 @@ def test_another_rotation_drops_the_step_captured_with_the_old_one(dec):
     dec.set_rotary(torch.zeros(16, 128))
     with pytest.raises(RuntimeError, match="captured"):
         dec.replay()
-    assert dec.positions is None
+    dec._static = (torch.zeros(1),) * 4  # still a step that takes raw queries: not for the host's
+    with pytest.raises(RuntimeError, match="rotated"):
+        dec.capture_host()
 
 
 def test_a_new_capture_drops_the_steps_over_the_buffers_it_replaces(dec, monkeypatch):
