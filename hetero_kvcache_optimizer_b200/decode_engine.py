@@ -67,6 +67,7 @@ class TieredKVDecoder:
         self.prefixes: Optional[List[kv.SharedPrefix]] = None
         self._groups: List[tuple] = []  # per sequence, the group of its slot in each layer's prefix
         self._behind: List[tuple] = []  # ... and the one that its own tokens were computed behind
+        self._mixed: List[int] = []     # sequences for which they differ
         self._nobody: Optional[torch.Tensor] = None
         self._rotary = None
         self.positions: Optional[torch.Tensor] = None
@@ -90,7 +91,7 @@ class TieredKVDecoder:
             d.k[:, :, self.sink:self.sink + nr] = k[:, :, S - nr:]
             d.v[:, :, self.sink:self.sink + nr] = v[:, :, S - nr:]
         nb = S - ns - nr
-        self._behind = list(self._groups)
+        self._set_behind(self._groups)
         if self.pools:  # pages that others share as well must not be written
             self._empty_pool(layer)
             self.pools[layer].reserve(nb)
@@ -105,7 +106,7 @@ class TieredKVDecoder:
     def set_state(self, body_len: int) -> None:
         """Declare that every layer holds ``body_len`` INT4 tokens and a full sink + ring
         (with ``num_pages``, on pages of each sequence's own)."""
-        self._behind = list(self._groups)
+        self._set_behind(self._groups)
         for l, (st, d) in enumerate(zip(self.stores, self.dense)):
             if self.pools:
                 self._empty_pool(l)
@@ -138,15 +139,18 @@ class TieredKVDecoder:
         self.prefixes = prefixes
         self._groups = ([tuple(bisect.bisect_right(p.group_start, b) if b < p.group_start[-1] else 0 for p in prefixes)
                          for b in range(self.batch)] if prefixes is not None else [])
-        self._behind = list(self._groups)
+        self._set_behind(self._groups)
         self.graph = self.host_graph = self._host = None
+
+    def _set_behind(self, groups: List[tuple]) -> None:
+        self._behind = list(groups)
+        self._mixed = [b for b, (x, y) in enumerate(zip(self._behind, self._groups)) if x != y]
 
     def _check_context(self) -> None:
         """A fork moves a sequence's own tokens, not its slot's prefix: attention over
         both would be over a context that no prompt had."""
-        if self.prefixes is not None and self._behind != self._groups:
-            mixed = [b for b in range(self.batch) if self._behind[b] != self._groups[b]]
-            raise RuntimeError(f"sequences {mixed} were forked from another prefix group: their tokens do not follow their "
+        if self._mixed:
+            raise RuntimeError(f"sequences {self._mixed} were forked from another prefix group: their tokens do not follow their "
                                "slot's prefix (fork within groups, fill them anew, or attach_prefix with other groups)")
 
     def reserve(self, tokens: int) -> None:
@@ -175,7 +179,7 @@ class TieredKVDecoder:
             raise ValueError(f"parents must be -1 or lie in [0, {self.batch})")
         if self._groups and not (isinstance(parents, torch.Tensor) and parents.is_cuda):
             old = self._behind
-            self._behind = [old[a] if 0 <= a < self.batch else self._groups[b] for b, a in enumerate(int(x) for x in parents)]
+            self._set_behind([old[a] if 0 <= a < self.batch else self._groups[b] for b, a in enumerate(int(x) for x in parents)])
         at = par.long().clamp(0, self.batch - 1)  # values on the device are not known here
         gone = par != at
         if self.positions is not None:  # of the captured step's next tokens
