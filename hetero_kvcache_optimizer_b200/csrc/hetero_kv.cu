@@ -1406,6 +1406,9 @@ hkv_status hkv_norm_rope(const hkv_rows* q, const hkv_rows* k, const hkv_rows* q
     if (!x.data || !y.data || x.heads <= 0 || x.heads != y.heads) return HKV_ERR_ARG;
     if ((reinterpret_cast<uintptr_t>(x.data) | reinterpret_cast<uintptr_t>(y.data)) & 1u) return HKV_ERR_ARG;
     if ((B > 1 && !y.stride_b) || (y.heads > 1 && !y.stride_h) || (T > 1 && !y.stride_t)) return HKV_ERR_ARG;
+    if (x.data == y.data && ((B > 1 && x.stride_b != y.stride_b) || (y.heads > 1 && x.stride_h != y.stride_h) ||
+                             (T > 1 && x.stride_t != y.stride_t)))
+      return HKV_ERR_ARG;  // in place, but not row by row
     p.x[i] = x.data;
     p.y[i] = y.data;
     p.w[i] = w[i];

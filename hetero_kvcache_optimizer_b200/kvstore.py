@@ -688,7 +688,8 @@ def norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: O
     token each). Rows of a negative position (padding) are not written; one
     behind the table sets DEVERR_BAD_POSITION and is not written either.
     ``table``: f32 [max_pos, rot] of cos | sin (``rope_table``); None: no
-    rotation. ``q_out`` / ``k_out``: where to write, e.g. q and k themselves.
+    rotation. ``q_out`` / ``k_out``: where to write, e.g. q and k themselves
+    (as they are strided; an output must not overlap an input otherwise).
     Either of q and k may be None. Returns (q_out, k_out)."""
     x0 = q if q is not None else k
     if x0 is None:
