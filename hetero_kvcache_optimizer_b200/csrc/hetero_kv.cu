@@ -48,7 +48,9 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // decode kernel (its barrier setup then overlaps the tail of the kernel before
 // it: 2.586 -> 2.561 ms per config-1 step) and for the quantise-pack kernel
 // (a chunked prefill's launches overlap their start with the previous one's
-// drain: 4.82 -> 4.68 ms for config 2's 896 chunk launches); the append kernel,
+// drain: 896 launches of 1,024 tokens 2.61 ms, of 4,096 4.80-4.82. Let in before
+// the wait, as a fused step behind them must not be, they took 3.87 and 4.69);
+// the append kernel,
 // whose blocks would wait resident beside the decode kernel's, measured slower
 // with it (2.608 ms) and launches normally. HKV_PDL (bit mask: 1 decode,
 // 2 append, 4 quantise-pack, 8 norm + rotation and page operations; default 13)
