@@ -633,9 +633,9 @@ hkv_status shared_plan(const hkv_int4_store* prefix, const int32_t* start, const
   // 128 rows 74.1, 256 as two row tiles 127.8. Wide products round K, V and P to f16: their
   // result is 4e-4 to 1.4e-3 off in the 2-norm, which a bf16 output's own 1.7e-3 covers (1.8e-3
   // to 2.1e-3 in all) and an f16 one's 2.1e-4 does not. f16 and f32 outputs (`exact`) therefore
-  // take row tiles of 16 on shared_rows_kernel (2e-5 to 1.9e-4) at every width: 31,680 tokens of
-  // 8 heads, bf16 against f32 outputs, 32 rows 39-40 and 43-45 us, 64 rows 48 and 68-73, 128
-  // rows 60 and 118-128; 256 rows over 65,536 tokens 169 and 406-449 (fp16min g32, ref g64).
+  // take row tiles of 16 on shared_rows_kernel (5e-6 to 1.5e-4) at every width: 31,680 tokens of
+  // 8 heads, bf16 against f32 outputs, 32 rows 36-40 and 43-47 us, 64 rows 48 and 70-75, 128
+  // rows 60 and 124-133; 256 rows over 65,536 tokens 172 and 431-461 (ref g64, fp16min g32).
   pl.N = rows <= 16 || exact ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
   pl.ns = pl.N == 16 ? 1 : hkv::sh_streams(pl.N);
   const int all = std::min(ctas > 0 ? ctas : device_sms(), 65535);
@@ -659,8 +659,8 @@ hkv_status shared_plan(const hkv_int4_store* prefix, const int32_t* start, const
     if (r != HKV_OK) return r;
     // nanoseconds of one SM: a tile of the prefix (measured, by the rows of its product),
     // 128 bytes of the own part's schedule (about 36 GB/s per SM, piece starts charged in it).
-    // 16 rows: 700 against 900 (1,100) for 16 samples of a 32K prompt, f16: 87 and 90 (102) us;
-    // 4 samples: 37.5 and 39.8 (41.5); 19 samples of three prompts 74 and 79 (84)
+    // 16 rows, ref: 700 against 900 (1,100) for 16 samples of a 32K prompt, f16: 83 and 90 (101)
+    // us; 4 samples 42.9 and 43.1 (41.3); 19 samples of three prompts 78.2 and 78.6 (87.9)
     const double mine = hint_steps * (pl.N == 16 ? 700. : pl.N == 32 ? 1050. : pl.N == 64 ? 1500. : 1900.), own = dp.sc.Btot * 3.6;
     pl.C = std::max(1, std::min(all - 1, (int)std::lround(all * mine / (mine + own))));
     pl.own_ctas = std::max(1, all - pl.C);

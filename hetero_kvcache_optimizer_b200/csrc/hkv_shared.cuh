@@ -751,23 +751,28 @@ __global__ void __launch_bounds__(sh_threads(N), 1) shared_prefix_kernel(const _
 //     instruction per pair; the accumulator starts at -1024 sum q, exact as the
 //     products are; the group's scale multiplies in fp32 afterwards; fp16min's mins
 //     are one more product, against sum q_d in f16 high and low parts;
-//   O^T += (n V^T) (s_g P)^T: the codes as exact integers, their scale in P's operand:
-//     fp16min's times P in f16 (2^-11 each), its mins one more product with the same P
-//     into an accumulator of its own; ref's f32 scale times P in fp32, as two f16 and
-//     two products (4 samples of 1,000 tokens, G 7: 17.8 us with it rounded, 17.5 so). The ref
-//     format's zero points enter as z sum q_d and as n - z.
+//   O^T += (n V^T) (s_g P)^T: the codes as exact integers, scale times P as two f16 and
+//     two products (one f16, rounded apart from P's product with the mins, which the codes'
+//     cancels: 2e-4 to 3.9e-4 off in all; the second costs 10 % of fp16min's time and
+//     nothing of ref's): of P in f16 (2^-11) for fp16min, whose mins are one more product
+//     with that P into an accumulator of its own, of P and the scale in fp32 for ref, whose
+//     zero points enter as z sum q_d and as n - z.
 // So nothing of K is rounded, and no operand crosses shared memory twice. Against 64
-// bits, outliers of ten times the rest among the key channels, 1,000 tokens: fp16min
-// 1.1e-4 to 1.7e-4 of the output in the 2-norm, ref 2e-5 (group 32) to 1e-4 (128; the
-// sums of 1024 + n in fp32); with ref's scale rounded 2.3e-4 to 2.6e-4. Two groups
+// bits, outliers of ten times the rest among the key channels: fp16min 5e-5 to 1.2e-4 of
+// the output in the 2-norm, ref 5e-6 to 1.5e-4 (group 128: the sums of 1024 + n in fp32).
+// Two groups
 // of four consumer warps take every second tile, 32 tokens a warp.
 // Bound by issue and latency of 8 consumer warps an SM (168 registers): 31,680 tokens of
-// 8 heads, 32 rows as two row tiles, fp16min 37 us alone, 3,160 warp instructions a tile,
-// 40 % of the issue slots, 29 % of the tensor pipe (mma.sync), 23 % of shared memory's
-// wavefronts busy; ref (group 32) 47 us, 4,780, 48, 31 and 27 %.
+// 8 heads, 32 rows as two row tiles, fp16min 41 us alone, 3,540 warp instructions a tile,
+// 40 % of the issue slots, 38 % of the tensor pipe (mma.sync), 21 % of shared memory's
+// wavefronts busy; ref (group 32) 47 us, 4,750, 48, 31 and 28 %.
 constexpr int kRowsThreads = 320;  // 8 consumer warps, 2 producers
 constexpr int kRowsSlots = 6;
 constexpr int kRowsPitch = HKV_D + 4;
+// P <= 2^4: times a scale it stays below f16's largest for |V| up to 61,000, and P of 2^-14
+// is still a normal f16 (with 2^8, and P / 16 for the first, 15,201 tokens of group 128 were
+// off by 3.9e-4).
+constexpr float kRowsLazy = 4.f;
 constexpr int kRowsSmem = kRowsSlots * kShRawBytes + 16 * 256 + 8 * 16 * kRowsPitch * 4;  // raw slots | query fragments | O per warp
 
 template <int FMT, int GROUP>
@@ -1003,7 +1008,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) shared_rows_kernel(const __gr
             }
           }
         }
-        // ---- softmax: the warp's own running max, moved when a score beats it by 2^8
+        // ---- softmax: the warp's own running max, moved when a score beats it by 2^4
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
@@ -1028,7 +1033,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) shared_rows_kernel(const __gr
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             top[b][e] = fmax3(fmaxf(x[0][b][e], x[0][b][e + 2]), x[1][b][e], x[1][b][e + 2]);
-            need |= top[b][e] > m[b][e] + kPfLazy;
+            need |= top[b][e] > m[b][e] + kRowsLazy;
           }
         if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
@@ -1046,12 +1051,11 @@ __global__ void __launch_bounds__(kRowsThreads, 1) shared_rows_kernel(const __gr
               zc[b][e] *= a, zc[b][e + 2] *= a;
             }
         }
-        // x becomes P / 16 (its f16 stays below the largest); fp16min: in f16, transposed:
-        // row r, tokens 2 j4, 2 j4 + 1 (+ 8)
+        // x becomes P; fp16min: in f16, transposed: row r, tokens 2 j4, 2 j4 + 1 (+ 8)
         uint32_t pt[2][NB][2];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-          const float m0 = m[b][0] + 4.f, m1 = m[b][1] + 4.f;
+          const float m0 = m[b][0], m1 = m[b][1];
 #pragma unroll
           for (int s2 = 0; s2 < 2; ++s2) {
             float* xx = x[s2][b];
@@ -1109,8 +1113,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) shared_rows_kernel(const __gr
             const uint4 c4 = *reinterpret_cast<const uint4*>(blk + HKV_V_CODES_OFF + v_chunk_off(q0 + 4 * e + j4, r));
             vw[e][0] = c4.x, vw[e][1] = c4.y, vw[e][2] = c4.z, vw[e][3] = c4.w;
           }
-          // the codes' other operand, P times the group's scale: fp16min's f16 scale times P as
-          // it meets the mins; ref's f32 scale as two f16, the second what the first leaves
+          // the codes' other operand, P times the group's scale, as two f16, the second what the
+          // first leaves: of P as it meets the mins (fp16min), of the fp32 product (ref)
           uint32_t ph[NB][2], pl[NB][2];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -1122,6 +1126,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) shared_rows_kernel(const __gr
                 for (int e = 0; e < 2; ++e) {
                   if constexpr (FMT == HKV_FMT_FP16MIN) {
                     ph[b][e] = hmul2(pt[s2][b][e], vs[e][g]);
+                    pl[b][e] = h2u(__hfma2(u2h(pt[s2][b][e]), u2h(vs[e][g]), __hneg2(u2h(ph[b][e]))));
                   } else {
                     const float2 y = __fmul2_rn(make_float2(x[s2][b][2 * e], x[s2][b][2 * e + 1]), make_float2(vf[e][g], vf[e][g]));
                     const uint32_t hi = pack2<__half>(y.x, y.y);
@@ -1144,10 +1149,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) shared_rows_kernel(const __gr
             for (int b = 0; b < NB; ++b) {
               mma16816<__half>(o[b][2 * k], a0, ph[b][0], ph[b][1]);
               mma16816<__half>(o[b][2 * k + 1], a1, ph[b][0], ph[b][1]);
-              if constexpr (FMT == HKV_FMT_REF) {
-                mma16816<__half>(o[b][2 * k], a0, pl[b][0], pl[b][1]);
-                mma16816<__half>(o[b][2 * k + 1], a1, pl[b][0], pl[b][1]);
-              }
+              mma16816<__half>(o[b][2 * k], a0, pl[b][0], pl[b][1]);
+              mma16816<__half>(o[b][2 * k + 1], a1, pl[b][0], pl[b][1]);
             }
           }
         }
@@ -1163,7 +1166,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) shared_rows_kernel(const __gr
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int k = 4; k < 32; k <<= 1) l[b][e] += __shfl_xor_sync(0xffffffffu, l[b][e], k);
-        if (r == 0) s_wm[warp][8 * b + 2 * j4 + e] = m[b][e], s_wl[warp][8 * b + 2 * j4 + e] = 16.f * l[b][e];
+        if (r == 0) s_wm[warp][8 * b + 2 * j4 + e] = m[b][e], s_wl[warp][8 * b + 2 * j4 + e] = l[b][e];
         float z[NG];  // fp16min: row g of the mins' product is in lane 4 g + j4
 #pragma unroll
         for (int g = 0; g < NG; ++g) z[g] = FMT == HKV_FMT_FP16MIN ? __shfl_sync(0xffffffffu, zc[b][e], 4 * g + j4) : 0.f;
@@ -1171,8 +1174,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) shared_rows_kernel(const __gr
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float zz = z[16 * i / GROUP];
-          dst[16 * i] = 16.f * (o[b][i][e] + zz);
-          dst[16 * i + 8] = 16.f * (o[b][i][e + 2] + zz);
+          dst[16 * i] = o[b][i][e] + zz;
+          dst[16 * i + 8] = o[b][i][e + 2] + zz;
         }
       }
     }

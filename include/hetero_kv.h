@@ -531,10 +531,10 @@ hkv_status hkv_pages_compact(const hkv_int4_store* src, int32_t B, int32_t H, co
  * Precision: as hkv_decode_attn for the own part. The prefix multiplies on the f16
  * tensor cores (a bf16 query is rounded to f16, |q| < 65504), sums and the softmax
  * statistics in fp32. out_dtype chooses its form: with f16 or f32 outputs the codes
- * of K and V are exact, whatever the number of rows (error against 64 bits 2e-5 to
- * 2e-4 in the 2-norm); with bf16 outputs more than 16 rows multiply dequantised K
+ * of K and V are exact, whatever the number of rows (error against 64 bits 5e-6
+ * to 1.5e-4 in the 2-norm); with bf16 outputs more than 16 rows multiply dequantised K
  * and V (|K|, |V| < 65504) and P as f16, 4e-4 to 1.4e-3, below the output's own
- * rounding of 1.7e-3 and 1.1 to 2.6 times as fast (32 to 256 rows). Three launches on `stream`: prefix and own part side by
+ * rounding of 1.7e-3 and 1.1 to 2.7 times as fast (32 to 256 rows). Three launches on `stream`: prefix and own part side by
  * side, each on a share of the `ctas` (<= 0: one per SM), then the merge. group_len
  * (HOST array of the prefixes' lengths as far as known; NULL: prefix->len for each)
  * and the len fields of body and dense size the shares; device lengths may exceed

@@ -51,9 +51,9 @@ def test_scales_between_two_f16_numbers(rows, group, dtype):
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_one_token_returns_its_value(rows, group):
     """One token: P = 1, so the output is code times scale. With at most 16 rows the codes
-    are exact and P / 16 times the scale is two f16. The second is a multiple of 2^-24 at
+    are exact and P times the scale is two f16. The second is a multiple of 2^-24 at
     the finest and 2^-11 of the first at most, so what is left is 2^-25 or 2^-22 of the
-    scale / 16, whichever is more; that times 16 and code - zero, and fp32: 2^-21 + 2^-21."""
+    scale, whichever is more; that times code - zero, and fp32: 2^-21 + 2^-21."""
     from hetero_kvcache_optimizer_b200 import kvstore as kv
     ng = 128 // group
     gen = torch.Generator(device="cuda").manual_seed(rows)
@@ -68,4 +68,29 @@ def test_one_token_returns_its_value(rows, group):
     out = kv.decode_shared(q, kv.SharedPrefix(store, [0, rows])).double()
     n = codes[0, 0, 0].view(ng, group).double() - zero.double()[:, None]
     ref = (n * scale.double()[:, None]).view(128)
-    assert ((out - ref).abs() - 2.0 ** -20 * ref.abs() - 16 * 2.0 ** -25 * n.abs().view(128)).max().item() <= 0
+    assert ((out - ref).abs() - 2.0 ** -20 * ref.abs() - 2.0 ** -25 * n.abs().view(128)).max().item() <= 0
+
+
+@pytest.mark.parametrize("rows", [2, 16, 40])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_codes_and_mins_cancel(rows, group):
+    """fp16min values that are zero as 15 scale + min: the codes' products and the mins' are
+    both 15 scale P and cancel if both see the same P. Left are fp32 sums (four steps of
+    2^-23 on either side: 2^-20 of 15 scale) and what the second f16 of scale times P cannot
+    hold, 2^-25 a token times its code, over a sum of P of at least 1."""
+    from hetero_kvcache_optimizer_b200 import kvstore as kv
+    T, ng = 20, 128 // group
+    gen = torch.Generator(device="cuda").manual_seed(group + rows)
+    scale = torch.randint(40, 128, (T, ng), generator=gen, device="cuda").double() * 2.0 ** -8
+    v = torch.zeros(T, ng, group, dtype=torch.float64, device="cuda")
+    v[:, :, 0] = -15 * scale  # exact in f16: 15 * 127 < 2^11
+    k = torch.randn(T, 128, generator=gen, device="cuda")
+    store = kv.Int4KVStore(1, 1, 128, fmt="fp16min", group=group, page_tokens=128)
+    kv.quantize_pack_kv(k.to(F16).view(1, 1, T, 128), v.to(F16).view(1, 1, T, 128), store)
+    store.set_lengths(T)
+    back = kv.dequantize_pack(store, 1, 0, T, dtype=torch.float32)[0, 0].view(T, ng, group)
+    assert bool((back[:, :, 1:] == 0).all()) and bool((back.double() == v).all())
+    q = torch.randn(rows, 1, 128, generator=gen, device="cuda").to(F16)
+    out = kv.decode_shared(q, kv.SharedPrefix(store, [0, rows])).view(rows, ng, group)
+    bound = 15 * (scale.max().item() * 2.0 ** -20 + T * 2.0 ** -25)
+    assert out[:, :, 1:].abs().max().item() <= bound
